@@ -246,6 +246,120 @@ int ormi_b200_comm_destroy(ormi_b200_ctx* ctx);
  * Results are deterministic; they differ from ormi_b200_sum only by fp32 summation order. */
 int ormi_b200_colsum_static(const float* in, int64_t rows, int64_t cols, float* out, void* stream);
 
+/* ------------------------------------------------------------------ transformer-block operators -- */
+
+/* Operators on raw device buffers beside ormi_b200_sum, ormi_b200_matmul and ormi_b200_gemm_bf16 (the reference has none
+ * of them: ormi-core/csrc/core/ops.h:4-10 ends at pointwise ops, MATMUL, SUM and views).  Rules they share:
+ *   - work is queued on the context's compute stream and the call returns at once.  A buffer that another stream fills or
+ *     reads is ordered by the caller (events against ormi_b200_stream);
+ *   - arguments are checked before the context is looked at and before anything is queued: a refused call has written
+ *     nothing;
+ *   - scratch comes from the context's pool, so the calls may be captured (ormi_b200_capture_begin) after one plain run;
+ *   - buffers live on the context's device; an output may overlap an input only where its description says so;
+ *   - results are bit-identical run to run (no atomics on values). */
+enum ormi_b200_dtype { ORMI_F32 = 0, ORMI_BF16 = 1, ORMI_E4M3 = 2, ORMI_I32 = 3 };
+
+/* A strided view of device memory; strides in elements, never negative.  data == NULL: the argument is left out. */
+typedef struct ormi_b200_view {
+    void*   data;
+    int32_t dtype;                         /* enum ormi_b200_dtype */
+    int32_t ndim;                          /* 1..4 */
+    int64_t shape[4];
+    int64_t strides[4];
+} ormi_b200_view;
+
+/* Root-mean-square norm of the last dimension, with the residual's addition in front of it:
+ *     s = x + residual            (rounded to x's type, stored to residual_out when given)
+ *     rstd = 1 / sqrt(mean(s^2) + eps),    out = s * rstd * weight
+ * x, residual, residual_out: F32 or BF16, one type, same shape; leading dimensions that do not collapse into one row
+ * stride are refused.  weight: [cols], F32 or BF16, or left out (ones).  out: F32, BF16 or E4M3.  rstd: [rows] F32,
+ * optional (the backward pass reads it).  With an E4M3 `out`, scales is [rows, groups] F32, contiguous: group = 0 is one
+ * scale for the row, group = 128 one for every 128 columns; scale = max|y| / 448 and out = round(y * (448 / max|y|)), zero
+ * for a group of zeros.  out may be x or residual in place; residual_out may be x or residual. */
+typedef struct ormi_b200_rmsnorm_args {
+    ormi_b200_view x, residual, weight, out, residual_out, rstd, scales;
+    int32_t group;
+    float   eps;
+} ormi_b200_rmsnorm_args;
+int ormi_b200_rmsnorm(ormi_b200_ctx* ctx, const ormi_b200_rmsnorm_args* args);
+
+/* Its backward pass.  s is residual_out of the forward call (x itself when there was no residual):
+ *     dx = rstd * (dout * weight - s * rstd^2 * mean(dout * weight * s)) + dresidual
+ *     dweight = sum over rows of dout * s * rstd
+ * dx is the gradient of x and of residual alike.  dresidual (optional): the gradient that reaches s past the norm.  dweight
+ * (optional): [cols], weight's type (F32 or BF16).  dout, s, dresidual, dx: one type, F32 or BF16.  dx may be dout or
+ * dresidual in place. */
+typedef struct ormi_b200_rmsnorm_backward_args {
+    ormi_b200_view dout, s, weight, rstd, dresidual, dx, dweight;
+} ormi_b200_rmsnorm_backward_args;
+int ormi_b200_rmsnorm_backward(ormi_b200_ctx* ctx, const ormi_b200_rmsnorm_backward_args* args);
+
+/* Softmax attention over [batch, length, heads, head_dim] views (head_dim contiguous, at most 256; any other strides):
+ *     z = scale * q.k;   cap > 0: z = cap * tanh(z / cap);   slopes: z -= slopes[head] * |pos - j|
+ *     out = softmax over the visible keys j of z, times v;   lse = log(sum of exp(z))
+ * Key j is visible to the query at position pos when all of these hold:
+ *     j < key_len[batch]                            (key_len left out: every key; what lies behind it is never used)
+ *     not causal, or j <= pos, or j < prefix[batch] (prefix left out: 0)
+ *     q_docs[batch, query] == k_docs[batch, j]      (left out: one document)
+ * pos = q_start[batch] + query; q_start left out: k_len - q_len, the last q_len positions.  A query that sees no key
+ * gets out = 0 and lse = -infinity (and zero gradients).  Keys and values inside key_len have to be finite where a
+ * query of the same call sees them or not; behind key_len they may hold anything.
+ * heads is a multiple of kv_heads: query head h reads key/value head h / (heads / kv_heads).
+ * q, k, v, out: one type, F32 or BF16.  lse: [batch, heads, q_len] F32, contiguous, optional.  slopes: [heads] F32.
+ * q_docs [batch, q_len], k_docs [batch, k_len], prefix, key_len, q_start [batch]: I32, contiguous, on the device. */
+typedef struct ormi_b200_attention_args {
+    ormi_b200_view q, k, v, out, lse;
+    ormi_b200_view slopes, q_docs, k_docs, prefix, key_len, q_start;
+    float   scale;
+    float   cap;                           /* 0: no cap */
+    int32_t causal;
+} ormi_b200_attention_args;
+int ormi_b200_attention(ormi_b200_ctx* ctx, const ormi_b200_attention_args* args);
+
+/* Its backward pass: dq, dk, dv from dout and the forward call's arguments, `out` and `lse` (required here) as the
+ * forward call wrote them.  dk and dv of a shared head are the sums over its query heads; keys nobody sees get zero.
+ * dq, dk, dv: q's type, the shapes of q, k, v.  Slopes, cap and scale are constants. */
+typedef struct ormi_b200_attention_backward_args {
+    ormi_b200_attention_args forward;
+    ormi_b200_view dout, dq, dk, dv;
+} ormi_b200_attention_backward_args;
+int ormi_b200_attention_backward(ormi_b200_ctx* ctx, const ormi_b200_attention_backward_args* args);
+
+/* One AdamW step over many tensors, in place (`step` counts from 1):
+ *     g = grad * grad_scale;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *     param -= lr * weight_decay * param + lr * (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps)
+ * param: n fp32 values.  grad: F32 or BF16.  copy16 (optional): n bf16 values, the new parameters rounded.  A bf16 copy
+ * that the context keeps of `param` for its matmuls ("matmul" = "bf16") is rewritten along with it.
+ * state_bits = 32: m and v are fp32.  state_bits = 8: m holds e4m3 codes of m, v holds e4m3 codes of sqrt(v), both n bytes,
+ * with one fp32 scale for every 128 elements in m_scales / v_scales (ceil(n / 128) each; value = code * scale, scale =
+ * largest magnitude of the block / 448).  Codes are rounded up or down at random in proportion to the distance (a state
+ * that moves by less than half a step would otherwise stand still), with bits hashed from (seed, step, tensor, element);
+ * a positive sqrt(v) never becomes zero.  All-zero codes and scales are the initial state.
+ * device_step (optional, for captured steps): a device counter of the steps done so far; the call takes *device_step + 1
+ * as its step and adds one.  device_lr, grad_scale (optional): device floats, read when the kernel runs. */
+typedef struct ormi_b200_adamw_tensor {
+    void*   param;
+    const void* grad;
+    void*   m;
+    void*   v;
+    void*   m_scales;
+    void*   v_scales;
+    void*   copy16;
+    int64_t n;
+    int32_t grad_dtype;                    /* ORMI_F32 or ORMI_BF16 */
+    float   weight_decay;
+} ormi_b200_adamw_tensor;
+typedef struct ormi_b200_adamw_config {
+    double  lr, beta1, beta2, eps;
+    int64_t step;
+    int64_t* device_step;
+    const float* device_lr;
+    const float* grad_scale;
+    uint32_t seed;
+    int32_t state_bits;
+} ormi_b200_adamw_config;
+int ormi_b200_adamw(ormi_b200_ctx* ctx, const ormi_b200_adamw_tensor* tensors, int n_tensors, const ormi_b200_adamw_config* config);
+
 /* ------------------------------------------------------------------ options, counters -- */
 
 /* Self-test of the device-side bounded waits (no counterpart in the reference): queues a one-warp kernel that waits on a

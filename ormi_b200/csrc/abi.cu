@@ -3,6 +3,7 @@
 #include <cstring>
 
 #include "context.h"
+#include "operators.h"
 #include "ormi_b200.h"
 
 using namespace ormi_b200;
@@ -387,6 +388,57 @@ int ormi_b200_gemm_bf16(ormi_b200_ctx* ctx, const void* a16, int a_transposed, c
     });
 }
 
+// ------------------------------------------------------------------------------------------------ transformer-block operators
+// the Python binding packs these by hand (ormi_b200/ops.py)
+static_assert(sizeof(ormi_b200_view) == 80 && sizeof(ormi_b200_rmsnorm_args) == 568 && sizeof(ormi_b200_rmsnorm_backward_args) == 560 &&
+              sizeof(ormi_b200_attention_args) == 896 && sizeof(ormi_b200_attention_backward_args) == 1216 && sizeof(ormi_b200_adamw_tensor) == 72 &&
+              sizeof(ormi_b200_adamw_config) == 72, "operator argument layout");
+
+int ormi_b200_rmsnorm(ormi_b200_ctx* ctx, const ormi_b200_rmsnorm_args* args) {
+    return guarded([&] {
+        need(args, "ormi_b200_rmsnorm: args is NULL");
+        rmsnorm_check(*args);
+        bind(ctx, "ormi_b200_rmsnorm", true);
+        rmsnorm(ctx, *args);
+    });
+}
+
+int ormi_b200_rmsnorm_backward(ormi_b200_ctx* ctx, const ormi_b200_rmsnorm_backward_args* args) {
+    return guarded([&] {
+        need(args, "ormi_b200_rmsnorm_backward: args is NULL");
+        rmsnorm_backward_check(*args);
+        bind(ctx, "ormi_b200_rmsnorm_backward", true);
+        rmsnorm_backward(ctx, *args);
+    });
+}
+
+int ormi_b200_attention(ormi_b200_ctx* ctx, const ormi_b200_attention_args* args) {
+    return guarded([&] {
+        need(args, "ormi_b200_attention: args is NULL");
+        attention_check(*args);
+        bind(ctx, "ormi_b200_attention", true);
+        attention(ctx, *args);
+    });
+}
+
+int ormi_b200_attention_backward(ormi_b200_ctx* ctx, const ormi_b200_attention_backward_args* args) {
+    return guarded([&] {
+        need(args, "ormi_b200_attention_backward: args is NULL");
+        attention_backward_check(*args);
+        bind(ctx, "ormi_b200_attention_backward", true);
+        attention_backward(ctx, *args);
+    });
+}
+
+int ormi_b200_adamw(ormi_b200_ctx* ctx, const ormi_b200_adamw_tensor* tensors, int n_tensors, const ormi_b200_adamw_config* config) {
+    return guarded([&] {
+        need(config && n_tensors >= 0 && (tensors || n_tensors == 0), "ormi_b200_adamw: bad arguments");
+        adamw_check(tensors, n_tensors, *config);
+        bind(ctx, "ormi_b200_adamw", true);
+        adamw(ctx, tensors, n_tensors, *config);
+    });
+}
+
 int ormi_b200_comm_unique_id(char id[128]) {
     return guarded([&] { need(id != nullptr, "ormi_b200_comm_unique_id: NULL argument"); comm_unique_id(id); });
 }
@@ -476,6 +528,7 @@ struct CapturedStep {
     cudaGraph_t graph = nullptr;
     cudaGraphExec_t exec = nullptr;
     std::vector<std::pair<void*, size_t>> blocks;      // every pool block the step touched: owned until the graph is destroyed
+    std::vector<std::pair<const void*, size_t>> writes;   // caller-owned memory that a replay writes
 };
 
 int ormi_b200_capture_begin(ormi_b200_ctx* ctx) {
@@ -487,6 +540,7 @@ int ormi_b200_capture_begin(ormi_b200_ctx* ctx) {
         check_gemm_error(ctx);
         ORMI_CUDA(cudaStreamBeginCapture(ctx->stream, cudaStreamCaptureModeThreadLocal));
         ctx->capture_blocks.clear();
+        ctx->capture_writes.clear();
         ctx->capturing = true;
     });
 }
@@ -519,6 +573,8 @@ int ormi_b200_capture_end(ormi_b200_ctx* ctx, void** out_graph) {
             }
         }
         ctx->capture_blocks.clear();
+        step->writes.swap(ctx->capture_writes);
+        ctx->capture_writes.clear();
         ctx->counters["captured_steps"]++;
         *out_graph = step.release();
     });
@@ -529,6 +585,7 @@ int ormi_b200_graph_launch(ormi_b200_ctx* ctx, void* graph) {
         bind(ctx, "ormi_b200_graph_launch");
         if (!graph) throw Error("ormi_b200_graph_launch: NULL graph");
         ORMI_CUDA(cudaGraphLaunch(((CapturedStep*)graph)->exec, ctx->stream));
+        for (auto& w : ((CapturedStep*)graph)->writes) shadow_drop(ctx, w.first, w.second);
         ctx->gemm_err_pending = true;
         ctx->counters["graph_launches"]++;
     });

@@ -1,0 +1,286 @@
+// AdamW over many tensors in one launch, with states in 32 bits or in 8.
+//
+//   g = grad * gs;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+//   p -= lr wd p + lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
+//
+// Bound by memory: 28 bytes per parameter with fp32 gradients and states, 16 with 8-bit states.  The tensors' descriptors
+// travel as kernel parameters (no copy to the device, so a call can be captured); a block takes a chunk of one tensor and
+// finds it by binary search over the running chunk counts.
+//
+// 8-bit states: e4m3 codes of m and of sqrt(v) (the root halves the exponent range: 2^17.8 of a block's codes span 2^35 of
+// v), one fp32 scale per 128 elements.  An update moves sqrt(v) by a fraction of a per cent, far less than half a step of a
+// 3-bit mantissa (6 %): rounding to nearest would freeze the state, so codes are rounded up with the probability of
+// what they are above the code below (unbiased), from 16 bits each of a 32-bit hash.  A code depends on the last bits of
+// m and v, so these are computed operation by operation (no contraction into FMAs): the formulas evaluated in fp32 in their
+// written order give the same codes on any machine.
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "op_math.cuh"
+#include "operators.h"
+
+namespace ormi_b200 {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kChunk = 4096;                 // elements per block: 32 blocks of 128 that share a scale
+
+struct Tensor {
+    float* param;
+    const void* grad;
+    void *m, *v;
+    float *m_scales, *v_scales;
+    bf16* copy16;
+    int64_t n;
+    float decay;
+    int first_chunk;                          // running count of chunks before this tensor
+    int index;                                // position in the caller's list (part of the rounding hash)
+    uint8_t grad_f32, vec;                    // vec: every pointer allows 4-element accesses
+};
+struct Common {
+    float b1, b2, c1, c2, eps, lr, inv_bc1, inv_sqrt_bc2;      // c1 = 1 - b1, c2 = 1 - b2
+    double b1_d, b2_d;
+    const float* device_lr;
+    const float* grad_scale;
+    const int64_t* device_step;
+    int64_t step;
+    uint32_t seed;
+    int n;
+};
+template <int N> struct Batch { Common c; Tensor t[N]; };
+
+// Two rounds of xor-shift and multiply (Wellons' "lowbias32" constants): every input bit reaches every output bit.
+__host__ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
+    x ^= x >> 16; x *= 0x7feb352du;
+    x ^= x >> 15; x *= 0x846ca68bu;
+    return x ^ (x >> 16);
+}
+
+// 0 <= a <= 448 to an e4m3 value, up with the probability of the remainder; u in [0, 1).  The step below 2^-6 is 2^-9.
+__device__ __forceinline__ float to_e4m3_grid(float a, float u) {
+    const uint32_t e = max(__float_as_uint(a) >> 23, 121u);                   // biased exponent, at least that of 2^-6
+    const float step = __uint_as_float((e - 3u) << 23), inv = __uint_as_float((257u - e) << 23);
+    return fminf(floorf(a * inv + u) * step, 448.f);
+}
+
+__device__ __forceinline__ float codes_per_unit(float top) { return top > 0.f ? __fmul_rn(1.f / top, 448.f) : 0.f; }
+
+struct Rates { float lr, inv_bc1, inv_sqrt_bc2, gs; uint32_t key; };
+
+// The step number and what follows from it: from the host, or from the device counter of a captured step.
+__device__ __forceinline__ Rates rates_of(const Common& c) {
+    Rates r{c.lr, c.inv_bc1, c.inv_sqrt_bc2, 1.f, 0};
+    int64_t step = c.step;
+    if (c.device_step) {
+        step = *c.device_step + 1;
+        r.inv_bc1 = 1.f / (float)(1.0 - pow(c.b1_d, (double)step));
+        r.inv_sqrt_bc2 = (float)(1.0 / sqrt(1.0 - pow(c.b2_d, (double)step)));
+    }
+    if (c.device_lr) r.lr = *c.device_lr;
+    if (c.grad_scale) r.gs = *c.grad_scale;
+    r.key = mix32(c.seed ^ (uint32_t)step);
+    return r;
+}
+
+// b1 m + c1 g and b2 v + (c2 g) g, each operation rounded by itself
+__device__ __forceinline__ float next_m(const Common& c, float m, float g) { return __fadd_rn(__fmul_rn(c.b1, m), __fmul_rn(c.c1, g)); }
+__device__ __forceinline__ float next_v(const Common& c, float v, float g) { return __fadd_rn(__fmul_rn(c.b2, v), __fmul_rn(__fmul_rn(c.c2, g), g)); }
+
+__device__ __forceinline__ float updated(float p, float m, float v, float decay, const Rates& r, float eps) {
+    return p - (r.lr * decay * p + r.lr * (m * r.inv_bc1) / (sqrtf(v) * r.inv_sqrt_bc2 + eps));
+}
+
+template <int N> __device__ __forceinline__ const Tensor& tensor_of(const Batch<N>& b, int chunk) {
+    int lo = 0, hi = b.c.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (b.t[mid].first_chunk <= chunk) lo = mid; else hi = mid - 1;
+    }
+    return b.t[lo];
+}
+
+// States in 32 bits, any alignment.
+template <int N>
+__global__ void __launch_bounds__(kThreads) adamw_f32(const __grid_constant__ Batch<N> b) {
+    __shared__ Rates shared_rates;
+    if (threadIdx.x == 0) shared_rates = rates_of(b.c);
+    __syncthreads();
+    const Rates r = shared_rates;
+    const Tensor& t = tensor_of(b, blockIdx.x);
+    const int64_t base = (int64_t)((int)blockIdx.x - t.first_chunk) * kChunk, end = min(base + kChunk, t.n);
+    float* pm = (float*)t.m;
+    float* pv = (float*)t.v;
+    for (int64_t i = base + threadIdx.x; i < end; i += kThreads) {
+        const float g = (t.grad_f32 ? ((const float*)t.grad)[i] : __bfloat162float(((const bf16*)t.grad)[i])) * r.gs;
+        const float m = next_m(b.c, pm[i], g), v = next_v(b.c, pv[i], g);
+        const float p = updated(t.param[i], m, v, t.decay, r, b.c.eps);
+        pm[i] = m; pv[i] = v; t.param[i] = p;
+        if (t.copy16) t.copy16[i] = __float2bfloat16_rn(p);
+    }
+}
+
+// States in 8 bits: a warp owns the 128 elements that share a scale, 4 per lane, 32 apart.
+template <int N>
+__global__ void __launch_bounds__(kThreads) adamw_e4m3(const __grid_constant__ Batch<N> b) {
+    __shared__ Rates shared_rates;
+    if (threadIdx.x == 0) shared_rates = rates_of(b.c);
+    __syncthreads();
+    const Rates r = shared_rates;
+    const Tensor& t = tensor_of(b, blockIdx.x);
+    const int64_t base = (int64_t)((int)blockIdx.x - t.first_chunk) * kChunk, end = min(base + kChunk, t.n);
+    const uint32_t key = mix32(r.key + (uint32_t)t.index);
+    const int lane = threadIdx.x & 31;
+    e4m3* cm = (e4m3*)t.m;
+    e4m3* cv = (e4m3*)t.v;
+    for (int64_t first = base + (threadIdx.x >> 5) * 128; first < end; first += kThreads / 32 * 128) {
+        const float sm = t.m_scales[first >> 7], sv = t.v_scales[first >> 7];
+        float m[4], root[4];
+        uint32_t top_m = 0, top_v = 0;
+        for (int k = 0; k < 4; ++k) {
+            const int64_t i = first + k * 32 + lane;
+            m[k] = root[k] = 0.f;
+            if (i >= end) continue;
+            const float g = (t.grad_f32 ? ((const float*)t.grad)[i] : __bfloat162float(((const bf16*)t.grad)[i])) * r.gs;
+            const float old = __fmul_rn(float(cv[i]), sv);
+            m[k] = next_m(b.c, __fmul_rn(float(cm[i]), sm), g);
+            const float v = next_v(b.c, __fmul_rn(old, old), g);
+            const float p = updated(t.param[i], m[k], v, t.decay, r, b.c.eps);
+            t.param[i] = p;
+            if (t.copy16) t.copy16[i] = __float2bfloat16_rn(p);
+            root[k] = sqrtf(v);
+            top_m = max(top_m, mag(m[k]));
+            top_v = max(top_v, mag(root[k]));
+        }
+        const float hi_m = __uint_as_float(__reduce_max_sync(0xffffffffu, top_m)), hi_v = __uint_as_float(__reduce_max_sync(0xffffffffu, top_v));
+        const float up_m = codes_per_unit(hi_m), up_v = codes_per_unit(hi_v);
+        for (int k = 0; k < 4; ++k) {
+            const int64_t i = first + k * 32 + lane;
+            if (i >= end) continue;
+            const uint32_t h = mix32((uint32_t)i ^ key);
+            const float a = fminf(__fmul_rn(fabsf(m[k]), up_m), 448.f), c = fminf(__fmul_rn(root[k], up_v), 448.f);
+            const float qm = to_e4m3_grid(a, (float)(h & 0xffffu) * (1.f / 65536.f));
+            const float qv = to_e4m3_grid(root[k] > 0.f ? fmaxf(c, 0x1p-9f) : 0.f, (float)(h >> 16) * (1.f / 65536.f));
+            cm[i] = from_f32<e4m3>(copysignf(qm, m[k]));
+            cv[i] = from_f32<e4m3>(qv);
+        }
+        if (lane == 0) { t.m_scales[first >> 7] = hi_m * (1.f / 448.f); t.v_scales[first >> 7] = hi_v * (1.f / 448.f); }
+    }
+}
+
+__global__ void count_step(int64_t* step) { ++*step; }
+
+template <int N>
+void launch(ormi_b200_ctx* ctx, Batch<N>& b, int chunks, int state_bits) {
+    if (state_bits == 32) adamw_f32<N><<<chunks, kThreads, 0, ctx->stream>>>(b);
+    else adamw_e4m3<N><<<chunks, kThreads, 0, ctx->stream>>>(b);
+    ORMI_CUDA(cudaGetLastError());
+    count_launch(ctx);
+}
+
+// The context's bf16 copy of `param` when it is a plain copy of exactly these n values (it is rewritten along with them);
+// any other copy that overlaps is stale and goes.  A captured step keeps rewriting the copy on every replay, so the
+// copy's block stays with the graph.
+void* kept_copy(ormi_b200_ctx* ctx, const ormi_b200_adamw_tensor& t) {
+    if (ctx->shadows.empty()) return nullptr;
+    auto it = ctx->shadows.find(t.param);
+    const bool whole = it != ctx->shadows.end() && it->second.ld == it->second.cols && (int64_t)it->second.rows * it->second.cols == t.n;
+    if (!whole || t.copy16) { shadow_drop(ctx, t.param, (size_t)t.n * 4); return nullptr; }
+    const Shadow16 keep = it->second;
+    ctx->shadows.erase(it);
+    shadow_drop(ctx, t.param, (size_t)t.n * 4);
+    ctx->shadows[t.param] = keep;
+    if (ctx->capturing) ctx->capture_blocks[keep.ptr] = keep.bytes;
+    return keep.ptr;
+}
+
+}  // namespace
+
+void adamw_check(const ormi_b200_adamw_tensor* t, int n, const ormi_b200_adamw_config& c) {
+    const char* op = "adamw";
+    op_need(c.state_bits == 32 || c.state_bits == 8, op, "state_bits is 32 or 8");
+    op_need(c.device_step || c.step >= 1, op, "step counts from 1");
+    op_need(c.beta1 >= 0 && c.beta1 < 1 && c.beta2 >= 0 && c.beta2 < 1, op, "beta1 and beta2 lie in [0, 1)");
+    op_need(c.eps >= 0 && std::isfinite(c.eps), op, "eps is negative or not finite");
+    op_need(std::isfinite(c.lr), op, "lr is not finite");
+    op_need((uintptr_t)c.device_step % 8 == 0 && (uintptr_t)c.device_lr % 4 == 0 && (uintptr_t)c.grad_scale % 4 == 0, op, "a device scalar does not start on a whole element");
+    struct Range { const char* lo; const char* hi; bool out; int tensor; };
+    std::vector<Range> ranges;
+    for (int i = 0; i < n; ++i) {
+        const ormi_b200_adamw_tensor& x = t[i];
+        const std::string who = "tensor " + std::to_string(i) + ": ";
+        op_need(x.n >= 0 && x.n < (int64_t)1 << 40, op, who + "n is negative or above 2^40");
+        if (x.n == 0) continue;
+        op_need(x.param && x.grad && x.m && x.v, op, who + "param, grad, m and v are needed");
+        op_need(x.grad_dtype == ORMI_F32 || x.grad_dtype == ORMI_BF16, op, who + "grad is F32 or BF16");
+        op_need(std::isfinite(x.weight_decay), op, who + "weight_decay is not finite");
+        op_need((x.m_scales && x.v_scales) == (c.state_bits == 8) && (c.state_bits == 8 || (!x.m_scales && !x.v_scales)), op, who + "m_scales and v_scales go with 8-bit states, and only with them");
+        const uintptr_t state = c.state_bits == 32 ? 4 : 1;
+        op_need((uintptr_t)x.param % 4 == 0 && (uintptr_t)x.grad % dtype_bytes(x.grad_dtype) == 0 && (uintptr_t)x.m % state == 0 && (uintptr_t)x.v % state == 0 &&
+                (uintptr_t)x.m_scales % 4 == 0 && (uintptr_t)x.v_scales % 4 == 0 && (uintptr_t)x.copy16 % 2 == 0, op, who + "a buffer does not start on a whole element");
+        auto add = [&](const void* p, int64_t bytes, bool out) { if (p) ranges.push_back({(const char*)p, (const char*)p + bytes, out, i}); };
+        add(x.param, x.n * 4, true); add(x.grad, x.n * dtype_bytes(x.grad_dtype), false);
+        add(x.m, x.n * (int64_t)state, true); add(x.v, x.n * (int64_t)state, true);
+        add(x.m_scales, (x.n + 127) / 128 * 4, true); add(x.v_scales, (x.n + 127) / 128 * 4, true);
+        add(x.copy16, x.n * 2, true);
+    }
+    // what is written lies apart from everything else (the same tensor twice would be updated by two blocks at once)
+    std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.lo < b.lo; });
+    const char* end_any = nullptr; const char* end_out = nullptr;
+    for (const Range& r : ranges) {
+        op_need(!(r.lo < end_out || (r.out && r.lo < end_any)), op, "tensor " + std::to_string(r.tensor) + ": a buffer that is written overlaps another one");
+        end_any = std::max(end_any, r.hi);
+        if (r.out) end_out = std::max(end_out, r.hi);
+    }
+}
+
+void adamw(ormi_b200_ctx* ctx, const ormi_b200_adamw_tensor* t, int n, const ormi_b200_adamw_config& c) {
+    Common common{};
+    common.b1 = (float)c.beta1; common.b2 = (float)c.beta2; common.c1 = (float)(1.0 - c.beta1); common.c2 = (float)(1.0 - c.beta2);
+    common.b1_d = c.beta1; common.b2_d = c.beta2;
+    common.eps = (float)c.eps; common.lr = (float)c.lr;
+    if (!c.device_step) {
+        common.inv_bc1 = 1.f / (float)(1.0 - std::pow(c.beta1, (double)c.step));
+        common.inv_sqrt_bc2 = (float)(1.0 / std::sqrt(1.0 - std::pow(c.beta2, (double)c.step)));
+    }
+    common.device_lr = c.device_lr; common.grad_scale = c.grad_scale; common.device_step = c.device_step;
+    common.step = c.step; common.seed = c.seed;
+    // 44 descriptors fit the classic 4 KB of kernel parameters; more tensors go 300 at a time (24 KB)
+    auto run = [&](auto batch) {
+        constexpr int cap = sizeof(batch.t) / sizeof(Tensor);
+        int i = 0;
+        while (i < n) {
+            batch.c = common;
+            int64_t chunks = 0;
+            int k = 0;
+            for (; i < n && k < cap; ++i) {
+                const ormi_b200_adamw_tensor& x = t[i];
+                if (x.n == 0) continue;
+                const int64_t mine = (x.n + kChunk - 1) / kChunk;
+                if (chunks + mine > 0x7fffffff) break;
+                Tensor& d = batch.t[k++];
+                d.param = (float*)x.param; d.grad = x.grad; d.m = x.m; d.v = x.v;
+                d.m_scales = (float*)x.m_scales; d.v_scales = (float*)x.v_scales;
+                void* kept = kept_copy(ctx, x);
+                d.copy16 = (bf16*)(x.copy16 ? x.copy16 : kept);
+                d.n = x.n; d.decay = x.weight_decay; d.first_chunk = (int)chunks; d.index = i;
+                d.grad_f32 = x.grad_dtype == ORMI_F32;
+                chunks += mine;
+                auto note = [&](void* p, size_t bytes) { written(ctx, p, bytes); };
+                if (c.state_bits == 32) { note(x.m, (size_t)x.n * 4); note(x.v, (size_t)x.n * 4); }
+                if (ctx->capturing) ctx->capture_writes.push_back({x.param, (size_t)x.n * 4});
+            }
+            if (!k) break;
+            batch.c.n = k;
+            launch(ctx, batch, (int)chunks, c.state_bits);
+        }
+    };
+    if (n <= 44) run(Batch<44>{}); else run(Batch<300>{});
+    if (c.device_step) {
+        count_step<<<1, 1, 0, ctx->stream>>>(c.device_step);
+        ORMI_CUDA(cudaGetLastError());
+        count_launch(ctx);
+    }
+}
+
+}  // namespace ormi_b200

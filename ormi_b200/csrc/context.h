@@ -111,6 +111,7 @@ struct ormi_b200_ctx {
     bool capturing = false;
     std::unordered_map<void*, size_t> capture_blocks;
     std::unordered_set<void*> graph_owned;
+    std::vector<std::pair<const void*, size_t>> capture_writes;   // caller-owned memory the captured operators write: bf16 copies of it are stale after a replay
     bool pool_canary = false;              // option "pool_canary": a guard zone behind every block, checked when the block comes back
     std::unordered_map<void*, size_t> canaries;   // block -> bytes asked for, of the blocks that carry a guard zone
     std::unordered_set<void*> pooled;      // every block that sits in free_blocks: a block returned twice is caught, not handed to two owners
