@@ -11,7 +11,7 @@
 #include <cmath>
 #include <vector>
 
-#include "attention.cuh"
+#include "attention_tc.cuh"
 
 namespace ormi_b200 {
 namespace {
@@ -500,7 +500,9 @@ void attention(ormi_b200_ctx* ctx, const ormi_b200_attention_args& a) {
     if (!p.batch || !p.q_len || !p.heads) return;
     written(ctx, a.out);
     written(ctx, a.lse);
-    attention_simple(ctx, p, a.q.dtype);
+    // few packed rows over the cache: a tile of 128 queries would be mostly padding
+    const bool few = (int64_t)p.q_len * p.group <= 16;
+    if (!few && attention_tc_supported(p, a.q.dtype)) attention_tc(ctx, p); else attention_simple(ctx, p, a.q.dtype);
 }
 
 void attention_backward_check(const ormi_b200_attention_backward_args& a) {

@@ -1,0 +1,385 @@
+// Forward attention on the tensor cores: bf16, head_dim up to 128.
+//
+// A block owns 256 queries of one head, as two tiles of 128 rows, and walks the tiles of 128 keys that any of them sees.
+// Warp 0 loads (TMA: Q once, K and V through a ring), warp 1 issues the products (tcgen05), warp 2 blanks the rows of V
+// behind key_len, and a warpgroup per tile of queries turns scores into probabilities: a thread owns a row, so the running
+// maximum and sum of the softmax need no exchange.  In tensor memory a tile has its scores S (128 columns), overwritten in
+// place by the probabilities as bf16, which the second product reads as its A operand, and its output O.  While one
+// warpgroup works on its scores the tensor cores run the other tile's products.
+//
+// O is rescaled only when a row's maximum has grown by more than 2^8 since the last time: probabilities up to 256 lose
+// nothing in fp32 sums nor, relatively, in bf16.
+#include <algorithm>
+
+#include "attention_tc.cuh"
+
+namespace ormi_b200 {
+namespace {
+
+using namespace tc;
+
+constexpr int kThreads = 384;                    // warps 0-3: load, multiply, blank, (idle); 4-7 and 8-11: softmax of a tile each
+
+template <int DP> struct ForwardShape {
+    static constexpr int kOperand = kTile * DP * 2;            // bytes of a tile of Q, K or V
+    static constexpr int kStages = DP == 128 ? 4 : 8;
+    static constexpr int kSmem = 1024 + (2 + kStages) * kOperand + kMaxTiles + 8 * 512 + 256;
+};
+
+template <int DP, bool CAP, bool BIAS, bool DOCS>
+__global__ void __launch_bounds__(kThreads, 1)
+attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                const __grid_constant__ TcParams p) {
+    using Shape = ForwardShape<DP>;
+    constexpr int ST = Shape::kStages, OP = Shape::kOperand;
+    extern __shared__ unsigned char raw[];
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    unsigned char* mem = raw + (base - smem_u32(raw));
+    const uint32_t q_at = base, ring = base + 2 * OP;
+    unsigned char* cls = mem + (2 + ST) * OP;                  // two bits for each tile of queries
+    int* docs = reinterpret_cast<int*>(cls + kMaxTiles);       // 128 for each softmax warp
+    const uint32_t bars = smem_u32(docs + 8 * 128);
+    const uint32_t q_full = bars, o_full = bars + 8, v_blank = bars + 16, blank_go = bars + 248;
+    auto s_full = [&](int w) { return bars + 24 + 8 * w; };
+    auto p_full = [&](int w) { return bars + 40 + 8 * w; };
+    auto kv_full = [&](int s) { return bars + 56 + 8 * s; };
+    auto kv_empty = [&](int s) { return bars + 56 + 8 * (ST + s); };
+    __shared__ uint32_t tmem_slot;
+    __shared__ Abort ab;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = blockIdx.x / p.a.heads, h = blockIdx.x % p.a.heads, kvh = h / p.a.group;
+    const int q0 = (int)(gridDim.y - 1 - blockIdx.y) * 2 * kTile;         // causal: the longest rows first
+    const RowMask m = row_mask(p.a, b);
+    // key_end of the first and the last query of each tile
+    int lo[2], hi[2];
+    for (int w = 0; w < 2; ++w) {
+        const int first = q0 + w * kTile, last = min(first + kTile, p.a.q_len) - 1;
+        lo[w] = key_end(m, m.start + first);
+        hi[w] = first < p.a.q_len ? key_end(m, m.start + last) : 0;
+    }
+    const int tiles = (max(max(hi[0], hi[1]), 0) + kTile - 1) / kTile;
+    // classes of the tiles, and which union tile holds the last valid key in its middle
+    for (int j = threadIdx.x; j < tiles; j += kThreads) {
+        int c = 0;
+        for (int w = 0; w < 2; ++w) c |= tile_class(p, b, q0 / kTile + w, lo[w], hi[w], j) << (2 * w);
+        cls[j] = (unsigned char)c;
+    }
+    const int blank_tile = m.keys < p.a.k_len && m.keys % kTile ? m.keys / kTile : -1;
+    if (threadIdx.x == 0) {
+        ab.flag = 0; ab.err = p.err;
+        mbar_init(q_full, 1); mbar_init(o_full, 1); mbar_init(v_blank, 1); mbar_init(blank_go, 1);
+        for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(p_full(w), 4); }
+        for (int s = 0; s < ST; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 1); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot;
+    auto s_at = [&](int w) { return tmem + w * 128; };
+    auto o_at = [&](int w) { return tmem + 256 + w * 128; };
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 0 && lane == 0) {
+            // ---------------------------------------------------------------- loads
+            mbar_expect_tx(q_full, 2 * OP);
+            for (int w = 0; w < 2; ++w)
+                for (int x = 0; x < DP / 64; ++x) tma_load_4d(q_at + w * OP + x * kBox, &map_q, q_full, 64 * x, q0 + w * kTile, h, b);
+            int seq = 0;
+            bool ok = true;
+            for (int j = 0; j < tiles && ok; ++j) {
+                if (!cls[j]) continue;
+                for (int kv = 0; kv < 2 && ok; ++kv, ++seq) {
+                    const int s = seq % ST;
+                    ok = mbar_wait(kv_empty(s), (seq / ST & 1) ^ 1, ab, 21);
+                    if (!ok) break;
+                    mbar_expect_tx(kv_full(s), OP);
+                    for (int x = 0; x < DP / 64; ++x) tma_load_4d(ring + s * OP + x * kBox, kv ? &map_v : &map_k, kv_full(s), 64 * x, j * kTile, kvh, b);
+                }
+            }
+            // nothing of this block's is in flight when it leaves
+            ok = ok && mbar_wait(q_full, 0, ab, 21);
+            for (int i = 0; i < ST && ok; ++i, ++seq) ok = mbar_wait(kv_empty(seq % ST), (seq / ST & 1) ^ 1, ab, 21);
+        } else if (warp == 1 && lane == 0) {
+            // ---------------------------------------------------------------- products
+            int u = -1, prev = 0, prev_j = -1, used_p[2] = {0, 0};
+            bool ok = mbar_wait(q_full, 0, ab, 22);
+            for (int j = 0; j <= tiles && ok; ++j) {
+                const int c = j < tiles ? cls[j] : 0;
+                if (!c && j < tiles) continue;
+                if (c) ++u;
+                const int k_seq = 2 * u, v_seq = (c ? 2 * (u - 1) : 2 * u) + 1;      // K of this tile, V of the one before
+                bool have_k = false, have_v = false;
+                for (int w = 0; w < 2 && ok; ++w) {
+                    if (prev >> (2 * w) & 3) {
+                        if (!have_v) {
+                            ok = mbar_wait(kv_full(v_seq % ST), v_seq / ST & 1, ab, 23);
+                            if (ok && prev_j == blank_tile) {              // warp 2 may begin: these rows have landed
+                                mbar_arrive(blank_go);
+                                ok = mbar_wait(v_blank, 0, ab, 24);
+                            }
+                            have_v = true;
+                        }
+                        ok = ok && mbar_wait(p_full(w), used_p[w] & 1, ab, 25);
+                        if (!ok) break;
+                        fence_after();
+                        product_tn<DP>(o_at(w), s_at(w), ring + (v_seq % ST) * OP, used_p[w] > 0);
+                        ++used_p[w];
+                    }
+                    if (c >> (2 * w) & 3) {
+                        if (!have_k) { ok = mbar_wait(kv_full(k_seq % ST), k_seq / ST & 1, ab, 26); have_k = true; }
+                        if (!ok) break;
+                        fence_after();
+                        product_nt<DP, kTile>(s_at(w), q_at + w * OP, ring + (k_seq % ST) * OP, 0);
+                        commit(s_full(w));
+                    }
+                }
+                if (!ok) break;
+                if (prev) commit(kv_empty(v_seq % ST));
+                if (c) commit(kv_empty(k_seq % ST));
+                prev = c;
+                prev_j = j;
+            }
+            commit(o_full);
+        } else if (warp == 2 && blank_tile >= 0 && blank_tile < tiles && cls[blank_tile]) {
+            // ---------------------------------------------------------------- rows of V behind key_len: zero, whatever they held
+            // (the issuer says when V has landed: a parity wait of this warp's own on the ring could be a phase late or early)
+            int u = 0;
+            for (int j = 0; j < blank_tile; ++j) u += cls[j] != 0;
+            const int s = (2 * u + 1) % ST;
+            if (warp_wait(blank_go, 0, ab, 27)) {
+                const int first = m.keys % kTile;
+                for (int x = 0; x < DP / 64; ++x)
+                    for (int i = first * 8 + lane; i < kTile * 8; i += 32)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(ring + s * OP + x * kBox + i * 16), "r"(0) : "memory");
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_blank);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        // -------------------------------------------------------------------- softmax: one row per thread
+        const int w = warp / 4 - 1;
+        const int t = q0 + w * kTile + (threadIdx.x & 127);
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;                       // this warp's 32 lanes of tensor memory
+        const bool live = t < p.a.q_len;
+        const int pos = m.start + t, end = live ? key_end(m, pos) : 0;
+        const int my_doc = DOCS && live ? m.q_docs[t] : 0;
+        const float slope = BIAS ? p.a.slopes[h] * kLog2e : 0.f;
+        int* my_docs = docs + (warp - 4) * 128;
+        float top = -INFINITY, total = 0.f;
+        int n = 0;
+        bool ok = true;
+        for (int j = 0; j < tiles; ++j) {
+            const int c = cls[j] >> (2 * w) & 3;
+            if (!c) continue;
+            const int key0 = j * kTile;
+            if (DOCS && c == kPartial) {
+                __syncwarp();
+                for (int i = lane; i < kTile; i += 32) my_docs[i] = key0 + i < p.a.k_len ? m.k_docs[key0 + i] : 0;
+                __syncwarp();
+            }
+            ok = warp_wait(s_full(w), n & 1, ab, 28);
+            if (!ok) break;
+            fence_after();
+            float z[128];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ld32(s_at(w) + lanes + 32 * i, reinterpret_cast<uint32_t*>(z) + 32 * i);
+            wait_ld();
+#pragma unroll
+            for (int i = 0; i < 128; ++i) {
+                z[i] = score_log2<CAP>(p, z[i]);
+                if (BIAS) z[i] = fmaf(-slope, fabsf((float)(pos - key0) - (float)i), z[i]);
+            }
+            if (c == kPartial) {
+                const int left = end - key0;
+#pragma unroll
+                for (int i = 0; i < 128; ++i) if (i >= left || (DOCS && my_docs[i] != my_doc)) z[i] = -INFINITY;
+            }
+            float mx[4] = {z[0], z[1], z[2], z[3]};
+#pragma unroll
+            for (int i = 4; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], z[i]);
+            const float big = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+            if (__any_sync(0xffffffffu, big > top + 8.f)) {
+                const float by = big == -INFINITY ? 1.f : ex2(top - big);
+                top = big;
+                total *= by;
+                if (n) {                                       // the product before this tile's scores is complete: commits are in order
+#pragma unroll 1
+                    for (int x = 0; x < DP; x += 32) {
+                        uint32_t o[32];
+                        ld32(o_at(w) + lanes + x, o);
+                        wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
+                        st32(o_at(w) + lanes + x, o);
+                    }
+                }
+            }
+            const float from = top == -INFINITY ? 0.f : top;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                uint32_t pk[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float a = ex2(z[32 * x + 2 * i] - from), d = ex2(z[32 * x + 2 * i + 1] - from);
+                    sum[2 * i & 3] += a;
+                    sum[(2 * i + 1) & 3] += d;
+                    pk[i] = pack_bf16x2(a, d);
+                }
+                st16(s_at(w) + lanes + 16 * x, pk);
+            }
+            total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full(w));
+            ++n;
+        }
+        if (ok && n) ok = warp_wait(o_full, 0, ab, 29);
+        if (ok) {
+            fence_after();
+            const float by = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
+            bf16* out = (bf16*)p.a.out + (int64_t)b * p.a.os.b + (int64_t)t * p.a.os.t + (int64_t)h * p.a.os.h;
+#pragma unroll 1
+            for (int x = 0; x < DP; x += 32) {
+                uint32_t o[32];
+                if (n) { ld32(o_at(w) + lanes + x, o); wait_ld(); }
+                else for (int i = 0; i < 32; ++i) o[i] = 0;
+                if (!live) continue;
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    if (x + i >= p.a.dim) break;
+                    uint4 v;
+                    v.x = pack_bf16x2(__uint_as_float(o[i]) * by, __uint_as_float(o[i + 1]) * by);
+                    v.y = pack_bf16x2(__uint_as_float(o[i + 2]) * by, __uint_as_float(o[i + 3]) * by);
+                    v.z = pack_bf16x2(__uint_as_float(o[i + 4]) * by, __uint_as_float(o[i + 5]) * by);
+                    v.w = pack_bf16x2(__uint_as_float(o[i + 6]) * by, __uint_as_float(o[i + 7]) * by);
+                    *reinterpret_cast<uint4*>(out + x + i) = v;
+                }
+            }
+            if (live && p.a.lse) p.a.lse[((int64_t)b * p.a.heads + h) * p.a.q_len + t] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
+        }
+    }
+    // ------------------------------------------------------------------------ teardown
+    __syncwarp();
+    if (ab.flag) {                                             // let copies that are still in flight land before the block goes away
+        const unsigned long long t0 = global_ns();
+        while (global_ns() - t0 < 200000ull) { }
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// Smallest and largest document of every tile of 128 positions: a warp per tile.
+__global__ void __launch_bounds__(256) attn_doc_bounds(const int32_t* docs, int batch, int len, int tiles, int2* bounds) {
+    const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (at >= (int64_t)batch * tiles) return;
+    const int b = at / tiles, j = at % tiles, lane = threadIdx.x & 31;
+    int lo = INT32_MAX, hi = INT32_MIN;
+    for (int i = j * kTile + lane; i < min((j + 1) * kTile, len); i += 32) {
+        const int d = docs[(int64_t)b * len + i];
+        lo = min(lo, d); hi = max(hi, d);
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) bounds[at] = make_int2(lo, hi);
+}
+
+template <int DP, bool CAP, bool BIAS, bool DOCS>
+void launch_forward(ormi_b200_ctx* ctx, const CUtensorMap* maps, const TcParams& p) {
+    auto kernel = attn_forward_tc<DP, CAP, BIAS, DOCS>;
+    constexpr int smem = ForwardShape<DP>::kSmem;
+    ORMI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kernel<<<dim3(p.a.batch * p.a.heads, (p.a.q_len + 2 * kTile - 1) / (2 * kTile)), kThreads, smem, ctx->stream>>>(maps[0], maps[1], maps[2], p);
+    ORMI_CUDA(cudaGetLastError());
+    count_launch(ctx);
+}
+
+template <int DP>
+void launch_by_mask(ormi_b200_ctx* ctx, const CUtensorMap* maps, const TcParams& p) {
+    const bool cap = p.a.cap > 0.f, bias = p.a.slopes, docs = p.a.k_docs;
+    if (cap) {
+        if (bias) docs ? launch_forward<DP, true, true, true>(ctx, maps, p) : launch_forward<DP, true, true, false>(ctx, maps, p);
+        else docs ? launch_forward<DP, true, false, true>(ctx, maps, p) : launch_forward<DP, true, false, false>(ctx, maps, p);
+    } else {
+        if (bias) docs ? launch_forward<DP, false, true, true>(ctx, maps, p) : launch_forward<DP, false, true, false>(ctx, maps, p);
+        else docs ? launch_forward<DP, false, false, true>(ctx, maps, p) : launch_forward<DP, false, false, false>(ctx, maps, p);
+    }
+}
+
+}  // namespace
+
+// A 4-D map (head_dim, position, head, batch) with boxes of 64 values x 128 positions: reads behind any extent give zero.
+void head_map(ormi_b200_ctx* ctx, CUtensorMap* map, const void* ptr, const Strides4& s, int batch, int len, int heads, int dim) {
+    cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)len, (cuuint64_t)heads, (cuuint64_t)batch};
+    // the stride of an extent of one is never used, but is checked
+    cuuint64_t strides[3] = {(cuuint64_t)(len > 1 ? s.t * 2 : 16), (cuuint64_t)(heads > 1 ? s.h * 2 : 16), (cuuint64_t)(batch > 1 ? s.b * 2 : 16)};
+    cuuint32_t box[4] = {64, (cuuint32_t)kTile, 1, 1}, one[4] = {1, 1, 1, 1};
+    ctx->drv.check(ctx->drv.TensorMapEncodeTiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
+                   "cuTensorMapEncodeTiled");
+}
+
+// TMA wants 16-byte addresses and strides; a stride of zero (a broadcast operand) is left to the other kernels.
+bool map_allowed(const void* ptr, const Strides4& s, int batch, int len, int heads) {
+    auto good = [](int64_t stride, int extent) { return extent <= 1 || (stride > 0 && stride % 8 == 0 && stride * 2 < (int64_t)1 << 40); };
+    return (uintptr_t)ptr % 16 == 0 && good(s.b, batch) && good(s.t, len) && good(s.h, heads);
+}
+
+size_t bounds_bytes(const AttnParams& p) {
+    return p.k_docs ? (size_t)p.batch * ((p.q_len + kTile - 1) / kTile + 1 + (p.k_len + kTile - 1) / kTile) * sizeof(int2) : 0;
+}
+
+TcParams tc_params(ormi_b200_ctx* ctx, const AttnParams& a, int2* bounds) {
+    TcParams p{};
+    p.a = a;
+    p.q_tiles = (a.q_len + kTile - 1) / kTile;
+    p.q_tiles += p.q_tiles & 1;                                  // a block looks at two tiles of queries
+    p.k_tiles = (a.k_len + kTile - 1) / kTile;
+    p.scale_log2 = a.cap > 0.f ? 2.f * kLog2e * a.scale / a.cap : a.scale * kLog2e;
+    p.cap_log2 = a.cap * kLog2e;
+    p.err = device_error_word(ctx);
+    ctx->gemm_err_pending = true;
+    if (a.k_docs) {
+        int2* kb = bounds + (size_t)a.batch * p.q_tiles;
+        attn_doc_bounds<<<(int)(((int64_t)a.batch * p.q_tiles + 7) / 8), 256, 0, ctx->stream>>>(a.q_docs, a.batch, a.q_len, p.q_tiles, bounds);
+        attn_doc_bounds<<<(int)(((int64_t)a.batch * p.k_tiles + 7) / 8), 256, 0, ctx->stream>>>(a.k_docs, a.batch, a.k_len, p.k_tiles, kb);
+        ORMI_CUDA(cudaGetLastError());
+        count_launch(ctx, 2);
+        p.q_bounds = bounds; p.k_bounds = kb;
+    }
+    return p;
+}
+
+bool attention_tc_supported(const AttnParams& p, int dtype) {
+    return dtype == ORMI_BF16 && p.dim <= 128 && p.dim % 8 == 0 && p.k_len >= 1 && p.k_len <= kMaxTiles * kTile && p.q_len <= 65535 * 2 * kTile &&
+           (int64_t)p.batch * p.heads < 0x7fffffff && map_allowed(p.q, p.qs, p.batch, p.q_len, p.heads) && map_allowed(p.k, p.ks, p.batch, p.k_len, p.kv_heads) &&
+           map_allowed(p.v, p.vs, p.batch, p.k_len, p.kv_heads) && map_allowed(p.out, p.os, p.batch, p.q_len, p.heads);
+}
+
+void attention_tc(ormi_b200_ctx* ctx, AttnParams& a) {
+    Scratch bounds(ctx, bounds_bytes(a));
+    const TcParams p = tc_params(ctx, a, (int2*)bounds.ptr);
+    CUtensorMap maps[3];
+    head_map(ctx, &maps[0], a.q, a.qs, a.batch, a.q_len, a.heads, a.dim);
+    head_map(ctx, &maps[1], a.k, a.ks, a.batch, a.k_len, a.kv_heads, a.dim);
+    head_map(ctx, &maps[2], a.v, a.vs, a.batch, a.k_len, a.kv_heads, a.dim);
+    if (a.dim <= 64) launch_by_mask<64>(ctx, maps, p); else launch_by_mask<128>(ctx, maps, p);
+    bounds.release();
+}
+
+}  // namespace ormi_b200
