@@ -1,0 +1,568 @@
+// Backward attention on the tensor cores: bf16, head_dim up to 128.
+//
+// Two kernels, so that no gradient is summed with atomics and results do not depend on the order of blocks:
+//   attn_back_kv   a block owns 128 keys of one key/value head and walks the tiles of 128 queries that see any of them, over
+//                  all query heads that share the head.  Scores are computed transposed (rows = keys), so that
+//                  probabilities and score gradients, rounded to bf16 in tensor memory, are the A operands of
+//                  dV += P^T dO and dK += dS^T Q directly.
+//   attn_back_q    a block owns 128 queries of one head and walks the tiles of keys: dQ += dS K.
+// The price is that both compute the scores (7 products instead of 5).  Warp 0 loads, warp 1 issues the products, warp 2
+// fetches the queries' statistics (or blanks the keys behind key_len), 8 warps do the arithmetic: two warpgroups, each half
+// of the columns of a tile.
+#include <algorithm>
+
+#include "attention_tc.cuh"
+
+namespace ormi_b200 {
+namespace {
+
+using namespace tc;
+
+constexpr int kThreads = 384;
+
+struct Stat { float lse2[kTile], delta[kTile]; int end[kTile], doc[kTile]; };      // of 128 queries
+
+template <int DP> struct BackShape {
+    static constexpr int kOperand = kTile * DP * 2;
+    static constexpr int kStages = DP == 128 ? 2 : 4;
+    static constexpr int kSmem = 1024 + (2 + 2 * kStages) * kOperand + kMaxTiles * 2 + kStages * (int)sizeof(Stat) + 256;
+};
+
+// The tiles whose class is not kSkip, in order, with bit 15 set where each pair has to be looked at; by one warp.
+template <typename F>
+__device__ __forceinline__ int list_tiles(unsigned short* list, int tiles, F&& class_of) {
+    const int lane = threadIdx.x & 31;
+    int n = 0;
+    for (int first = 0; first < tiles; first += 32) {
+        const int c = first + lane < tiles ? class_of(first + lane) : kSkip;
+        const unsigned hit = __ballot_sync(0xffffffffu, c != kSkip);
+        if (c != kSkip) list[n + __popc(hit & ((1u << lane) - 1))] = (unsigned short)((first + lane) | (c == kPartial ? 0x8000 : 0));
+        n += __popc(hit);
+    }
+    return n;
+}
+
+// Base-2 score and the derivative of the cap, from the raw product.
+template <bool CAP>
+__device__ __forceinline__ float score_and_slope(const TcParams& p, float raw, float& dcap) {
+    if (!CAP) { dcap = 1.f; return raw * p.scale_log2; }
+    const float r = __fdividef(1.f, ex2(raw * p.scale_log2) + 1.f);             // tanh = 1 - 2 r, 1 - tanh^2 = 4 r (1 - r)
+    dcap = 4.f * r * (1.f - r);
+    return fmaf(-2.f * p.cap_log2, r, p.cap_log2);
+}
+
+// 32 columns of tensor memory to 32 bf16 values of a row, times `by`.
+__device__ __forceinline__ void store_row32(bf16* out, int x, int dim, const uint32_t* o, float by) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+        if (x + i >= dim) break;
+        uint4 v;
+        v.x = pack_bf16x2(__uint_as_float(o[i]) * by, __uint_as_float(o[i + 1]) * by);
+        v.y = pack_bf16x2(__uint_as_float(o[i + 2]) * by, __uint_as_float(o[i + 3]) * by);
+        v.z = pack_bf16x2(__uint_as_float(o[i + 4]) * by, __uint_as_float(o[i + 5]) * by);
+        v.w = pack_bf16x2(__uint_as_float(o[i + 6]) * by, __uint_as_float(o[i + 7]) * by);
+        *reinterpret_cast<uint4*>(out + x + i) = v;
+    }
+}
+
+// A operand of 128 bf16 columns that two warpgroups wrote into the first halves of their own 64 columns.
+template <int DP>
+__device__ __forceinline__ void product_halves(uint32_t d, uint32_t a, uint32_t b, uint32_t accumulate) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mma_ts(d, a + (k / 4) * 64 + (k % 4) * 8, desc(b, true) + ((k * 2048) >> 4), idesc(DP, true), accumulate || k > 0);
+}
+
+template <int DP, bool CAP, bool BIAS, bool DOCS>
+__global__ void __launch_bounds__(kThreads, 1)
+attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+             const __grid_constant__ CUtensorMap map_do, const __grid_constant__ TcParams p) {
+    using Shape = BackShape<DP>;
+    constexpr int ST = Shape::kStages, OP = Shape::kOperand;
+    extern __shared__ unsigned char raw[];
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    unsigned char* mem = raw + (base - smem_u32(raw));
+    const uint32_t k_at = base, v_at = base + OP;
+    auto q_at = [&](int s) { return base + (2 + 2 * s) * OP; };
+    auto do_at = [&](int s) { return base + (3 + 2 * s) * OP; };
+    Stat* stats = reinterpret_cast<Stat*>(mem + (2 + 2 * ST) * OP);
+    unsigned short* list = reinterpret_cast<unsigned short*>(stats + ST);
+    const uint32_t bars = smem_u32(list + kMaxTiles);
+    const uint32_t kv_full = bars, s_full = bars + 8, dp_full = bars + 16, p_ready = bars + 24, ds_ready = bars + 32, done = bars + 40;
+    auto q_full = [&](int s) { return bars + 48 + 8 * s; };
+    auto do_full = [&](int s) { return bars + 48 + 8 * (ST + s); };
+    auto empty = [&](int s) { return bars + 48 + 8 * (2 * ST + s); };
+    auto stat_full = [&](int s) { return bars + 48 + 8 * (3 * ST + s); };
+    auto stat_empty = [&](int s) { return bars + 48 + 8 * (4 * ST + s); };
+    __shared__ uint32_t tmem_slot;
+    __shared__ int list_size;
+    __shared__ Abort ab;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = blockIdx.x / p.a.kv_heads, kvh = blockIdx.x % p.a.kv_heads;
+    const int key0 = blockIdx.y * kTile;                                   // causal: the first keys are seen by most queries
+    const RowMask m = row_mask(p.a, b);
+    if (warp == 0) {
+        const int n = key0 >= m.keys ? 0 : list_tiles(list, (p.a.q_len + kTile - 1) / kTile, [&](int t) {
+            const int first = t * kTile, last = min(first + kTile, p.a.q_len) - 1;
+            return tile_class(p, b, t, key_end(m, m.start + first), key_end(m, m.start + last), key0 / kTile);
+        });
+        if (lane == 0) list_size = n;
+    }
+    if (threadIdx.x == 0) {
+        ab.flag = 0; ab.err = p.err;
+        mbar_init(kv_full, 1); mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(done, 1);
+        mbar_init(p_ready, 8); mbar_init(ds_ready, 8);
+        for (int s = 0; s < ST; ++s) { mbar_init(q_full(s), 1); mbar_init(do_full(s), 1); mbar_init(empty(s), 1); mbar_init(stat_full(s), 1); mbar_init(stat_empty(s), 8); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot, s_at = tmem, dp_at = tmem + 128, dv_at = tmem + 256, dk_at = tmem + 384;
+    const int per_head = list_size, total = per_head * p.a.group;
+
+    if (warp == 0) {
+        if (lane == 0 && total) {
+            mbar_expect_tx(kv_full, 2 * OP);
+            for (int x = 0; x < DP / 64; ++x) {
+                tma_load_4d(k_at + x * kBox, &map_k, kv_full, 64 * x, key0, kvh, b);
+                tma_load_4d(v_at + x * kBox, &map_v, kv_full, 64 * x, key0, kvh, b);
+            }
+            bool ok = true;
+            int i = 0;
+            for (; i < total && ok; ++i) {
+                const int s = i % ST, h = kvh * p.a.group + i / per_head, q0 = (list[i % per_head] & 0x7fff) * kTile;
+                ok = mbar_wait(empty(s), (i / ST & 1) ^ 1, ab, 31);
+                if (!ok) break;
+                mbar_expect_tx(q_full(s), OP);
+                for (int x = 0; x < DP / 64; ++x) tma_load_4d(q_at(s) + x * kBox, &map_q, q_full(s), 64 * x, q0, h, b);
+                mbar_expect_tx(do_full(s), OP);
+                for (int x = 0; x < DP / 64; ++x) tma_load_4d(do_at(s) + x * kBox, &map_do, do_full(s), 64 * x, q0, h, b);
+            }
+            for (int k = 0; k < ST && ok; ++k, ++i) ok = mbar_wait(empty(i % ST), (i / ST & 1) ^ 1, ab, 31);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && total) {
+            bool ok = mbar_wait(kv_full, 0, ab, 32);
+            auto scores = [&](int i) {
+                ok = ok && mbar_wait(q_full(i % ST), i / ST & 1, ab, 33);
+                if (!ok) return;
+                fence_after();
+                product_nt<DP, kTile>(s_at, k_at, q_at(i % ST), 0);
+                commit(s_full);
+            };
+            auto gaps = [&](int i) {
+                ok = ok && mbar_wait(do_full(i % ST), i / ST & 1, ab, 34);
+                if (!ok) return;
+                fence_after();
+                product_nt<DP, kTile>(dp_at, v_at, do_at(i % ST), 0);
+                commit(dp_full);
+            };
+            scores(0);
+            gaps(0);
+            // P sits in the scores' columns and dS in the columns of dP: the next tile's products follow their readers in order
+            for (int i = 0; i < total && ok; ++i) {
+                ok = mbar_wait(p_ready, i & 1, ab, 35);
+                if (!ok) break;
+                fence_after();
+                product_halves<DP>(dv_at, s_at, do_at(i % ST), i > 0);
+                if (i + 1 < total) scores(i + 1);
+                ok = ok && mbar_wait(ds_ready, i & 1, ab, 36);
+                if (!ok) break;
+                fence_after();
+                product_halves<DP>(dk_at, dp_at, q_at(i % ST), i > 0);
+                commit(empty(i % ST));
+                if (i + 1 < total) gaps(i + 1);
+            }
+            commit(done);
+        }
+    } else if (warp == 2) {
+        // the queries' statistics; a row that sees nothing, or does not exist, gets +infinity: its probabilities vanish
+        for (int i = 0; i < total; ++i) {
+            const int s = i % ST, h = kvh * p.a.group + i / per_head, q0 = (list[i % per_head] & 0x7fff) * kTile;
+            float l[4], d[4];
+            int e[4], doc[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int t = q0 + k * 32 + lane;
+                const bool live = t < p.a.q_len;
+                const int64_t line = ((int64_t)b * p.a.heads + h) * p.a.q_len + t;
+                l[k] = live ? p.a.lse[line] * kLog2e : INFINITY;
+                if (l[k] == -INFINITY) l[k] = INFINITY;
+                d[k] = live ? p.a.delta[line] : 0.f;
+                e[k] = live ? key_end(m, m.start + t) : 0;
+                doc[k] = DOCS && live ? m.q_docs[t] : 0;
+            }
+            if (!warp_wait(stat_empty(s), (i / ST & 1) ^ 1, ab, 37)) break;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                stats[s].lse2[k * 32 + lane] = l[k]; stats[s].delta[k * 32 + lane] = d[k];
+                stats[s].end[k * 32 + lane] = e[k];
+                if (DOCS) stats[s].doc[k * 32 + lane] = doc[k];
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(stat_full(s));
+        }
+    } else if (warp >= 4) {
+        const int w = warp / 4 - 1, row = threadIdx.x & 127, key = key0 + row;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+        const bool live = key < m.keys;
+        const int my_doc = DOCS && live ? m.k_docs[key] : 0;
+        bool ok = true;
+        for (int i = 0; i < total; ++i) {
+            const int s = i % ST, entry = list[i % per_head], q0 = (entry & 0x7fff) * kTile;
+            const bool partial = entry & 0x8000;
+            const Stat& st = stats[s];
+            const float slope = BIAS ? p.a.slopes[kvh * p.a.group + i / per_head] * kLog2e : 0.f;
+            const float ahead = (float)(m.start + q0 + 64 * w - key);
+            ok = warp_wait(stat_full(s), i / ST & 1, ab, 38) && warp_wait(s_full, i & 1, ab, 38);
+            if (!ok) break;
+            fence_after();
+            float g[64];
+            ld32(s_at + lanes + 64 * w, reinterpret_cast<uint32_t*>(g));
+            ld32(s_at + lanes + 64 * w + 32, reinterpret_cast<uint32_t*>(g) + 32);
+            wait_ld();
+            uint32_t pk[32];
+#pragma unroll
+            for (int c = 0; c < 64; c += 4) {
+                const float4 l = *reinterpret_cast<const float4*>(&st.lse2[64 * w + c]);
+                const float lse2[4] = {l.x, l.y, l.z, l.w};
+                float prob[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float dcap;
+                    float z = score_and_slope<CAP>(p, g[c + k], dcap);
+                    if (BIAS) z = fmaf(-slope, fabsf(ahead + (float)(c + k)), z);
+                    prob[k] = ex2(z - lse2[k]);
+                    g[c + k] = dcap;
+                }
+                if (partial) {
+                    const int4 e = *reinterpret_cast<const int4*>(&st.end[64 * w + c]);
+                    const int end[4] = {e.x, e.y, e.z, e.w};
+                    int4 dd = make_int4(0, 0, 0, 0);
+                    if (DOCS) dd = *reinterpret_cast<const int4*>(&st.doc[64 * w + c]);
+                    const int doc[4] = {dd.x, dd.y, dd.z, dd.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) if (key >= end[k] || (DOCS && doc[k] != my_doc)) { prob[k] = 0.f; g[c + k] = 0.f; }
+                }
+                pk[c / 2] = pack_bf16x2(prob[0], prob[1]);
+                pk[c / 2 + 1] = pack_bf16x2(prob[2], prob[3]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) g[c + k] = CAP ? g[c + k] * prob[k] : prob[k];
+            }
+            st32(s_at + lanes + 64 * w, pk);
+            wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_ready);
+            ok = warp_wait(dp_full, i & 1, ab, 39);
+            if (!ok) break;
+            fence_after();
+            float gap[64];
+            ld32(dp_at + lanes + 64 * w, reinterpret_cast<uint32_t*>(gap));
+            ld32(dp_at + lanes + 64 * w + 32, reinterpret_cast<uint32_t*>(gap) + 32);
+            wait_ld();
+#pragma unroll
+            for (int c = 0; c < 64; c += 4) {
+                const float4 d = *reinterpret_cast<const float4*>(&st.delta[64 * w + c]);
+                const float delta[4] = {d.x, d.y, d.z, d.w};
+                float ds[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) ds[k] = partial && g[c + k] == 0.f ? 0.f : g[c + k] * (gap[c + k] - delta[k]);
+                pk[c / 2] = pack_bf16x2(ds[0], ds[1]);
+                pk[c / 2 + 1] = pack_bf16x2(ds[2], ds[3]);
+            }
+            st32(dp_at + lanes + 64 * w, pk);
+            wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(ds_ready); mbar_arrive(stat_empty(s)); }
+        }
+        if (ok && total) ok = warp_wait(done, 0, ab, 40);
+        if (ok) {
+            // warpgroup 0 writes dV, warpgroup 1 dK; keys that nobody sees get zero
+            fence_after();
+            const Strides4& os = w ? p.a.dks : p.a.dvs;
+            bf16* out = (bf16*)(w ? p.a.dk : p.a.dv) + (int64_t)b * os.b + (int64_t)key * os.t + (int64_t)kvh * os.h;
+#pragma unroll 1
+            for (int x = 0; x < DP; x += 32) {
+                uint32_t o[32];
+                if (total) { ld32((w ? dk_at : dv_at) + lanes + x, o); wait_ld(); }
+                else for (int i = 0; i < 32; ++i) o[i] = 0;
+                if (key < p.a.k_len) store_row32(out, x, p.a.dim, o, w ? p.a.scale : 1.f);
+            }
+        }
+    }
+    __syncwarp();
+    if (ab.flag) {                                             // let copies that are still in flight land before the block goes away
+        const unsigned long long t0 = global_ns();
+        while (global_ns() - t0 < 200000ull) { }
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+template <int DP, bool CAP, bool BIAS, bool DOCS>
+__global__ void __launch_bounds__(kThreads, 1)
+attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+            const __grid_constant__ CUtensorMap map_do, const __grid_constant__ TcParams p) {
+    using Shape = BackShape<DP>;
+    constexpr int ST = Shape::kStages, OP = Shape::kOperand;
+    extern __shared__ unsigned char raw[];
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    unsigned char* mem = raw + (base - smem_u32(raw));
+    const uint32_t q_at = base, do_at = base + OP;
+    auto k_at = [&](int s) { return base + (2 + 2 * s) * OP; };
+    auto v_at = [&](int s) { return base + (3 + 2 * s) * OP; };
+    int* docs = reinterpret_cast<int*>(mem + (2 + 2 * ST) * OP);                 // 64 for each compute warp
+    unsigned short* list = reinterpret_cast<unsigned short*>(docs + 8 * 64);
+    const uint32_t bars = smem_u32(list + kMaxTiles);
+    const uint32_t q_full = bars, dp_full = bars + 8, ds_ready = bars + 16, done = bars + 24, blank_go = bars + 32, blanked = bars + 40;
+    auto s_full = [&](int x) { return bars + 48 + 8 * x; };
+    auto s_empty = [&](int x) { return bars + 64 + 8 * x; };
+    auto k_full = [&](int s) { return bars + 80 + 8 * s; };
+    auto v_full = [&](int s) { return bars + 80 + 8 * (ST + s); };
+    auto empty = [&](int s) { return bars + 80 + 8 * (2 * ST + s); };
+    __shared__ uint32_t tmem_slot;
+    __shared__ int list_size;
+    __shared__ Abort ab;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = blockIdx.x / p.a.heads, h = blockIdx.x % p.a.heads, kvh = h / p.a.group;
+    const int q0 = (int)(gridDim.y - 1 - blockIdx.y) * kTile;
+    const RowMask m = row_mask(p.a, b);
+    const int blank_tile = m.keys < p.a.k_len && m.keys % kTile ? m.keys / kTile : -1;
+    if (warp == 0) {
+        const int lo = key_end(m, m.start + q0), hi = key_end(m, m.start + min(q0 + kTile, p.a.q_len) - 1);
+        const int n = list_tiles(list, (max(hi, 0) + kTile - 1) / kTile, [&](int j) { return tile_class(p, b, q0 / kTile, lo, hi, j); });
+        if (lane == 0) list_size = n;
+    }
+    if (threadIdx.x == 0) {
+        ab.flag = 0; ab.err = p.err;
+        mbar_init(q_full, 1); mbar_init(dp_full, 1); mbar_init(ds_ready, 8); mbar_init(done, 1); mbar_init(blank_go, 1); mbar_init(blanked, 1);
+        for (int x = 0; x < 2; ++x) { mbar_init(s_full(x), 1); mbar_init(s_empty(x), 8); }
+        for (int s = 0; s < ST; ++s) { mbar_init(k_full(s), 1); mbar_init(v_full(s), 1); mbar_init(empty(s), 1); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot, dp_at = tmem + 256, dq_at = tmem + 384;
+    auto s_at = [&](int x) { return tmem + 128 * x; };
+    const int total = list_size;
+
+    if (warp == 0) {
+        if (lane == 0 && total) {
+            mbar_expect_tx(q_full, 2 * OP);
+            for (int x = 0; x < DP / 64; ++x) {
+                tma_load_4d(q_at + x * kBox, &map_q, q_full, 64 * x, q0, h, b);
+                tma_load_4d(do_at + x * kBox, &map_do, q_full, 64 * x, q0, h, b);
+            }
+            bool ok = true;
+            int i = 0;
+            for (; i < total && ok; ++i) {
+                const int s = i % ST, key0 = (list[i] & 0x7fff) * kTile;
+                ok = mbar_wait(empty(s), (i / ST & 1) ^ 1, ab, 41);
+                if (!ok) break;
+                mbar_expect_tx(k_full(s), OP);
+                for (int x = 0; x < DP / 64; ++x) tma_load_4d(k_at(s) + x * kBox, &map_k, k_full(s), 64 * x, key0, kvh, b);
+                mbar_expect_tx(v_full(s), OP);
+                for (int x = 0; x < DP / 64; ++x) tma_load_4d(v_at(s) + x * kBox, &map_v, v_full(s), 64 * x, key0, kvh, b);
+            }
+            for (int k = 0; k < ST && ok; ++k, ++i) ok = mbar_wait(empty(i % ST), (i / ST & 1) ^ 1, ab, 41);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && total) {
+            bool ok = mbar_wait(q_full, 0, ab, 42);
+            auto scores = [&](int i) {
+                ok = ok && mbar_wait(k_full(i % ST), i / ST & 1, ab, 43);
+                if (ok && (list[i] & 0x7fff) == blank_tile) {            // warp 2 blanks the rows behind key_len first
+                    mbar_arrive(blank_go);
+                    ok = mbar_wait(blanked, 0, ab, 43);
+                }
+                ok = ok && mbar_wait(s_empty(i & 1), (i / 2 & 1) ^ 1, ab, 44);
+                if (!ok) return;
+                fence_after();
+                product_nt<DP, kTile>(s_at(i & 1), q_at, k_at(i % ST), 0);
+                commit(s_full(i & 1));
+            };
+            auto gaps = [&](int i) {
+                ok = ok && mbar_wait(v_full(i % ST), i / ST & 1, ab, 45);
+                if (!ok) return;
+                fence_after();
+                product_nt<DP, kTile>(dp_at, do_at, v_at(i % ST), 0);
+                commit(dp_full);
+            };
+            scores(0);
+            gaps(0);
+            for (int i = 0; i < total && ok; ++i) {
+                if (i + 1 < total) scores(i + 1);                        // runs while the gradients of tile i are computed
+                ok = ok && mbar_wait(ds_ready, i & 1, ab, 46);
+                if (!ok) break;
+                fence_after();
+                product_halves<DP>(dq_at, dp_at, k_at(i % ST), i > 0);
+                commit(empty(i % ST));
+                if (i + 1 < total) gaps(i + 1);
+            }
+            commit(done);
+        }
+    } else if (warp == 2) {
+        if (total && blank_tile >= 0 && (list[total - 1] & 0x7fff) == blank_tile) {
+            const int s = (total - 1) % ST;
+            if (warp_wait(blank_go, 0, ab, 47)) {
+                for (int x = 0; x < DP / 64; ++x)
+                    for (int i = m.keys % kTile * 8 + lane; i < kTile * 8; i += 32)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(k_at(s) + x * kBox + i * 16), "r"(0) : "memory");
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(blanked);
+            }
+        }
+    } else if (warp >= 4) {
+        const int w = warp / 4 - 1, t = q0 + (threadIdx.x & 127);
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+        const bool live = t < p.a.q_len;
+        const int pos = m.start + t, end = live ? key_end(m, pos) : 0;
+        const int my_doc = DOCS && live ? m.q_docs[t] : 0;
+        const float slope = BIAS ? p.a.slopes[h] * kLog2e : 0.f;
+        const int64_t line = ((int64_t)b * p.a.heads + h) * p.a.q_len + t;
+        float lse2 = live ? p.a.lse[line] * kLog2e : INFINITY;
+        if (lse2 == -INFINITY) lse2 = INFINITY;
+        const float delta = live ? p.a.delta[line] : 0.f;
+        int* my_docs = docs + (warp - 4) * 64;
+        bool ok = true;
+        for (int i = 0; i < total; ++i) {
+            const int entry = list[i], key0 = (entry & 0x7fff) * kTile + 64 * w;
+            const bool partial = entry & 0x8000;
+            if (DOCS && partial) {
+                __syncwarp();
+                for (int k = lane; k < 64; k += 32) my_docs[k] = key0 + k < p.a.k_len ? m.k_docs[key0 + k] : 0;
+                __syncwarp();
+            }
+            ok = warp_wait(s_full(i & 1), i / 2 & 1, ab, 48);
+            if (!ok) break;
+            fence_after();
+            float g[64];
+            ld32(s_at(i & 1) + lanes + 64 * w, reinterpret_cast<uint32_t*>(g));
+            ld32(s_at(i & 1) + lanes + 64 * w + 32, reinterpret_cast<uint32_t*>(g) + 32);
+            wait_ld();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_empty(i & 1));
+            const float ahead = (float)(pos - key0);
+            const int left = end - key0;
+#pragma unroll
+            for (int c = 0; c < 64; ++c) {
+                float dcap;
+                float z = score_and_slope<CAP>(p, g[c], dcap);
+                if (BIAS) z = fmaf(-slope, fabsf(ahead - (float)c), z);
+                g[c] = ex2(z - lse2) * dcap;
+            }
+            if (partial) {
+#pragma unroll
+                for (int c = 0; c < 64; ++c) if (c >= left || (DOCS && my_docs[c] != my_doc)) g[c] = 0.f;
+            }
+            ok = warp_wait(dp_full, i & 1, ab, 49);
+            if (!ok) break;
+            fence_after();
+            float gap[64];
+            ld32(dp_at + lanes + 64 * w, reinterpret_cast<uint32_t*>(gap));
+            ld32(dp_at + lanes + 64 * w + 32, reinterpret_cast<uint32_t*>(gap) + 32);
+            wait_ld();
+            uint32_t pk[32];
+#pragma unroll
+            for (int c = 0; c < 64; c += 2) {
+                const float x = partial && g[c] == 0.f ? 0.f : g[c] * (gap[c] - delta), y = partial && g[c + 1] == 0.f ? 0.f : g[c + 1] * (gap[c + 1] - delta);
+                pk[c / 2] = pack_bf16x2(x, y);
+            }
+            st32(dp_at + lanes + 64 * w, pk);
+            wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ds_ready);
+        }
+        if (ok && total) ok = warp_wait(done, 0, ab, 50);
+        if (ok) {
+            fence_after();
+            bf16* out = (bf16*)p.a.dq + (int64_t)b * p.a.dqs.b + (int64_t)t * p.a.dqs.t + (int64_t)h * p.a.dqs.h;
+#pragma unroll 1
+            for (int x = w * (DP / 2); x < (w + 1) * (DP / 2); x += 32) {          // a half of the columns each
+                uint32_t o[32];
+                if (total) { ld32(dq_at + lanes + x, o); wait_ld(); }
+                else for (int i = 0; i < 32; ++i) o[i] = 0;
+                if (live) store_row32(out, x, p.a.dim, o, p.a.scale);
+            }
+        }
+    }
+    __syncwarp();
+    if (ab.flag) {
+        const unsigned long long t0 = global_ns();
+        while (global_ns() - t0 < 200000ull) { }
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+template <int DP, bool CAP, bool BIAS, bool DOCS>
+void launch_backward(ormi_b200_ctx* ctx, const CUtensorMap* maps, const TcParams& p) {
+    constexpr int smem = BackShape<DP>::kSmem;
+    auto kv = attn_back_kv<DP, CAP, BIAS, DOCS>;
+    auto q = attn_back_q<DP, CAP, BIAS, DOCS>;
+    ORMI_CUDA(cudaFuncSetAttribute(kv, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    ORMI_CUDA(cudaFuncSetAttribute(q, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kv<<<dim3(p.a.batch * p.a.kv_heads, (p.a.k_len + kTile - 1) / kTile), kThreads, smem, ctx->stream>>>(maps[0], maps[1], maps[2], maps[3], p);
+    q<<<dim3(p.a.batch * p.a.heads, (p.a.q_len + kTile - 1) / kTile), kThreads, smem, ctx->stream>>>(maps[0], maps[1], maps[2], maps[3], p);
+    ORMI_CUDA(cudaGetLastError());
+    count_launch(ctx, 2);
+}
+
+template <int DP>
+void launch_by_mask(ormi_b200_ctx* ctx, const CUtensorMap* maps, const TcParams& p) {
+    const bool cap = p.a.cap > 0.f, bias = p.a.slopes, docs = p.a.k_docs;
+    if (cap) {
+        if (bias) docs ? launch_backward<DP, true, true, true>(ctx, maps, p) : launch_backward<DP, true, true, false>(ctx, maps, p);
+        else docs ? launch_backward<DP, true, false, true>(ctx, maps, p) : launch_backward<DP, true, false, false>(ctx, maps, p);
+    } else {
+        if (bias) docs ? launch_backward<DP, false, true, true>(ctx, maps, p) : launch_backward<DP, false, true, false>(ctx, maps, p);
+        else docs ? launch_backward<DP, false, false, true>(ctx, maps, p) : launch_backward<DP, false, false, false>(ctx, maps, p);
+    }
+}
+
+}  // namespace
+
+bool attention_backward_tc_supported(const AttnParams& p, int dtype) {
+    return attention_tc_supported(p, dtype) && p.q_len >= 1 && p.q_len <= kMaxTiles * kTile && map_allowed(p.dout, p.dos, p.batch, p.q_len, p.heads) &&
+           map_allowed(p.dq, p.dqs, p.batch, p.q_len, p.heads) && map_allowed(p.dk, p.dks, p.batch, p.k_len, p.kv_heads) && map_allowed(p.dv, p.dvs, p.batch, p.k_len, p.kv_heads);
+}
+
+void attention_backward_tc(ormi_b200_ctx* ctx, AttnParams& a) {
+    Scratch bounds(ctx, bounds_bytes(a));
+    const TcParams p = tc_params(ctx, a, (int2*)bounds.ptr);
+    CUtensorMap maps[4];
+    head_map(ctx, &maps[0], a.q, a.qs, a.batch, a.q_len, a.heads, a.dim);
+    head_map(ctx, &maps[1], a.k, a.ks, a.batch, a.k_len, a.kv_heads, a.dim);
+    head_map(ctx, &maps[2], a.v, a.vs, a.batch, a.k_len, a.kv_heads, a.dim);
+    head_map(ctx, &maps[3], a.dout, a.dos, a.batch, a.q_len, a.heads, a.dim);
+    if (a.dim <= 64) launch_by_mask<64>(ctx, maps, p); else launch_by_mask<128>(ctx, maps, p);
+    bounds.release();
+}
+
+}  // namespace ormi_b200

@@ -42,6 +42,8 @@ __device__ __forceinline__ float score_log2(const TcParams& p, float raw) {
 
 bool attention_tc_supported(const AttnParams& p, int dtype);
 void attention_tc(ormi_b200_ctx* ctx, AttnParams& p);
+bool attention_backward_tc_supported(const AttnParams& p, int dtype);
+void attention_backward_tc(ormi_b200_ctx* ctx, AttnParams& p);
 
 // host side (attention_tc.cu)
 void head_map(ormi_b200_ctx* ctx, CUtensorMap* map, const void* ptr, const Strides4& s, int batch, int len, int heads, int dim);
