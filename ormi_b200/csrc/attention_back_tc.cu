@@ -20,7 +20,7 @@ using namespace tc;
 
 constexpr int kThreads = 384;
 
-struct Stat { float lse2[kTile], delta[kTile]; int end[kTile], doc[kTile]; };      // of 128 queries
+struct Stat { float lse2[kTile], delta[kTile]; int end[kTile], doc[kTile]; };      // of 128 queries; the first two negated
 
 template <int DP> struct BackShape {
     static constexpr int kOperand = kTile * DP * 2;
@@ -40,15 +40,6 @@ __device__ __forceinline__ int list_tiles(unsigned short* list, int tiles, F&& c
         n += __popc(hit);
     }
     return n;
-}
-
-// Base-2 score and the derivative of the cap, from the raw product.
-template <bool CAP>
-__device__ __forceinline__ float score_and_slope(const TcParams& p, float raw, float& dcap) {
-    if (!CAP) { dcap = 1.f; return raw * p.scale_log2; }
-    const float r = __fdividef(1.f, ex2(raw * p.scale_log2) + 1.f);             // tanh = 1 - 2 r, 1 - tanh^2 = 4 r (1 - r)
-    dcap = 4.f * r * (1.f - r);
-    return fmaf(-2.f * p.cap_log2, r, p.cap_log2);
 }
 
 // 32 columns of tensor memory to 32 bf16 values of a row, times `by`.
@@ -182,7 +173,7 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             commit(done);
         }
     } else if (warp == 2) {
-        // the queries' statistics; a row that sees nothing, or does not exist, gets +infinity: its probabilities vanish
+        // the queries' statistics; a row that sees nothing, or does not exist, gets an infinite one: its probabilities vanish
         for (int i = 0; i < total; ++i) {
             const int s = i % ST, h = kvh * p.a.group + i / per_head, q0 = (list[i % per_head] & 0x7fff) * kTile;
             float l[4], d[4];
@@ -201,7 +192,7 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             if (!warp_wait(stat_empty(s), (i / ST & 1) ^ 1, ab, 37)) break;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                stats[s].lse2[k * 32 + lane] = l[k]; stats[s].delta[k * 32 + lane] = d[k];
+                stats[s].lse2[k * 32 + lane] = -l[k]; stats[s].delta[k * 32 + lane] = -d[k];
                 stats[s].end[k * 32 + lane] = e[k];
                 if (DOCS) stats[s].doc[k * 32 + lane] = doc[k];
             }
@@ -223,37 +214,42 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             ok = warp_wait(stat_full(s), i / ST & 1, ab, 38) && warp_wait(s_full, i & 1, ab, 38);
             if (!ok) break;
             fence_after();
-            float g[64];
-            ld32(s_at + lanes + 64 * w, reinterpret_cast<uint32_t*>(g));
-            ld32(s_at + lanes + 64 * w + 32, reinterpret_cast<uint32_t*>(g) + 32);
+            float2 z[32], g[32];                        // g: what the gradient of a raw product is a multiple of
+            ld32(s_at + lanes + 64 * w, reinterpret_cast<uint32_t*>(z));
+            ld32(s_at + lanes + 64 * w + 32, reinterpret_cast<uint32_t*>(z) + 32);
             wait_ld();
+            if (CAP) cap_scores<32, true>(p, z, g);
+            if (BIAS) {
+#pragma unroll
+                for (int c = 0; c < 32; ++c) {
+                    if (!CAP) z[c] = mul2(z[c], both(p.scale_log2));
+                    z[c] = make_float2(fmaf(-slope, fabsf(ahead + (float)(2 * c)), z[c].x), fmaf(-slope, fabsf(ahead + (float)(2 * c + 1)), z[c].y));
+                }
+            }
             uint32_t pk[32];
 #pragma unroll
-            for (int c = 0; c < 64; c += 4) {
-                const float4 l = *reinterpret_cast<const float4*>(&st.lse2[64 * w + c]);
-                const float lse2[4] = {l.x, l.y, l.z, l.w};
-                float prob[4];
+            for (int c = 0; c < 32; c += 2) {
+                const float4 l = *reinterpret_cast<const float4*>(&st.lse2[64 * w + 2 * c]);
+                float2 a[2] = {make_float2(l.x, l.y), make_float2(l.z, l.w)};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    float dcap;
-                    float z = score_and_slope<CAP>(p, g[c + k], dcap);
-                    if (BIAS) z = fmaf(-slope, fabsf(ahead + (float)(c + k)), z);
-                    prob[k] = ex2(z - lse2[k]);
-                    g[c + k] = dcap;
+                for (int k = 0; k < 2; ++k) {
+                    a[k] = CAP || BIAS ? add2(z[c + k], a[k]) : fma2(z[c + k], both(p.scale_log2), a[k]);
+                    z[c + k] = make_float2(ex2(a[k].x), ex2(a[k].y));
                 }
                 if (partial) {
-                    const int4 e = *reinterpret_cast<const int4*>(&st.end[64 * w + c]);
-                    const int end[4] = {e.x, e.y, e.z, e.w};
-                    int4 dd = make_int4(0, 0, 0, 0);
-                    if (DOCS) dd = *reinterpret_cast<const int4*>(&st.doc[64 * w + c]);
-                    const int doc[4] = {dd.x, dd.y, dd.z, dd.w};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) if (key >= end[k] || (DOCS && doc[k] != my_doc)) { prob[k] = 0.f; g[c + k] = 0.f; }
+                    const int4 e = *reinterpret_cast<const int4*>(&st.end[64 * w + 2 * c]);
+                    int4 d = make_int4(my_doc, my_doc, my_doc, my_doc);
+                    if (DOCS) d = *reinterpret_cast<const int4*>(&st.doc[64 * w + 2 * c]);
+                    if ((key >= e.x) | (d.x != my_doc)) { z[c].x = 0.f; if (CAP) g[c].x = 0.f; }
+                    if ((key >= e.y) | (d.y != my_doc)) { z[c].y = 0.f; if (CAP) g[c].y = 0.f; }
+                    if ((key >= e.z) | (d.z != my_doc)) { z[c + 1].x = 0.f; if (CAP) g[c + 1].x = 0.f; }
+                    if ((key >= e.w) | (d.w != my_doc)) { z[c + 1].y = 0.f; if (CAP) g[c + 1].y = 0.f; }
                 }
-                pk[c / 2] = pack_bf16x2(prob[0], prob[1]);
-                pk[c / 2 + 1] = pack_bf16x2(prob[2], prob[3]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) g[c + k] = CAP ? g[c + k] * prob[k] : prob[k];
+                for (int k = 0; k < 2; ++k) {
+                    pk[c + k] = pack_bf16x2(z[c + k].x, z[c + k].y);
+                    g[c + k] = CAP ? mul2(g[c + k], z[c + k]) : z[c + k];
+                }
             }
             st32(s_at + lanes + 64 * w, pk);
             wait_st();
@@ -263,19 +259,20 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             ok = warp_wait(dp_full, i & 1, ab, 39);
             if (!ok) break;
             fence_after();
-            float gap[64];
+            float2 gap[32];
             ld32(dp_at + lanes + 64 * w, reinterpret_cast<uint32_t*>(gap));
             ld32(dp_at + lanes + 64 * w + 32, reinterpret_cast<uint32_t*>(gap) + 32);
             wait_ld();
+            if (partial) {                              // a masked pair's V may hold anything
 #pragma unroll
-            for (int c = 0; c < 64; c += 4) {
-                const float4 d = *reinterpret_cast<const float4*>(&st.delta[64 * w + c]);
-                const float delta[4] = {d.x, d.y, d.z, d.w};
-                float ds[4];
+                for (int c = 0; c < 32; ++c) { if (g[c].x == 0.f) gap[c].x = 0.f; if (g[c].y == 0.f) gap[c].y = 0.f; }
+            }
 #pragma unroll
-                for (int k = 0; k < 4; ++k) ds[k] = partial && g[c + k] == 0.f ? 0.f : g[c + k] * (gap[c + k] - delta[k]);
-                pk[c / 2] = pack_bf16x2(ds[0], ds[1]);
-                pk[c / 2 + 1] = pack_bf16x2(ds[2], ds[3]);
+            for (int c = 0; c < 32; c += 2) {
+                const float4 d = *reinterpret_cast<const float4*>(&st.delta[64 * w + 2 * c]);
+                const float2 x = mul2(g[c], add2(gap[c], make_float2(d.x, d.y))), y = mul2(g[c + 1], add2(gap[c + 1], make_float2(d.z, d.w)));
+                pk[c] = pack_bf16x2(x.x, x.y);
+                pk[c + 1] = pack_bf16x2(y.x, y.y);
             }
             st32(dp_at + lanes + 64 * w, pk);
             wait_st();
@@ -456,38 +453,49 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
             ok = warp_wait(s_full(i & 1), i / 2 & 1, ab, 48);
             if (!ok) break;
             fence_after();
-            float g[64];
-            ld32(s_at(i & 1) + lanes + 64 * w, reinterpret_cast<uint32_t*>(g));
-            ld32(s_at(i & 1) + lanes + 64 * w + 32, reinterpret_cast<uint32_t*>(g) + 32);
+            float2 z[32], g[32];
+            ld32(s_at(i & 1) + lanes + 64 * w, reinterpret_cast<uint32_t*>(z));
+            ld32(s_at(i & 1) + lanes + 64 * w + 32, reinterpret_cast<uint32_t*>(z) + 32);
             wait_ld();
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(s_empty(i & 1));
             const float ahead = (float)(pos - key0);
             const int left = end - key0;
+            if (CAP) cap_scores<32, true>(p, z, g);
 #pragma unroll
-            for (int c = 0; c < 64; ++c) {
-                float dcap;
-                float z = score_and_slope<CAP>(p, g[c], dcap);
-                if (BIAS) z = fmaf(-slope, fabsf(ahead - (float)c), z);
-                g[c] = ex2(z - lse2) * dcap;
+            for (int c = 0; c < 32; ++c) {
+                if (BIAS) {
+                    if (!CAP) z[c] = mul2(z[c], both(p.scale_log2));
+                    z[c] = make_float2(fmaf(-slope, fabsf(ahead - (float)(2 * c)), z[c].x), fmaf(-slope, fabsf(ahead - (float)(2 * c + 1)), z[c].y));
+                }
+                z[c] = CAP || BIAS ? add2(z[c], both(-lse2)) : fma2(z[c], both(p.scale_log2), both(-lse2));
+                z[c] = make_float2(ex2(z[c].x), ex2(z[c].y));
+                g[c] = CAP ? mul2(g[c], z[c]) : z[c];
             }
             if (partial) {
 #pragma unroll
-                for (int c = 0; c < 64; ++c) if (c >= left || (DOCS && my_docs[c] != my_doc)) g[c] = 0.f;
+                for (int c = 0; c < 32; ++c) {
+                    if ((2 * c >= left) | (DOCS && my_docs[2 * c] != my_doc)) g[c].x = 0.f;
+                    if ((2 * c + 1 >= left) | (DOCS && my_docs[2 * c + 1] != my_doc)) g[c].y = 0.f;
+                }
             }
             ok = warp_wait(dp_full, i & 1, ab, 49);
             if (!ok) break;
             fence_after();
-            float gap[64];
+            float2 gap[32];
             ld32(dp_at + lanes + 64 * w, reinterpret_cast<uint32_t*>(gap));
             ld32(dp_at + lanes + 64 * w + 32, reinterpret_cast<uint32_t*>(gap) + 32);
             wait_ld();
+            if (partial) {                              // a masked pair's V may hold anything
+#pragma unroll
+                for (int c = 0; c < 32; ++c) { if (g[c].x == 0.f) gap[c].x = 0.f; if (g[c].y == 0.f) gap[c].y = 0.f; }
+            }
             uint32_t pk[32];
 #pragma unroll
-            for (int c = 0; c < 64; c += 2) {
-                const float x = partial && g[c] == 0.f ? 0.f : g[c] * (gap[c] - delta), y = partial && g[c + 1] == 0.f ? 0.f : g[c + 1] * (gap[c + 1] - delta);
-                pk[c / 2] = pack_bf16x2(x, y);
+            for (int c = 0; c < 32; ++c) {
+                const float2 x = mul2(g[c], add2(gap[c], both(-delta)));
+                pk[c] = pack_bf16x2(x.x, x.y);
             }
             st32(dp_at + lanes + 64 * w, pk);
             wait_st();

@@ -190,24 +190,44 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             ok = warp_wait(s_full(w), n & 1, ab, 28);
             if (!ok) break;
             fence_after();
-            float z[128];
+            float2 z[64];
 #pragma unroll
             for (int i = 0; i < 4; ++i) ld32(s_at(w) + lanes + 32 * i, reinterpret_cast<uint32_t*>(z) + 32 * i);
             wait_ld();
+            // With neither cap nor bias the raw products go through max and exponential as they are, the scale (positive)
+            // riding on the subtraction of the maximum.
+            constexpr bool PLAIN = !CAP && !BIAS;
+            if (CAP) cap_scores<64, false>(p, z, nullptr);
+            if (BIAS) {
+                const float ahead = (float)(pos - key0);
+                if (__all_sync(0xffffffffu, pos - key0 >= kTile - 1)) {          // every key at or before the query: the distance is linear
+                    const float first = -slope * ahead;
 #pragma unroll
-            for (int i = 0; i < 128; ++i) {
-                z[i] = score_log2<CAP>(p, z[i]);
-                if (BIAS) z[i] = fmaf(-slope, fabsf((float)(pos - key0) - (float)i), z[i]);
+                    for (int i = 0; i < 64; ++i) {
+                        const float2 far = fma2(both(slope), make_float2((float)(2 * i), (float)(2 * i + 1)), both(first));
+                        z[i] = CAP ? add2(z[i], far) : fma2(z[i], both(p.scale_log2), far);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) {
+                        if (!CAP) z[i] = mul2(z[i], both(p.scale_log2));
+                        z[i] = make_float2(fmaf(-slope, fabsf(ahead - (float)(2 * i)), z[i].x), fmaf(-slope, fabsf(ahead - (float)(2 * i + 1)), z[i].y));
+                    }
+                }
             }
             if (c == kPartial) {
                 const int left = end - key0;
 #pragma unroll
-                for (int i = 0; i < 128; ++i) if (i >= left || (DOCS && my_docs[i] != my_doc)) z[i] = -INFINITY;
+                for (int i = 0; i < 64; ++i) {
+                    if ((2 * i >= left) | (DOCS && my_docs[2 * i] != my_doc)) z[i].x = -INFINITY;
+                    if ((2 * i + 1 >= left) | (DOCS && my_docs[2 * i + 1] != my_doc)) z[i].y = -INFINITY;
+                }
             }
-            float mx[4] = {z[0], z[1], z[2], z[3]};
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 4; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], z[i]);
-            const float big = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+            for (int i = 0; i < 64; ++i) mx[i & 3] = max3(mx[i & 3], z[i].x, z[i].y);
+            const float seen = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            const float big = fmaxf(top, PLAIN ? seen * p.scale_log2 : seen);
             if (__any_sync(0xffffffffu, big > top + 8.f)) {
                 const float by = big == -INFINITY ? 1.f : ex2(top - big);
                 top = big;
@@ -225,20 +245,20 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 }
             }
             const float from = top == -INFINITY ? 0.f : top;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            float2 sum[2] = {both(0.f), both(0.f)};
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 uint32_t pk[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float a = ex2(z[32 * x + 2 * i] - from), d = ex2(z[32 * x + 2 * i + 1] - from);
-                    sum[2 * i & 3] += a;
-                    sum[(2 * i + 1) & 3] += d;
-                    pk[i] = pack_bf16x2(a, d);
+                    const float2 a = PLAIN ? fma2(z[16 * x + i], both(p.scale_log2), both(-from)) : add2(z[16 * x + i], both(-from));
+                    const float2 e = make_float2(ex2(a.x), ex2(a.y));
+                    sum[i & 1] = add2(sum[i & 1], e);
+                    pk[i] = pack_bf16x2(e.x, e.y);
                 }
                 st16(s_at(w) + lanes + 16 * x, pk);
             }
-            total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            total += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             wait_st();
             fence_before();
             __syncwarp();
@@ -284,19 +304,24 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     }
 }
 
-// Smallest and largest document of every tile of 128 positions: a warp per tile.
-__global__ void __launch_bounds__(256) attn_doc_bounds(const int32_t* docs, int batch, int len, int tiles, int2* bounds) {
-    const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (at >= (int64_t)batch * tiles) return;
-    const int b = at / tiles, j = at % tiles, lane = threadIdx.x & 31;
+// Smallest and largest document of every tile of 128 positions, of the queries and then of the keys: a warp per tile.
+__global__ void __launch_bounds__(256) attn_doc_bounds(TcParams p, int2* bounds) {
+    int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t q_count = (int64_t)p.a.batch * p.q_tiles;
+    if (at >= q_count + (int64_t)p.a.batch * p.k_tiles) return;
+    bounds += at;
+    const bool keys = at >= q_count;
+    if (keys) at -= q_count;
+    const int tiles = keys ? p.k_tiles : p.q_tiles, len = keys ? p.a.k_len : p.a.q_len;
+    const int32_t* docs = (keys ? p.a.k_docs : p.a.q_docs) + at / tiles * len;
+    const int j = at % tiles, lane = threadIdx.x & 31;
     int lo = INT32_MAX, hi = INT32_MIN;
     for (int i = j * kTile + lane; i < min((j + 1) * kTile, len); i += 32) {
-        const int d = docs[(int64_t)b * len + i];
-        lo = min(lo, d); hi = max(hi, d);
+        lo = min(lo, docs[i]); hi = max(hi, docs[i]);
     }
     lo = __reduce_min_sync(0xffffffffu, lo);
     hi = __reduce_max_sync(0xffffffffu, hi);
-    if (lane == 0) bounds[at] = make_int2(lo, hi);
+    if (lane == 0) *bounds = make_int2(lo, hi);
 }
 
 template <int DP, bool CAP, bool BIAS, bool DOCS>
@@ -350,23 +375,27 @@ TcParams tc_params(ormi_b200_ctx* ctx, const AttnParams& a, int2* bounds) {
     p.q_tiles = (a.q_len + kTile - 1) / kTile;
     p.q_tiles += p.q_tiles & 1;                                  // a block looks at two tiles of queries
     p.k_tiles = (a.k_len + kTile - 1) / kTile;
-    p.scale_log2 = a.cap > 0.f ? 2.f * kLog2e * a.scale / a.cap : a.scale * kLog2e;
+    p.scale_log2 = a.scale * kLog2e;
     p.cap_log2 = a.cap * kLog2e;
+    if (a.cap > 0.f) {
+        p.x_per_raw = a.scale / a.cap;
+        p.exp_per_raw = 2.f * kLog2e * a.scale / a.cap;
+        p.poly_limit = 0.5f * a.cap / a.scale;
+    }
     p.err = device_error_word(ctx);
     ctx->gemm_err_pending = true;
     if (a.k_docs) {
         int2* kb = bounds + (size_t)a.batch * p.q_tiles;
-        attn_doc_bounds<<<(int)(((int64_t)a.batch * p.q_tiles + 7) / 8), 256, 0, ctx->stream>>>(a.q_docs, a.batch, a.q_len, p.q_tiles, bounds);
-        attn_doc_bounds<<<(int)(((int64_t)a.batch * p.k_tiles + 7) / 8), 256, 0, ctx->stream>>>(a.k_docs, a.batch, a.k_len, p.k_tiles, kb);
+        attn_doc_bounds<<<(int)(((int64_t)a.batch * (p.q_tiles + p.k_tiles) + 7) / 8), 256, 0, ctx->stream>>>(p, bounds);
         ORMI_CUDA(cudaGetLastError());
-        count_launch(ctx, 2);
+        count_launch(ctx);
         p.q_bounds = bounds; p.k_bounds = kb;
     }
     return p;
 }
 
 bool attention_tc_supported(const AttnParams& p, int dtype) {
-    return dtype == ORMI_BF16 && p.dim <= 128 && p.dim % 8 == 0 && p.k_len >= 1 && p.k_len <= kMaxTiles * kTile && p.q_len <= 65535 * 2 * kTile &&
+    return dtype == ORMI_BF16 && p.scale > 0.f && p.dim <= 128 && p.dim % 8 == 0 && p.k_len >= 1 && p.k_len <= kMaxTiles * kTile && p.q_len <= 65535 * 2 * kTile &&
            (int64_t)p.batch * p.heads < 0x7fffffff && map_allowed(p.q, p.qs, p.batch, p.q_len, p.heads) && map_allowed(p.k, p.ks, p.batch, p.k_len, p.kv_heads) &&
            map_allowed(p.v, p.vs, p.batch, p.k_len, p.kv_heads) && map_allowed(p.out, p.os, p.batch, p.q_len, p.heads);
 }
