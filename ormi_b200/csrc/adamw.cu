@@ -87,8 +87,17 @@ __device__ __forceinline__ Rates rates_of(const Common& c) {
 __device__ __forceinline__ float next_m(const Common& c, float m, float g) { return __fadd_rn(__fmul_rn(c.b1, m), __fmul_rn(c.c1, g)); }
 __device__ __forceinline__ float next_v(const Common& c, float v, float g) { return __fadd_rn(__fmul_rn(c.b2, v), __fmul_rn(__fmul_rn(c.c2, g), g)); }
 
-__device__ __forceinline__ float updated(float p, float m, float v, float decay, const Rates& r, float eps) {
-    return p - (r.lr * decay * p + r.lr * (m * r.inv_bc1) / (sqrtf(v) * r.inv_sqrt_bc2 + eps));
+// The quotient is an approximate one (2 ulp of the update, which is a small part of the parameter): an exact division costs
+// as much as the rest of the update.
+__device__ __forceinline__ float updated(float p, float m, float root, float decay, const Rates& r, float eps) {
+    return p - (r.lr * decay * p + __fdividef(r.lr * (m * r.inv_bc1), root * r.inv_sqrt_bc2 + eps));
+}
+
+// Four gradients from element i on.
+__device__ __forceinline__ float4 grads4(const Tensor& t, int64_t i) {
+    if (t.grad_f32) return *reinterpret_cast<const float4*>((const float*)t.grad + i);
+    const uint2 u = *reinterpret_cast<const uint2*>((const bf16*)t.grad + i);
+    return make_float4(bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y));
 }
 
 template <int N> __device__ __forceinline__ const Tensor& tensor_of(const Batch<N>& b, int chunk) {
@@ -111,16 +120,79 @@ __global__ void __launch_bounds__(kThreads) adamw_f32(const __grid_constant__ Ba
     const int64_t base = (int64_t)((int)blockIdx.x - t.first_chunk) * kChunk, end = min(base + kChunk, t.n);
     float* pm = (float*)t.m;
     float* pv = (float*)t.v;
+    if (t.vec && end - base == kChunk) {                       // four elements at a time; every load of the chunk is asked for first
+        float4 p[4], m[4], v[4], g[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t i = base + (k * kThreads + threadIdx.x) * 4;
+            p[k] = *reinterpret_cast<const float4*>(t.param + i);
+            m[k] = *reinterpret_cast<const float4*>(pm + i);
+            v[k] = *reinterpret_cast<const float4*>(pv + i);
+            g[k] = grads4(t, i);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t i = base + (k * kThreads + threadIdx.x) * 4;
+            auto one = [&](float& p, float& m, float& v, float g) {
+                m = next_m(b.c, m, g * r.gs); v = next_v(b.c, v, g * r.gs);
+                p = updated(p, m, sqrtf(v), t.decay, r, b.c.eps);
+            };
+            one(p[k].x, m[k].x, v[k].x, g[k].x); one(p[k].y, m[k].y, v[k].y, g[k].y);
+            one(p[k].z, m[k].z, v[k].z, g[k].z); one(p[k].w, m[k].w, v[k].w, g[k].w);
+            *reinterpret_cast<float4*>(t.param + i) = p[k];
+            *reinterpret_cast<float4*>(pm + i) = m[k];
+            *reinterpret_cast<float4*>(pv + i) = v[k];
+            if (t.copy16) *reinterpret_cast<uint2*>(t.copy16 + i) = make_uint2(pack_bf16x2(p[k].x, p[k].y), pack_bf16x2(p[k].z, p[k].w));
+        }
+        return;
+    }
     for (int64_t i = base + threadIdx.x; i < end; i += kThreads) {
         const float g = (t.grad_f32 ? ((const float*)t.grad)[i] : __bfloat162float(((const bf16*)t.grad)[i])) * r.gs;
         const float m = next_m(b.c, pm[i], g), v = next_v(b.c, pv[i], g);
-        const float p = updated(t.param[i], m, v, t.decay, r, b.c.eps);
+        const float p = updated(t.param[i], m, sqrtf(v), t.decay, r, b.c.eps);
         pm[i] = m; pv[i] = v; t.param[i] = p;
         if (t.copy16) t.copy16[i] = __float2bfloat16_rn(p);
     }
 }
 
-// States in 8 bits: a warp owns the 128 elements that share a scale, 4 per lane, 32 apart.
+// The 128 elements that share a scale, 4 per lane: new parameters in p, new states as codes.  The hash of element `at(k)`
+// decides its rounding.
+template <typename At>
+__device__ __forceinline__ void step_block(const Common& c, const Rates& r, float decay, uint32_t key, const float (&g)[4], const float (&cm)[4], const float (&cv)[4], float sm, float sv,
+                                           float (&p)[4], float (&qm)[4], float (&qv)[4], float& hi_m, float& hi_v, At&& at) {
+    float m[4], root[4];
+    uint32_t top_m = 0, top_v = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float grad = __fmul_rn(g[k], r.gs), old = __fmul_rn(cv[k], sv);
+        m[k] = next_m(c, __fmul_rn(cm[k], sm), grad);
+        root[k] = sqrtf(next_v(c, __fmul_rn(old, old), grad));
+        p[k] = updated(p[k], m[k], root[k], decay, r, c.eps);
+        top_m = max(top_m, mag(m[k]));
+        top_v = max(top_v, mag(root[k]));
+    }
+    hi_m = __uint_as_float(__reduce_max_sync(0xffffffffu, top_m));
+    hi_v = __uint_as_float(__reduce_max_sync(0xffffffffu, top_v));
+    const float up_m = codes_per_unit(hi_m), up_v = codes_per_unit(hi_v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t h = mix32((uint32_t)at(k) ^ key);
+        const float a = fminf(__fmul_rn(fabsf(m[k]), up_m), 448.f), b = fminf(__fmul_rn(root[k], up_v), 448.f);
+        qm[k] = copysignf(to_e4m3_grid(a, (float)(h & 0xffffu) * (1.f / 65536.f)), m[k]);
+        qv[k] = to_e4m3_grid(root[k] > 0.f ? fmaxf(b, 0x1p-9f) : 0.f, (float)(h >> 16) * (1.f / 65536.f));
+    }
+}
+
+__device__ __forceinline__ void codes4(uint32_t u, float (&v)[4]) {
+    const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u & 0xffff), __NV_E4M3), hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u >> 16), __NV_E4M3);
+    const float2 a = __half22float2(lo), b = __half22float2(hi);
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+}
+__device__ __forceinline__ uint32_t to_codes4(const float (&v)[4]) {
+    return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3) | (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3) << 16;
+}
+
+// States in 8 bits: a warp owns the 128 elements that share a scale; four in a row per lane where aligned, else 32 apart.
 template <int N>
 __global__ void __launch_bounds__(kThreads) adamw_e4m3(const __grid_constant__ Batch<N> b) {
     __shared__ Rates shared_rates;
@@ -130,39 +202,60 @@ __global__ void __launch_bounds__(kThreads) adamw_e4m3(const __grid_constant__ B
     const Tensor& t = tensor_of(b, blockIdx.x);
     const int64_t base = (int64_t)((int)blockIdx.x - t.first_chunk) * kChunk, end = min(base + kChunk, t.n);
     const uint32_t key = mix32(r.key + (uint32_t)t.index);
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     e4m3* cm = (e4m3*)t.m;
     e4m3* cv = (e4m3*)t.v;
-    for (int64_t first = base + (threadIdx.x >> 5) * 128; first < end; first += kThreads / 32 * 128) {
-        const float sm = t.m_scales[first >> 7], sv = t.v_scales[first >> 7];
-        float m[4], root[4];
-        uint32_t top_m = 0, top_v = 0;
-        for (int k = 0; k < 4; ++k) {
-            const int64_t i = first + k * 32 + lane;
-            m[k] = root[k] = 0.f;
-            if (i >= end) continue;
-            const float g = (t.grad_f32 ? ((const float*)t.grad)[i] : __bfloat162float(((const bf16*)t.grad)[i])) * r.gs;
-            const float old = __fmul_rn(float(cv[i]), sv);
-            m[k] = next_m(b.c, __fmul_rn(float(cm[i]), sm), g);
-            const float v = next_v(b.c, __fmul_rn(old, old), g);
-            const float p = updated(t.param[i], m[k], v, t.decay, r, b.c.eps);
-            t.param[i] = p;
-            if (t.copy16) t.copy16[i] = __float2bfloat16_rn(p);
-            root[k] = sqrtf(v);
-            top_m = max(top_m, mag(m[k]));
-            top_v = max(top_v, mag(root[k]));
+    if (t.vec && end - base == kChunk) {
+        constexpr int TURNS = kChunk / (kThreads / 32 * 128);
+        float4 pp[TURNS], gg[TURNS];
+        uint32_t um[TURNS], uv[TURNS];
+        float sm[TURNS], sv[TURNS];
+#pragma unroll
+        for (int k = 0; k < TURNS; ++k) {
+            const int64_t first = base + (k * (kThreads / 32) + warp) * 128, i = first + lane * 4;
+            pp[k] = *reinterpret_cast<const float4*>(t.param + i);
+            gg[k] = grads4(t, i);
+            um[k] = *reinterpret_cast<const uint32_t*>(cm + i);
+            uv[k] = *reinterpret_cast<const uint32_t*>(cv + i);
+            sm[k] = t.m_scales[first >> 7]; sv[k] = t.v_scales[first >> 7];
         }
-        const float hi_m = __uint_as_float(__reduce_max_sync(0xffffffffu, top_m)), hi_v = __uint_as_float(__reduce_max_sync(0xffffffffu, top_v));
-        const float up_m = codes_per_unit(hi_m), up_v = codes_per_unit(hi_v);
-        for (int k = 0; k < 4; ++k) {
-            const int64_t i = first + k * 32 + lane;
-            if (i >= end) continue;
-            const uint32_t h = mix32((uint32_t)i ^ key);
-            const float a = fminf(__fmul_rn(fabsf(m[k]), up_m), 448.f), c = fminf(__fmul_rn(root[k], up_v), 448.f);
-            const float qm = to_e4m3_grid(a, (float)(h & 0xffffu) * (1.f / 65536.f));
-            const float qv = to_e4m3_grid(root[k] > 0.f ? fmaxf(c, 0x1p-9f) : 0.f, (float)(h >> 16) * (1.f / 65536.f));
-            cm[i] = from_f32<e4m3>(copysignf(qm, m[k]));
-            cv[i] = from_f32<e4m3>(qv);
+#pragma unroll
+        for (int k = 0; k < TURNS; ++k) {
+            const int64_t first = base + (k * (kThreads / 32) + warp) * 128, i = first + lane * 4;
+            float p[4] = {pp[k].x, pp[k].y, pp[k].z, pp[k].w}, m[4], v[4], qm[4], qv[4], hi_m, hi_v;
+            const float g[4] = {gg[k].x, gg[k].y, gg[k].z, gg[k].w};
+            codes4(um[k], m);
+            codes4(uv[k], v);
+            step_block(b.c, r, t.decay, key, g, m, v, sm[k], sv[k], p, qm, qv, hi_m, hi_v, [&](int e) { return i + e; });
+            *reinterpret_cast<float4*>(t.param + i) = make_float4(p[0], p[1], p[2], p[3]);
+            *reinterpret_cast<uint32_t*>(cm + i) = to_codes4(qm);
+            *reinterpret_cast<uint32_t*>(cv + i) = to_codes4(qv);
+            if (t.copy16) *reinterpret_cast<uint2*>(t.copy16 + i) = make_uint2(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]));
+            if (lane == 0) { t.m_scales[first >> 7] = hi_m * (1.f / 448.f); t.v_scales[first >> 7] = hi_v * (1.f / 448.f); }
+        }
+        return;
+    }
+    for (int64_t first = base + warp * 128; first < end; first += kThreads / 32 * 128) {
+        const float sm = t.m_scales[first >> 7], sv = t.v_scales[first >> 7];
+        float p[4], g[4], m[4], v[4], qm[4], qv[4], hi_m, hi_v;
+        auto at = [&](int e) { return first + e * 32 + lane; };
+        // behind the end: zeros, which leave zeros
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool in = at(e) < end;
+            p[e] = in ? t.param[at(e)] : 0.f;
+            g[e] = !in ? 0.f : t.grad_f32 ? ((const float*)t.grad)[at(e)] : __bfloat162float(((const bf16*)t.grad)[at(e)]);
+            m[e] = in ? float(cm[at(e)]) : 0.f;
+            v[e] = in ? float(cv[at(e)]) : 0.f;
+        }
+        step_block(b.c, r, t.decay, key, g, m, v, sm, sv, p, qm, qv, hi_m, hi_v, at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (at(e) >= end) continue;
+            t.param[at(e)] = p[e];
+            if (t.copy16) t.copy16[at(e)] = __float2bfloat16_rn(p[e]);
+            cm[at(e)] = from_f32<e4m3>(qm[e]);
+            cv[at(e)] = from_f32<e4m3>(qv[e]);
         }
         if (lane == 0) { t.m_scales[first >> 7] = hi_m * (1.f / 448.f); t.v_scales[first >> 7] = hi_v * (1.f / 448.f); }
     }
@@ -198,26 +291,26 @@ void* kept_copy(ormi_b200_ctx* ctx, const ormi_b200_adamw_tensor& t) {
 
 void adamw_check(const ormi_b200_adamw_tensor* t, int n, const ormi_b200_adamw_config& c) {
     const char* op = "adamw";
-    op_need(c.state_bits == 32 || c.state_bits == 8, op, "state_bits is 32 or 8");
-    op_need(c.device_step || c.step >= 1, op, "step counts from 1");
-    op_need(c.beta1 >= 0 && c.beta1 < 1 && c.beta2 >= 0 && c.beta2 < 1, op, "beta1 and beta2 lie in [0, 1)");
-    op_need(c.eps >= 0 && std::isfinite(c.eps), op, "eps is negative or not finite");
-    op_need(std::isfinite(c.lr), op, "lr is not finite");
-    op_need((uintptr_t)c.device_step % 8 == 0 && (uintptr_t)c.device_lr % 4 == 0 && (uintptr_t)c.grad_scale % 4 == 0, op, "a device scalar does not start on a whole element");
+    OP_NEED(c.state_bits == 32 || c.state_bits == 8, op, "state_bits is 32 or 8");
+    OP_NEED(c.device_step || c.step >= 1, op, "step counts from 1");
+    OP_NEED(c.beta1 >= 0 && c.beta1 < 1 && c.beta2 >= 0 && c.beta2 < 1, op, "beta1 and beta2 lie in [0, 1)");
+    OP_NEED(c.eps >= 0 && std::isfinite(c.eps), op, "eps is negative or not finite");
+    OP_NEED(std::isfinite(c.lr), op, "lr is not finite");
+    OP_NEED((uintptr_t)c.device_step % 8 == 0 && (uintptr_t)c.device_lr % 4 == 0 && (uintptr_t)c.grad_scale % 4 == 0, op, "a device scalar does not start on a whole element");
     struct Range { const char* lo; const char* hi; bool out; int tensor; };
     std::vector<Range> ranges;
     for (int i = 0; i < n; ++i) {
         const ormi_b200_adamw_tensor& x = t[i];
-        const std::string who = "tensor " + std::to_string(i) + ": ";
-        op_need(x.n >= 0 && x.n < (int64_t)1 << 40, op, who + "n is negative or above 2^40");
+        auto who = [&] { return "tensor " + std::to_string(i) + ": "; };
+        OP_NEED(x.n >= 0 && x.n < (int64_t)1 << 40, op, who() + "n is negative or above 2^40");
         if (x.n == 0) continue;
-        op_need(x.param && x.grad && x.m && x.v, op, who + "param, grad, m and v are needed");
-        op_need(x.grad_dtype == ORMI_F32 || x.grad_dtype == ORMI_BF16, op, who + "grad is F32 or BF16");
-        op_need(std::isfinite(x.weight_decay), op, who + "weight_decay is not finite");
-        op_need((x.m_scales && x.v_scales) == (c.state_bits == 8) && (c.state_bits == 8 || (!x.m_scales && !x.v_scales)), op, who + "m_scales and v_scales go with 8-bit states, and only with them");
+        OP_NEED(x.param && x.grad && x.m && x.v, op, who() + "param, grad, m and v are needed");
+        OP_NEED(x.grad_dtype == ORMI_F32 || x.grad_dtype == ORMI_BF16, op, who() + "grad is F32 or BF16");
+        OP_NEED(std::isfinite(x.weight_decay), op, who() + "weight_decay is not finite");
+        OP_NEED((x.m_scales && x.v_scales) == (c.state_bits == 8) && (c.state_bits == 8 || (!x.m_scales && !x.v_scales)), op, who() + "m_scales and v_scales go with 8-bit states, and only with them");
         const uintptr_t state = c.state_bits == 32 ? 4 : 1;
-        op_need((uintptr_t)x.param % 4 == 0 && (uintptr_t)x.grad % dtype_bytes(x.grad_dtype) == 0 && (uintptr_t)x.m % state == 0 && (uintptr_t)x.v % state == 0 &&
-                (uintptr_t)x.m_scales % 4 == 0 && (uintptr_t)x.v_scales % 4 == 0 && (uintptr_t)x.copy16 % 2 == 0, op, who + "a buffer does not start on a whole element");
+        OP_NEED((uintptr_t)x.param % 4 == 0 && (uintptr_t)x.grad % dtype_bytes(x.grad_dtype) == 0 && (uintptr_t)x.m % state == 0 && (uintptr_t)x.v % state == 0 &&
+                (uintptr_t)x.m_scales % 4 == 0 && (uintptr_t)x.v_scales % 4 == 0 && (uintptr_t)x.copy16 % 2 == 0, op, who() + "a buffer does not start on a whole element");
         auto add = [&](const void* p, int64_t bytes, bool out) { if (p) ranges.push_back({(const char*)p, (const char*)p + bytes, out, i}); };
         add(x.param, x.n * 4, true); add(x.grad, x.n * dtype_bytes(x.grad_dtype), false);
         add(x.m, x.n * (int64_t)state, true); add(x.v, x.n * (int64_t)state, true);
@@ -228,7 +321,7 @@ void adamw_check(const ormi_b200_adamw_tensor* t, int n, const ormi_b200_adamw_c
     std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.lo < b.lo; });
     const char* end_any = nullptr; const char* end_out = nullptr;
     for (const Range& r : ranges) {
-        op_need(!(r.lo < end_out || (r.out && r.lo < end_any)), op, "tensor " + std::to_string(r.tensor) + ": a buffer that is written overlaps another one");
+        OP_NEED(!(r.lo < end_out || (r.out && r.lo < end_any)), op, "tensor " + std::to_string(r.tensor) + ": a buffer that is written overlaps another one");
         end_any = std::max(end_any, r.hi);
         if (r.out) end_out = std::max(end_out, r.hi);
     }
@@ -265,6 +358,8 @@ void adamw(ormi_b200_ctx* ctx, const ormi_b200_adamw_tensor* t, int n, const orm
                 d.copy16 = (bf16*)(x.copy16 ? x.copy16 : kept);
                 d.n = x.n; d.decay = x.weight_decay; d.first_chunk = (int)chunks; d.index = i;
                 d.grad_f32 = x.grad_dtype == ORMI_F32;
+                const uintptr_t states = (uintptr_t)x.m | (uintptr_t)x.v;
+                d.vec = ((uintptr_t)x.param | (c.state_bits == 32 ? states : states * 4)) % 16 == 0 && (uintptr_t)x.grad % (d.grad_f32 ? 16 : 8) == 0 && (uintptr_t)d.copy16 % 8 == 0;
                 chunks += mine;
                 auto note = [&](void* p, size_t bytes) { written(ctx, p, bytes); };
                 if (c.state_bits == 32) { note(x.m, (size_t)x.n * 4); note(x.v, (size_t)x.n * 4); }

@@ -398,10 +398,10 @@ namespace {
 
 void heads_check(const char* op, const char* name, const ormi_b200_view& v, const ormi_b200_view& like, bool same_shape, bool output) {
     view_check(op, name, v, 4, 4);
-    const std::string n(name);
-    op_need(v.dtype == like.dtype, op, n + " has another type than q");
-    op_need(v.shape[3] <= 1 || v.strides[3] == 1, op, n + ": head_dim is not contiguous");
-    if (same_shape) for (int d = 0; d < 4; ++d) op_need(v.shape[d] == like.shape[d], op, n + " has another shape");
+    auto n = [&] { return std::string(name); };
+    OP_NEED(v.dtype == like.dtype, op, n() + " has another type than q");
+    OP_NEED(v.shape[3] <= 1 || v.strides[3] == 1, op, n() + ": head_dim is not contiguous");
+    if (same_shape) for (int d = 0; d < 4; ++d) OP_NEED(v.shape[d] == like.shape[d], op, n() + " has another shape");
     if (output && count_of(v)) {
         // rows of head_dim values that lie apart: sorted by stride, each dimension steps over everything inside it
         int order[3] = {0, 1, 2};
@@ -409,7 +409,7 @@ void heads_check(const char* op, const char* name, const ormi_b200_view& v, cons
         int64_t inner = v.shape[3];
         for (int d : order) {
             if (v.shape[d] <= 1) continue;
-            op_need(v.strides[d] >= inner, op, n + ": its rows overlap");
+            OP_NEED(v.strides[d] >= inner, op, n() + ": its rows overlap");
             inner = (v.shape[d] - 1) * v.strides[d] + inner;
         }
     }
@@ -418,51 +418,51 @@ void heads_check(const char* op, const char* name, const ormi_b200_view& v, cons
 void ints_check(const char* op, const char* name, const ormi_b200_view& v, int64_t rows, int64_t cols) {
     if (!v.data) return;
     view_check(op, name, v, cols < 0 ? 1 : 2, cols < 0 ? 1 : 2);
-    op_need(v.dtype == ORMI_I32 && contiguous(v) && v.shape[0] == rows && (cols < 0 || v.shape[1] == cols), op,
+    OP_NEED(v.dtype == ORMI_I32 && contiguous(v) && v.shape[0] == rows && (cols < 0 || v.shape[1] == cols), op,
             std::string(name) + (cols < 0 ? " is not [batch] I32, contiguous" : " is not [batch, length] I32, contiguous"));
 }
 
 void forward_check(const char* op, const ormi_b200_attention_args& a, bool backward) {
     view_check(op, "q", a.q, 4, 4);
-    op_need(a.q.dtype == ORMI_F32 || a.q.dtype == ORMI_BF16, op, "q is F32 or BF16");
+    OP_NEED(a.q.dtype == ORMI_F32 || a.q.dtype == ORMI_BF16, op, "q is F32 or BF16");
     heads_check(op, "q", a.q, a.q, true, false);
     heads_check(op, "k", a.k, a.q, false, false);
     heads_check(op, "v", a.v, a.k, true, false);
     heads_check(op, "out", a.out, a.q, true, !backward);
     const int64_t b = a.q.shape[0], nq = a.q.shape[1], h = a.q.shape[2], d = a.q.shape[3], nk = a.k.shape[1], hk = a.k.shape[2];
-    op_need(a.k.shape[0] == b && a.k.shape[3] == d, op, "k has another batch or head_dim than q");
-    op_need(d >= 1 && d <= 256, op, "head_dim is 1 to 256");
-    op_need(h == 0 || (hk >= 1 && h % hk == 0), op, "heads is not a multiple of kv_heads");
-    op_need(h > 0 || hk == 0, op, "heads is zero");
-    op_need(b * hk <= 65535, op, "batch * kv_heads is above 65535");
-    op_need(b * h * nq < ((int64_t)1 << 31) && nq * (hk ? h / hk : 1) < ((int64_t)1 << 31) - 256 && nk < ((int64_t)1 << 31) - 256, op, "too many rows");
+    OP_NEED(a.k.shape[0] == b && a.k.shape[3] == d, op, "k has another batch or head_dim than q");
+    OP_NEED(d >= 1 && d <= 256, op, "head_dim is 1 to 256");
+    OP_NEED(h == 0 || (hk >= 1 && h % hk == 0), op, "heads is not a multiple of kv_heads");
+    OP_NEED(h > 0 || hk == 0, op, "heads is zero");
+    OP_NEED(b * hk <= 65535, op, "batch * kv_heads is above 65535");
+    OP_NEED(b * h * nq < ((int64_t)1 << 31) && nq * (hk ? h / hk : 1) < ((int64_t)1 << 31) - 256 && nk < ((int64_t)1 << 31) - 256, op, "too many rows");
     if (a.lse.data || backward) {
         view_check(op, "lse", a.lse, 3, 3);
-        op_need(a.lse.dtype == ORMI_F32 && contiguous(a.lse) && a.lse.shape[0] == b && a.lse.shape[1] == h && a.lse.shape[2] == nq, op, "lse is not [batch, heads, q_len] F32, contiguous");
+        OP_NEED(a.lse.dtype == ORMI_F32 && contiguous(a.lse) && a.lse.shape[0] == b && a.lse.shape[1] == h && a.lse.shape[2] == nq, op, "lse is not [batch, heads, q_len] F32, contiguous");
     }
     if (a.slopes.data) {
         view_check(op, "slopes", a.slopes, 1, 1);
-        op_need(a.slopes.dtype == ORMI_F32 && contiguous(a.slopes) && a.slopes.shape[0] == h, op, "slopes is not [heads] F32, contiguous");
+        OP_NEED(a.slopes.dtype == ORMI_F32 && contiguous(a.slopes) && a.slopes.shape[0] == h, op, "slopes is not [heads] F32, contiguous");
     }
-    op_need((a.q_docs.ndim == 0) == (a.k_docs.ndim == 0), op, "q_docs and k_docs go together");
+    OP_NEED((a.q_docs.ndim == 0) == (a.k_docs.ndim == 0), op, "q_docs and k_docs go together");
     ints_check(op, "q_docs", a.q_docs, b, nq);
     ints_check(op, "k_docs", a.k_docs, b, nk);
     ints_check(op, "prefix", a.prefix, b, -1);
     ints_check(op, "key_len", a.key_len, b, -1);
     ints_check(op, "q_start", a.q_start, b, -1);
-    op_need(std::isfinite(a.scale), op, "scale is not finite");
-    op_need(a.cap >= 0.f && std::isfinite(a.cap), op, "cap is negative or not finite");
-    op_need(a.causal || !a.prefix.data, op, "prefix goes with causal");
+    OP_NEED(std::isfinite(a.scale), op, "scale is not finite");
+    OP_NEED(a.cap >= 0.f && std::isfinite(a.cap), op, "cap is negative or not finite");
+    OP_NEED(a.causal || !a.prefix.data, op, "prefix goes with causal");
 }
 
 struct Named { const char* name; const ormi_b200_view* v; };
 
 void apart_check(const char* op, const std::vector<Named>& outs, const std::vector<Named>& ins) {
     for (size_t i = 0; i < outs.size(); ++i) {
-        for (auto& in : ins) op_need(!overlap(*outs[i].v, *in.v), op, std::string(outs[i].name) + " overlaps " + in.name);
+        for (auto& in : ins) OP_NEED(!overlap(*outs[i].v, *in.v), op, std::string(outs[i].name) + " overlaps " + in.name);
         // outputs may be slices of one buffer; the same place twice is a mistake
         for (size_t j = 0; j < i; ++j)
-            op_need(!outs[i].v->data || outs[i].v->data != outs[j].v->data || count_of(*outs[i].v) == 0 || count_of(*outs[j].v) == 0, op,
+            OP_NEED(!outs[i].v->data || outs[i].v->data != outs[j].v->data || count_of(*outs[i].v) == 0 || count_of(*outs[j].v) == 0, op,
                     std::string(outs[i].name) + " and " + outs[j].name + " are the same buffer");
     }
 }
@@ -492,7 +492,7 @@ AttnParams params_of(const ormi_b200_attention_args& a) {
 void attention_check(const ormi_b200_attention_args& a) {
     forward_check("attention", a, false);
     apart_check("attention", {{"out", &a.out}, {"lse", &a.lse}}, inputs_of(a));
-    op_need(!overlap(a.out, a.lse), "attention", "out overlaps lse");
+    OP_NEED(!overlap(a.out, a.lse), "attention", "out overlaps lse");
 }
 
 void attention(ormi_b200_ctx* ctx, const ormi_b200_attention_args& a) {

@@ -21,9 +21,9 @@ void attention_backward(ormi_b200_ctx* ctx, const ormi_b200_attention_backward_a
 void adamw_check(const ormi_b200_adamw_tensor* t, int n, const ormi_b200_adamw_config& c);
 void adamw(ormi_b200_ctx* ctx, const ormi_b200_adamw_tensor* t, int n, const ormi_b200_adamw_config& c);
 
-inline void op_need(bool ok, const char* op, const std::string& what) {
-    if (!ok) throw Error(std::string("ormi_b200_") + op + ": " + what);
-}
+[[noreturn]] inline void op_fail(const char* op, const std::string& what) { throw Error(std::string("ormi_b200_") + op + ": " + what); }
+// The text is only put together when the check fails: small calls are bound by the host.
+#define OP_NEED(ok, op, what) do { if (!(ok)) op_fail(op, what); } while (0)
 
 inline int dtype_bytes(int dtype) { return dtype == ORMI_F32 || dtype == ORMI_I32 ? 4 : dtype == ORMI_BF16 ? 2 : 1; }
 
@@ -51,19 +51,19 @@ inline bool same_place(const ormi_b200_view& a, const ormi_b200_view& b) {
 
 // The checks every view goes through: rank, extents, strides whose span fits in 63 bits, alignment to the element.
 inline void view_check(const char* op, const char* name, const ormi_b200_view& v, int lo_rank, int hi_rank) {
-    const std::string n(name);
-    op_need(v.ndim >= 1 && v.ndim <= 4, op, v.data ? n + " has " + std::to_string(v.ndim) + " dimensions" : n + " is missing");
+    auto n = [&] { return std::string(name); };
+    OP_NEED(v.ndim >= 1 && v.ndim <= 4, op, v.data ? n() + " has " + std::to_string(v.ndim) + " dimensions" : n() + " is missing");
     int64_t count = 1;
     for (int d = 0; d < v.ndim; ++d) count *= v.shape[d] != 0;
-    op_need(v.data || !count, op, n + " is missing");              // nothing at no address is an empty buffer
-    op_need(v.dtype >= ORMI_F32 && v.dtype <= ORMI_I32, op, n + " has an unknown type");
-    op_need(v.ndim >= lo_rank && v.ndim <= hi_rank, op, n + " has " + std::to_string(v.ndim) + " dimensions, " +
+    OP_NEED(v.data || !count, op, n() + " is missing");              // nothing at no address is an empty buffer
+    OP_NEED(v.dtype >= ORMI_F32 && v.dtype <= ORMI_I32, op, n() + " has an unknown type");
+    OP_NEED(v.ndim >= lo_rank && v.ndim <= hi_rank, op, n() + " has " + std::to_string(v.ndim) + " dimensions, " +
             (lo_rank == hi_rank ? std::to_string(lo_rank) : std::to_string(lo_rank) + " to " + std::to_string(hi_rank)) + " wanted");
     for (int d = 0; d < v.ndim; ++d) {
-        op_need(v.shape[d] >= 0 && v.shape[d] < (int64_t)1 << 31, op, n + " has an extent below zero or above 2^31 - 1");
-        op_need(v.strides[d] >= 0 && v.strides[d] < (int64_t)1 << 40, op, n + " has a stride below zero or above 2^40");
+        OP_NEED(v.shape[d] >= 0 && v.shape[d] < (int64_t)1 << 31, op, n() + " has an extent below zero or above 2^31 - 1");
+        OP_NEED(v.strides[d] >= 0 && v.strides[d] < (int64_t)1 << 40, op, n() + " has a stride below zero or above 2^40");
     }
-    op_need((uintptr_t)v.data % dtype_bytes(v.dtype) == 0, op, n + " does not start on a whole element");
+    OP_NEED((uintptr_t)v.data % dtype_bytes(v.dtype) == 0, op, n() + " does not start on a whole element");
 }
 inline int64_t count_of(const ormi_b200_view& v) {
     int64_t n = 1;

@@ -81,6 +81,165 @@ __global__ void __launch_bounds__(256) norm_any(NormParams p) {
     }
 }
 
+// Four 32-bit registers of a row: 16 bytes of it where everything is aligned, else four single elements 32 columns apart.
+template <typename T, bool AL> struct Piece {
+    static constexpr int VEC = AL ? 16 / (int)sizeof(T) : 4;
+    static constexpr int CHUNK = 32 * VEC;                     // columns of a warp's 32 pieces
+    uint32_t w[4];
+    // column of element e: first + e where aligned, first + 32 e where not
+    static __device__ __forceinline__ int first(int chunk) { return chunk * CHUNK + (threadIdx.x & 31) * (AL ? VEC : 1); }
+    static __device__ __forceinline__ int col(int c0, int e) { return c0 + (AL ? e : 32 * e); }
+    __device__ __forceinline__ void load(const T* row, int c0, int cols) {
+        if (AL) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (c0 < cols) v = *reinterpret_cast<const uint4*>(row + c0);
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = c0 + 32 * e < cols ? __float_as_uint(to_f32(row[c0 + 32 * e])) : 0u;
+        }
+    }
+    __device__ __forceinline__ float get(int e) const {
+        if (AL && sizeof(T) == 2) return e & 1 ? bf16_hi(w[e >> 1]) : bf16_lo(w[e >> 1]);
+        return __uint_as_float(w[e]);
+    }
+};
+
+// VEC values to a row of type O, in Piece order.
+template <typename O, bool AL, int VEC>
+__device__ __forceinline__ void put(O* row, int c0, int cols, const float (&v)[VEC]) {
+    if (!AL) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) if (c0 + 32 * e < cols) row[c0 + 32 * e] = from_f32<O>(v[e]);
+        return;
+    }
+    if (c0 >= cols) return;
+    if (sizeof(O) == 4) {
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4) *reinterpret_cast<float4*>((float*)row + c0 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+    } else if (sizeof(O) == 2) {
+        uint32_t u[VEC / 2];
+#pragma unroll
+        for (int e = 0; e < VEC; e += 2) u[e / 2] = pack_bf16x2(v[e], v[e + 1]);
+        if (VEC == 8) *reinterpret_cast<uint4*>(row + c0) = make_uint4(u[0], u[1], u[2 % (VEC / 2)], u[3 % (VEC / 2)]);
+        else *reinterpret_cast<uint2*>(row + c0) = make_uint2(u[0], u[1]);
+    } else {
+        uint32_t u[VEC / 4];
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4)
+            u[e / 4] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[e], v[e + 1]), __NV_SATFINITE, __NV_E4M3) |
+                       (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[e + 2], v[e + 3]), __NV_SATFINITE, __NV_E4M3) << 16;
+        if (VEC == 8) *reinterpret_cast<uint2*>(row + c0) = make_uint2(u[0], u[1 % (VEC / 4)]);
+        else *reinterpret_cast<uint32_t*>(row + c0) = u[0];
+    }
+}
+
+template <bool AL, int VEC>
+__device__ __forceinline__ void weights(const void* w, int f32, int c0, int cols, float (&v)[VEC]) {
+    if (!w) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = 1.f;
+    } else if (!AL) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = c0 + 32 * e < cols ? weight_at(w, f32, c0 + 32 * e) : 0.f;
+    } else if (c0 >= cols) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = 0.f;
+    } else if (f32) {
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4) {
+            const float4 x = __ldg(reinterpret_cast<const float4*>((const float*)w + c0 + e));
+            v[e] = x.x; v[e + 1] = x.y; v[e + 2] = x.z; v[e + 3] = x.w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4) {
+            const uint2 x = __ldg(reinterpret_cast<const uint2*>((const bf16*)w + c0 + e));
+            v[e] = bf16_lo(x.x); v[e + 1] = bf16_hi(x.x); v[e + 2] = bf16_lo(x.y); v[e + 3] = bf16_hi(x.y);
+        }
+    }
+}
+
+// One row per block (of as many warps as the row needs), or per warp for narrow rows: the row is read once and stays in
+// registers, four pieces per thread, so that all its loads are in flight together.
+template <typename T, typename O, bool AL, bool WARP_ROW>
+__global__ void __launch_bounds__(WARP_ROW ? 256 : 1024) norm_row(NormParams p) {
+    using P = Piece<T, AL>;
+    constexpr int NV = 4, VEC = P::VEC;
+    __shared__ float box[33];
+    const int warp = threadIdx.x >> 5, nw = WARP_ROW ? 1 : blockDim.x >> 5;
+    const int64_t row = WARP_ROW ? (int64_t)blockIdx.x * 8 + warp : blockIdx.x;
+    if (WARP_ROW && row >= p.rows) return;
+    const T* x = (const T*)p.x + row * p.x_row;
+    P a[NV], r[NV];
+    int c0[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        c0[v] = P::first(WARP_ROW ? v : v * nw + warp);
+        a[v].load(x, c0[v], p.cols);
+    }
+    if (p.residual) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) r[v].load((const T*)p.residual + row * p.residual_row, c0[v], p.cols);
+    }
+    float s[NV][VEC], sq = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            s[v][e] = a[v].get(e);
+            if (p.residual) s[v][e] = to_f32(from_f32<T>(s[v][e] + r[v].get(e)));
+            sq = fmaf(s[v][e], s[v][e], sq);
+        }
+    }
+    if (p.residual_out) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) put<T, AL, VEC>((T*)p.residual_out + row * p.residual_out_row, c0[v], p.cols, s[v]);
+    }
+    sq = WARP_ROW ? warp_sum(sq) : block_sum(sq, box);
+    const float rstd = 1.f / sqrtf(sq / (float)p.cols + p.eps);
+    if (p.rstd && (WARP_ROW ? (threadIdx.x & 31) : threadIdx.x) == 0) p.rstd[row] = rstd;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        float w[VEC];
+        weights<AL, VEC>(p.weight, p.weight_f32, c0[v], p.cols, w);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[v][e] *= rstd * w[e];
+    }
+    if (sizeof(O) == 1) {
+        if (p.group == 0) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) m = max(m, mag(s[v][e]));
+            const float top = WARP_ROW ? __uint_as_float(__reduce_max_sync(0xffffffffu, m)) : block_max_mag(m, (uint32_t*)box);
+            const float up = top > 0.f ? 448.f * (1.f / top) : 0.f;
+            if ((WARP_ROW ? (threadIdx.x & 31) : threadIdx.x) == 0) p.scales[row] = top * (1.f / 448.f);
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s[v][e] *= up;
+        } else {
+            // 128 columns are a warp's piece, or half of it where a piece holds 8 values
+            const uint32_t half = VEC == 8 ? (threadIdx.x & 16 ? 0xffff0000u : 0x0000ffffu) : 0xffffffffu;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) m = max(m, mag(s[v][e]));
+                const float top = __uint_as_float(__reduce_max_sync(half, m));
+                const float up = top > 0.f ? 448.f * (1.f / top) : 0.f;
+                if ((threadIdx.x & (VEC == 8 ? 15 : 31)) == 0 && c0[v] < p.cols) p.scales[row * p.groups + c0[v] / 128] = top * (1.f / 448.f);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s[v][e] *= up;
+            }
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v) put<O, AL, VEC>((O*)p.out + row * p.out_row, c0[v], p.cols, s[v]);
+}
+
 struct NormBackParams {
     const void *dout, *s, *weight, *dresidual;
     const float* rstd;
@@ -131,6 +290,107 @@ __global__ void __launch_bounds__(256) norm_dweight_any(NormBackParams p) {
     }
 }
 
+// Rows in registers, as in the forward pass.  A block takes every gridDim-th row (or its warps do), keeps its columns' part of
+// dweight in registers from row to row and writes it once, and asks for the next row's values before it reduces this one.
+// With 1024 threads there are 64 registers each: the next row is not asked for ahead and the weights are read again per row.
+template <typename T, bool AL, int THREADS>                   // THREADS: 0 = a row per warp, 8 warps; else the most that a row takes
+__global__ void __launch_bounds__(THREADS ? THREADS : 256) norm_back_row(NormBackParams p) {
+    using P = Piece<T, AL>;
+    constexpr bool WARP_ROW = THREADS == 0, AHEAD = THREADS <= 512;
+    constexpr int NV = 2, VEC = P::VEC;
+    extern __shared__ float sum_dw[];                          // WARP_ROW: one row of dweight
+    __shared__ float box[2][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = WARP_ROW ? 1 : blockDim.x >> 5;
+    const int64_t step = WARP_ROW ? (int64_t)gridDim.x * 8 : gridDim.x;
+    int64_t row = WARP_ROW ? (int64_t)blockIdx.x * 8 + warp : blockIdx.x;
+    int c0[NV];
+    float w[NV][VEC], dw[NV][VEC];
+    P dy[NV], s[NV], ds[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        c0[v] = P::first(WARP_ROW ? v : v * nw + warp);
+        if (AHEAD) weights<AL, VEC>(p.weight, p.weight_f32, c0[v], p.cols, w[v]);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) dw[v][e] = 0.f;
+    }
+    auto fetch = [&](int64_t r, P (&a)[NV], P (&b)[NV], P (&c)[NV]) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            a[v].load((const T*)p.dout + r * p.dout_row, c0[v], p.cols);
+            b[v].load((const T*)p.s + r * p.s_row, c0[v], p.cols);
+            if (p.dresidual) c[v].load((const T*)p.dresidual + r * p.dresidual_row, c0[v], p.cols);
+        }
+    };
+    const float by = 1.f / (float)p.cols;
+    float rstd = 0.f;
+    if (row < p.rows) { fetch(row, dy, s, ds); rstd = p.rstd[row]; }
+    for (int turn = 0; row < p.rows; turn ^= 1) {
+        float dot = 0.f;
+        if (!AHEAD) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) weights<AL, VEC>(p.weight, p.weight_f32, c0[v], p.cols, w[v]);
+        }
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) dot = fmaf(dy[v].get(e) * w[v][e], s[v].get(e), dot);
+        const int64_t next = row + step;
+        P dy2[NV], s2[NV], ds2[NV];
+        float rstd2 = 0.f;
+        if (AHEAD && next < p.rows) { fetch(next, dy2, s2, ds2); rstd2 = p.rstd[next]; }
+        dot = warp_sum(dot);
+        if (!WARP_ROW) {
+            // one barrier per row: the two boxes take turns
+            if (lane == 0) box[turn][warp] = dot;
+            __syncthreads();
+            dot = 0.f;
+            for (int k = 0; k < nw; ++k) dot += box[turn][k];
+        }
+        const float k = dot * by * rstd * rstd;
+        T* dx = (T*)p.dx + row * p.dx_row;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            float o[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float g = dy[v].get(e), x = s[v].get(e);
+                o[e] = rstd * (g * w[v][e] - x * k);
+                if (p.dresidual) o[e] += ds[v].get(e);
+                dw[v][e] = fmaf(g, x * rstd, dw[v][e]);
+            }
+            put<T, AL, VEC>(dx, c0[v], p.cols, o);
+        }
+        row = next;
+        if (AHEAD) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) { dy[v] = dy2[v]; s[v] = s2[v]; ds[v] = ds2[v]; }
+            rstd = rstd2;
+        } else if (row < p.rows) {
+            fetch(row, dy, s, ds);
+            rstd = p.rstd[row];
+        }
+    }
+    if (!p.dweight) return;
+    float* out = p.partial + (int64_t)blockIdx.x * p.cols;
+    if (!WARP_ROW) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) { const int c = P::col(c0[v], e); if (c < p.cols) out[c] = dw[v][e]; }
+        return;
+    }
+    for (int k = 0; k < 8; ++k) {                              // the warps in order
+        if (warp == k) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) { const int c = P::col(c0[v], e); if (c < p.cols) sum_dw[c] = k ? sum_dw[c] + dw[v][e] : dw[v][e]; }
+        }
+        __syncthreads();
+    }
+    for (int c = threadIdx.x; c < p.cols; c += 256) out[c] = sum_dw[c];
+}
+
 // dweight[c] = sum of the partial rows in order: 32 columns per block, its 32 warps share the rows.
 __global__ void __launch_bounds__(1024) norm_dweight_join(const float* __restrict__ partial, int parts, int cols, void* dweight, int f32) {
     __shared__ float box[32][33];
@@ -158,7 +418,7 @@ Rows rows_of(const char* op, const char* name, const ormi_b200_view& v) {
     for (int d = v.ndim - 2; d >= 0; --d) {
         if (v.shape[d] == 1) continue;
         if (first) { r.stride = v.strides[d]; first = false; }
-        else op_need(v.strides[d] == r.rows * r.stride, op, std::string(name) + ": the leading dimensions do not collapse into one row stride");
+        else OP_NEED(v.strides[d] == r.rows * r.stride, op, std::string(name) + ": the leading dimensions do not collapse into one row stride");
         r.rows *= v.shape[d];
     }
     return r;
@@ -166,30 +426,30 @@ Rows rows_of(const char* op, const char* name, const ormi_b200_view& v) {
 
 void matrix_check(const char* op, const char* name, const ormi_b200_view& v, const ormi_b200_view& like, bool same_type) {
     view_check(op, name, v, 1, 4);
-    const std::string n(name);
-    op_need(v.ndim == like.ndim, op, n + " has another shape");
-    for (int d = 0; d < v.ndim; ++d) op_need(v.shape[d] == like.shape[d], op, n + " has another shape");
-    op_need(v.shape[v.ndim - 1] <= 1 || v.strides[v.ndim - 1] == 1 || count_of(v) == 0, op, n + ": the last dimension is not contiguous");
-    if (same_type) op_need(v.dtype == like.dtype, op, n + " has another type");
-    op_need(v.dtype == ORMI_F32 || v.dtype == ORMI_BF16 || (!same_type && v.dtype == ORMI_E4M3), op, n + " has a type that is not taken here");
+    auto n = [&] { return std::string(name); };
+    OP_NEED(v.ndim == like.ndim, op, n() + " has another shape");
+    for (int d = 0; d < v.ndim; ++d) OP_NEED(v.shape[d] == like.shape[d], op, n() + " has another shape");
+    OP_NEED(v.shape[v.ndim - 1] <= 1 || v.strides[v.ndim - 1] == 1 || count_of(v) == 0, op, n() + ": the last dimension is not contiguous");
+    if (same_type) OP_NEED(v.dtype == like.dtype, op, n() + " has another type");
+    OP_NEED(v.dtype == ORMI_F32 || v.dtype == ORMI_BF16 || (!same_type && v.dtype == ORMI_E4M3), op, n() + " has a type that is not taken here");
     rows_of(op, name, v);
 }
 
 // An output's rows must not lie on one another.
 void output_check(const char* op, const char* name, const ormi_b200_view& v) {
     const Rows r = rows_of(op, name, v);
-    op_need(r.rows <= 1 || count_of(v) == 0 || r.stride >= v.shape[v.ndim - 1], op, std::string(name) + ": its rows overlap");
+    OP_NEED(r.rows <= 1 || count_of(v) == 0 || r.stride >= v.shape[v.ndim - 1], op, std::string(name) + ": its rows overlap");
 }
 
 void weight_check(const char* op, const char* name, const ormi_b200_view& v, int64_t cols) {
     view_check(op, name, v, 1, 1);
-    op_need(v.dtype == ORMI_F32 || v.dtype == ORMI_BF16, op, std::string(name) + " is F32 or BF16");
-    op_need(v.shape[0] == cols && (cols <= 1 || v.strides[0] == 1), op, std::string(name) + " is not [cols], contiguous");
+    OP_NEED(v.dtype == ORMI_F32 || v.dtype == ORMI_BF16, op, std::string(name) + " is F32 or BF16");
+    OP_NEED(v.shape[0] == cols && (cols <= 1 || v.strides[0] == 1), op, std::string(name) + " is not [cols], contiguous");
 }
 
 void rstd_check(const char* op, const ormi_b200_view& v, int64_t rows) {
     view_check(op, "rstd", v, 1, 4);
-    op_need(v.dtype == ORMI_F32 && contiguous(v) && count_of(v) == rows, op, "rstd is not [rows] F32, contiguous");
+    OP_NEED(v.dtype == ORMI_F32 && contiguous(v) && count_of(v) == rows, op, "rstd is not [rows] F32, contiguous");
 }
 
 void apart(const char* op, const char* out_name, const ormi_b200_view& out, const char* in_name, const ormi_b200_view& in, bool in_place) {
@@ -197,27 +457,82 @@ void apart(const char* op, const char* out_name, const ormi_b200_view& out, cons
     throw Error(std::string("ormi_b200_") + op + ": " + out_name + " overlaps " + in_name);
 }
 
+// Whether 16-byte accesses (8- and 4-byte ones for narrower outputs) work on every row of a matrix.
+bool rows_aligned(const void* p, int64_t row, int elem, int vec) {
+    const int bytes = std::min(16, elem * vec);
+    return !p || ((uintptr_t)p % bytes == 0 && row * elem % bytes == 0);
+}
+
+template <typename T, typename O, bool AL>
+void launch_norm_row(ormi_b200_ctx* ctx, const NormParams& p) {
+    constexpr int chunk = Piece<T, AL>::CHUNK;
+    const int chunks = (p.cols + chunk - 1) / chunk;
+    if (chunks <= 4) norm_row<T, O, AL, true><<<(int)((p.rows + 7) / 8), 256, 0, ctx->stream>>>(p);
+    else norm_row<T, O, AL, false><<<(int)p.rows, (chunks + 3) / 4 * 32, 0, ctx->stream>>>(p);
+}
+
 template <typename T, typename O>
 void launch_norm(ormi_b200_ctx* ctx, const NormParams& p) {
-    const int grid = (int)std::min<int64_t>(p.rows, (int64_t)ctx->num_sms * 8);
-    norm_any<T, O><<<grid, 256, 0, ctx->stream>>>(p);
+    constexpr int vec = 16 / sizeof(T);
+    const bool al = p.cols % vec == 0 && rows_aligned(p.x, p.x_row, sizeof(T), vec) && rows_aligned(p.residual, p.residual_row, sizeof(T), vec) &&
+                    rows_aligned(p.residual_out, p.residual_out_row, sizeof(T), vec) && rows_aligned(p.out, p.out_row, sizeof(O), vec) &&
+                    rows_aligned(p.weight, 0, 4, 4);
+    // 32 warps of four pieces hold a row of 16384 columns, 32768 where a piece is 8 bf16 values
+    const int most = 128 * (al ? Piece<T, true>::CHUNK : Piece<T, false>::CHUNK);
+    if (p.cols <= most && p.rows < 0x7fffffff) {
+        if (al) launch_norm_row<T, O, true>(ctx, p); else launch_norm_row<T, O, false>(ctx, p);
+    } else {
+        norm_any<T, O><<<(int)std::min<int64_t>(p.rows, (int64_t)ctx->num_sms * 8), 256, 0, ctx->stream>>>(p);
+    }
     ORMI_CUDA(cudaGetLastError());
     count_launch(ctx);
 }
 
+template <typename T, bool AL, int THREADS>
+int launch_norm_back_row(ormi_b200_ctx* ctx, const NormBackParams& p, int threads, bool dry) {
+    auto kernel = norm_back_row<T, AL, THREADS>;
+    const int smem = THREADS ? 0 : p.cols * 4;
+    static int per_sm[33] = {};                                // by warps: asking costs more than a small launch
+    int& most = per_sm[threads / 32];
+    if (!most) {
+        int n = 0;
+        ORMI_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, THREADS ? 0 : 2 * Piece<T, AL>::CHUNK * 4));
+        most = std::max(1, n);
+    }
+    const int grid = (int)std::min<int64_t>(THREADS ? p.rows : (p.rows + 7) / 8, (int64_t)ctx->num_sms * most);
+    if (!dry) kernel<<<grid, threads, smem, ctx->stream>>>(p);
+    return grid;
+}
+
+template <typename T, bool AL>
+int launch_norm_back_rows(ormi_b200_ctx* ctx, const NormBackParams& p, bool dry) {
+    const int pieces = (p.cols + Piece<T, AL>::CHUNK - 1) / Piece<T, AL>::CHUNK, threads = (pieces + 1) / 2 * 32;
+    if (pieces <= 2) return launch_norm_back_row<T, AL, 0>(ctx, p, 256, dry);
+    if (threads <= 256) return launch_norm_back_row<T, AL, 256>(ctx, p, threads, dry);
+    if (threads <= 512) return launch_norm_back_row<T, AL, 512>(ctx, p, threads, dry);
+    return launch_norm_back_row<T, AL, 1024>(ctx, p, threads, dry);
+}
+
 template <typename T>
 void launch_norm_back(ormi_b200_ctx* ctx, NormBackParams& p) {
-    Scratch partial(ctx, p.dweight ? (size_t)256 * p.cols * 4 : 0);
-    if (p.dweight) {
-        p.partial = (float*)partial.ptr;
-        p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(256, p.rows / 64));
-        norm_dweight_any<T><<<dim3((p.cols + 31) / 32, p.parts), 256, 0, ctx->stream>>>(p);
-        norm_dweight_join<<<(p.cols + 31) / 32, 1024, 0, ctx->stream>>>(p.partial, p.parts, p.cols, p.dweight, p.weight_f32);
-        count_launch(ctx, 2);
+    constexpr int vec = 16 / sizeof(T);
+    const bool al = p.cols % vec == 0 && rows_aligned(p.dout, p.dout_row, sizeof(T), vec) && rows_aligned(p.s, p.s_row, sizeof(T), vec) &&
+                    rows_aligned(p.dresidual, p.dresidual_row, sizeof(T), vec) && rows_aligned(p.dx, p.dx_row, sizeof(T), vec) && rows_aligned(p.weight, 0, 4, 4);
+    // 32 warps of two pieces
+    const bool in_registers = p.rows > 0 && p.cols <= 64 * (al ? Piece<T, true>::CHUNK : Piece<T, false>::CHUNK);
+    if (in_registers) p.parts = al ? launch_norm_back_rows<T, true>(ctx, p, true) : launch_norm_back_rows<T, false>(ctx, p, true);
+    else p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(256, p.rows / 64));
+    Scratch partial(ctx, p.dweight ? (size_t)p.parts * p.cols * 4 : 0);
+    p.partial = (float*)partial.ptr;
+    if (in_registers) {
+        if (al) launch_norm_back_rows<T, true>(ctx, p, false); else launch_norm_back_rows<T, false>(ctx, p, false);
+        count_launch(ctx);
+    } else {
+        if (p.dweight) { norm_dweight_any<T><<<dim3((p.cols + 31) / 32, p.parts), 256, 0, ctx->stream>>>(p); count_launch(ctx); }
+        if (p.rows) { norm_back_any<T><<<(int)std::min<int64_t>(p.rows, (int64_t)ctx->num_sms * 8), 256, 0, ctx->stream>>>(p); count_launch(ctx); }
     }
-    if (p.rows) {
-        const int grid = (int)std::min<int64_t>(p.rows, (int64_t)ctx->num_sms * 8);
-        norm_back_any<T><<<grid, 256, 0, ctx->stream>>>(p);
+    if (p.dweight) {
+        norm_dweight_join<<<(p.cols + 31) / 32, 1024, 0, ctx->stream>>>(p.partial, p.parts, p.cols, p.dweight, p.weight_f32);
         count_launch(ctx);
     }
     ORMI_CUDA(cudaGetLastError());
@@ -230,8 +545,8 @@ void rmsnorm_check(const ormi_b200_rmsnorm_args& a) {
     const char* op = "rmsnorm";
     matrix_check(op, "x", a.x, a.x, true);
     const int64_t cols = a.x.shape[a.x.ndim - 1], rows = rows_of(op, "x", a.x).rows;
-    op_need(cols >= 1, op, "x has no columns");
-    op_need(a.eps >= 0.f, op, "eps is negative or not a number");
+    OP_NEED(cols >= 1, op, "x has no columns");
+    OP_NEED(a.eps >= 0.f, op, "eps is negative or not a number");
     if (a.residual.data) matrix_check(op, "residual", a.residual, a.x, true);
     if (a.residual_out.data) {
         matrix_check(op, "residual_out", a.residual_out, a.x, true);
@@ -241,12 +556,12 @@ void rmsnorm_check(const ormi_b200_rmsnorm_args& a) {
     matrix_check(op, "out", a.out, a.x, false);
     output_check(op, "out", a.out);
     if (a.rstd.data) rstd_check(op, a.rstd, rows);
-    op_need((a.out.dtype == ORMI_E4M3) == (a.scales.data != nullptr), op, "scales go with an E4M3 out, and only with it");
+    OP_NEED((a.out.dtype == ORMI_E4M3) == (a.scales.data != nullptr), op, "scales go with an E4M3 out, and only with it");
     if (a.scales.data) {
-        op_need(a.group == 0 || a.group == 128, op, "group is 0 (one scale for a row) or 128");
+        OP_NEED(a.group == 0 || a.group == 128, op, "group is 0 (one scale for a row) or 128");
         view_check(op, "scales", a.scales, 1, 4);
         const int64_t groups = a.group ? (cols + a.group - 1) / a.group : 1;
-        op_need(a.scales.dtype == ORMI_F32 && contiguous(a.scales) && count_of(a.scales) == rows * groups, op, "scales is not [rows, groups] F32, contiguous");
+        OP_NEED(a.scales.dtype == ORMI_F32 && contiguous(a.scales) && count_of(a.scales) == rows * groups, op, "scales is not [rows, groups] F32, contiguous");
     }
     const struct { const char* name; const ormi_b200_view& v; } outs[] = {{"out", a.out}, {"residual_out", a.residual_out}, {"rstd", a.rstd}, {"scales", a.scales}};
     const struct { const char* name; const ormi_b200_view& v; } ins[] = {{"x", a.x}, {"residual", a.residual}, {"weight", a.weight}};
@@ -284,7 +599,7 @@ void rmsnorm_backward_check(const ormi_b200_rmsnorm_backward_args& a) {
     const char* op = "rmsnorm_backward";
     matrix_check(op, "dout", a.dout, a.dout, true);
     const int64_t cols = a.dout.shape[a.dout.ndim - 1], rows = rows_of(op, "dout", a.dout).rows;
-    op_need(cols >= 1, op, "dout has no columns");
+    OP_NEED(cols >= 1, op, "dout has no columns");
     matrix_check(op, "s", a.s, a.dout, true);
     if (a.dresidual.data) matrix_check(op, "dresidual", a.dresidual, a.dout, true);
     matrix_check(op, "dx", a.dx, a.dout, true);
@@ -293,7 +608,7 @@ void rmsnorm_backward_check(const ormi_b200_rmsnorm_backward_args& a) {
     if (a.weight.data) weight_check(op, "weight", a.weight, cols);
     if (a.dweight.data) {
         weight_check(op, "dweight", a.dweight, cols);
-        if (a.weight.data) op_need(a.dweight.dtype == a.weight.dtype, op, "dweight has another type than weight");
+        if (a.weight.data) OP_NEED(a.dweight.dtype == a.weight.dtype, op, "dweight has another type than weight");
     }
     const struct { const char* name; const ormi_b200_view& v; } ins[] = {{"dout", a.dout}, {"s", a.s}, {"weight", a.weight}, {"rstd", a.rstd}, {"dresidual", a.dresidual}};
     for (int i = 0; i < 5; ++i) {
