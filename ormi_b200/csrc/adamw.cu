@@ -57,11 +57,12 @@ __host__ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
     return x ^ (x >> 16);
 }
 
-// 0 <= a <= 448 to an e4m3 value, up with the probability of the remainder; u in [0, 1).  The step below 2^-6 is 2^-9.
-__device__ __forceinline__ float to_e4m3_grid(float a, float u) {
-    const uint32_t e = max(__float_as_uint(a) >> 23, 121u);                   // biased exponent, at least that of 2^-6
-    const float step = __uint_as_float((e - 3u) << 23), inv = __uint_as_float((257u - e) << 23);
-    return fminf(floorf(a * inv + u) * step, 448.f);
+// 0 <= a <= 448 to an e4m3 value, up with the probability u / 2^16 of what it is above the value below (u: 16 bits).  From 2^-6
+// on the value below is a with the last 20 bits of its mantissa cut off: adding u << 4 carries with that probability, 448
+// itself has nothing to carry from.  Below, values are 2^-9 apart.
+__device__ __forceinline__ float to_e4m3_grid(float a, uint32_t u) {
+    if (a < 0x1p-6f) return floorf(a * 512.f + (float)u * (1.f / 65536.f)) * 0x1p-9f;
+    return __uint_as_float((__float_as_uint(a) + (u << 4)) & 0xfff00000u);
 }
 
 __device__ __forceinline__ float codes_per_unit(float top) { return top > 0.f ? __fmul_rn(1.f / top, 448.f) : 0.f; }
@@ -90,7 +91,9 @@ __device__ __forceinline__ float next_v(const Common& c, float v, float g) { ret
 // The quotient is an approximate one (2 ulp of the update, which is a small part of the parameter): an exact division costs
 // as much as the rest of the update.
 __device__ __forceinline__ float updated(float p, float m, float root, float decay, const Rates& r, float eps) {
-    return p - (r.lr * decay * p + __fdividef(r.lr * (m * r.inv_bc1), root * r.inv_sqrt_bc2 + eps));
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(root * r.inv_sqrt_bc2 + eps));
+    return p - (r.lr * decay * p + r.lr * (m * r.inv_bc1) * inv);
 }
 
 // Four gradients from element i on.
@@ -178,8 +181,8 @@ __device__ __forceinline__ void step_block(const Common& c, const Rates& r, floa
     for (int k = 0; k < 4; ++k) {
         const uint32_t h = mix32((uint32_t)at(k) ^ key);
         const float a = fminf(__fmul_rn(fabsf(m[k]), up_m), 448.f), b = fminf(__fmul_rn(root[k], up_v), 448.f);
-        qm[k] = copysignf(to_e4m3_grid(a, (float)(h & 0xffffu) * (1.f / 65536.f)), m[k]);
-        qv[k] = to_e4m3_grid(root[k] > 0.f ? fmaxf(b, 0x1p-9f) : 0.f, (float)(h >> 16) * (1.f / 65536.f));
+        qm[k] = copysignf(to_e4m3_grid(a, h & 0xffffu), m[k]);
+        qv[k] = to_e4m3_grid(b < 0x1p-9f && root[k] > 0.f ? 0x1p-9f : b, h >> 16);
     }
 }
 

@@ -5,6 +5,7 @@
 //
 // Both are bound by memory: every element is read and written once and takes a handful of operations.
 #include <algorithm>
+#include <atomic>
 
 #include "op_math.cuh"
 #include "operators.h"
@@ -291,14 +292,24 @@ __global__ void __launch_bounds__(256) norm_dweight_any(NormBackParams p) {
 }
 
 // Rows in registers, as in the forward pass.  A block takes every gridDim-th row (or its warps do), keeps its columns' part of
-// dweight in registers from row to row and writes it once, and asks for the next row's values before it reduces this one.
-// With 1024 threads there are 64 registers each: the next row is not asked for ahead and the weights are read again per row.
-template <typename T, bool AL, int THREADS>                   // THREADS: 0 = a row per warp, 8 warps; else the most that a row takes
+// dweight in registers from row to row and writes it once.  The rows to come are on their way meanwhile: aligned ones into
+// shared memory, where every thread copies (cp.async) and reads back its own pieces, so nobody waits for anybody; others
+// into registers, one row ahead.  With 1024 threads there are 64 registers each: the weights are read again for every row.
+__device__ __forceinline__ void copy16(void* to, const void* from, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(in ? 16 : 0) : "memory");
+}
+// bytes of shared memory in front of the copies, and of one row's copies
+__host__ __device__ constexpr int back_sum_bytes(bool warp_row, int chunk) { return warp_row ? 2 * chunk * 4 : 0; }
+__host__ __device__ constexpr int back_stage_bytes(int threads, int nv) { return 3 * nv * threads * 16; }
+
+template <typename T, bool AL, int THREADS, int NV, int STAGES>   // THREADS: 0 = a row per warp, 8 warps; else the most that a row takes
 __global__ void __launch_bounds__(THREADS ? THREADS : 256) norm_back_row(NormBackParams p) {
     using P = Piece<T, AL>;
-    constexpr bool WARP_ROW = THREADS == 0, AHEAD = THREADS <= 512;
-    constexpr int NV = 2, VEC = P::VEC;
-    extern __shared__ float sum_dw[];                          // WARP_ROW: one row of dweight
+    constexpr bool WARP_ROW = THREADS == 0, RING = AL, AHEAD = !RING && THREADS <= 512, HOLD = THREADS <= 512;
+    constexpr int VEC = P::VEC;
+    extern __shared__ __align__(16) unsigned char shared[];
+    float* sum_dw = reinterpret_cast<float*>(shared);          // WARP_ROW: one row of dweight
+    uint4* ring = reinterpret_cast<uint4*>(shared + back_sum_bytes(WARP_ROW, P::CHUNK));
     __shared__ float box[2][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = WARP_ROW ? 1 : blockDim.x >> 5;
     const int64_t step = WARP_ROW ? (int64_t)gridDim.x * 8 : gridDim.x;
@@ -309,7 +320,7 @@ __global__ void __launch_bounds__(THREADS ? THREADS : 256) norm_back_row(NormBac
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         c0[v] = P::first(WARP_ROW ? v : v * nw + warp);
-        if (AHEAD) weights<AL, VEC>(p.weight, p.weight_f32, c0[v], p.cols, w[v]);
+        if (HOLD) weights<AL, VEC>(p.weight, p.weight_f32, c0[v], p.cols, w[v]);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) dw[v][e] = 0.f;
     }
@@ -321,12 +332,44 @@ __global__ void __launch_bounds__(THREADS ? THREADS : 256) norm_back_row(NormBac
             if (p.dresidual) c[v].load((const T*)p.dresidual + r * p.dresidual_row, c0[v], p.cols);
         }
     };
+    auto slot = [&](int stage, int which, int v) { return ring + ((stage * 3 + which) * NV + v) * blockDim.x + threadIdx.x; };
+    auto ask = [&](int64_t r, int stage) {
+        if (r < p.rows) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const bool in = c0[v] < p.cols;
+                const int c = in ? c0[v] : 0;
+                copy16(slot(stage, 0, v), (const T*)p.dout + r * p.dout_row + c, in);
+                copy16(slot(stage, 1, v), (const T*)p.s + r * p.s_row + c, in);
+                if (p.dresidual) copy16(slot(stage, 2, v), (const T*)p.dresidual + r * p.dresidual_row + c, in);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto take = [&](int stage, int which, P (&a)[NV]) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) { const uint4 u = *slot(stage, which, v); a[v].w[0] = u.x; a[v].w[1] = u.y; a[v].w[2] = u.z; a[v].w[3] = u.w; }
+    };
     const float by = 1.f / (float)p.cols;
-    float rstd = 0.f;
-    if (row < p.rows) { fetch(row, dy, s, ds); rstd = p.rstd[row]; }
+    float rstd = row < p.rows ? p.rstd[row] : 0.f;
+    if (RING) {
+#pragma unroll
+        for (int k = 0; k < STAGES - 1; ++k) ask(row + k * step, k);
+    } else if (row < p.rows) fetch(row, dy, s, ds);
+    int stage = 0;
     for (int turn = 0; row < p.rows; turn ^= 1) {
+        const int64_t next = row + step;
+        if (RING) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+            take(stage, 0, dy);
+            take(stage, 1, s);
+            if (p.dresidual) take(stage, 2, ds);
+            const int last = stage == 0 ? STAGES - 1 : stage - 1;          // what was taken a turn ago
+            ask(row + (STAGES - 1) * step, last);
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+        }
         float dot = 0.f;
-        if (!AHEAD) {
+        if (!HOLD) {
 #pragma unroll
             for (int v = 0; v < NV; ++v) weights<AL, VEC>(p.weight, p.weight_f32, c0[v], p.cols, w[v]);
         }
@@ -334,10 +377,9 @@ __global__ void __launch_bounds__(THREADS ? THREADS : 256) norm_back_row(NormBac
         for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) dot = fmaf(dy[v].get(e) * w[v][e], s[v].get(e), dot);
-        const int64_t next = row + step;
         P dy2[NV], s2[NV], ds2[NV];
-        float rstd2 = 0.f;
-        if (AHEAD && next < p.rows) { fetch(next, dy2, s2, ds2); rstd2 = p.rstd[next]; }
+        if (AHEAD && next < p.rows) fetch(next, dy2, s2, ds2);
+        const float rstd2 = next < p.rows ? p.rstd[next] : 0.f;
         dot = warp_sum(dot);
         if (!WARP_ROW) {
             // one barrier per row: the two boxes take turns
@@ -361,14 +403,11 @@ __global__ void __launch_bounds__(THREADS ? THREADS : 256) norm_back_row(NormBac
             put<T, AL, VEC>(dx, c0[v], p.cols, o);
         }
         row = next;
+        rstd = rstd2;
         if (AHEAD) {
 #pragma unroll
             for (int v = 0; v < NV; ++v) { dy[v] = dy2[v]; s[v] = s2[v]; ds[v] = ds2[v]; }
-            rstd = rstd2;
-        } else if (row < p.rows) {
-            fetch(row, dy, s, ds);
-            rstd = p.rstd[row];
-        }
+        } else if (!RING && row < p.rows) fetch(row, dy, s, ds);
     }
     if (!p.dweight) return;
     float* out = p.partial + (int64_t)blockIdx.x * p.cols;
@@ -488,16 +527,18 @@ void launch_norm(ormi_b200_ctx* ctx, const NormParams& p) {
     count_launch(ctx);
 }
 
-template <typename T, bool AL, int THREADS>
+template <typename T, bool AL, int THREADS, int NV, int STAGES>
 int launch_norm_back_row(ormi_b200_ctx* ctx, const NormBackParams& p, int threads, bool dry) {
-    auto kernel = norm_back_row<T, AL, THREADS>;
-    const int smem = THREADS ? 0 : p.cols * 4;
-    static int per_sm[33] = {};                                // by warps: asking costs more than a small launch
-    int& most = per_sm[threads / 32];
+    auto kernel = norm_back_row<T, AL, THREADS, NV, STAGES>;
+    const int smem = back_sum_bytes(!THREADS, Piece<T, AL>::CHUNK) + (AL ? STAGES * back_stage_bytes(threads, NV) : 0);
+    // the limit holds for the current device only, so it is set by every call
+    if (smem) ORMI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, back_sum_bytes(!THREADS, Piece<T, AL>::CHUNK) + (AL ? STAGES * back_stage_bytes(THREADS ? THREADS : 256, NV) : 0)));
+    static std::atomic<int> per_sm[33];                        // by warps: asking costs more than a small launch
+    int most = per_sm[threads / 32];
     if (!most) {
         int n = 0;
-        ORMI_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, THREADS ? 0 : 2 * Piece<T, AL>::CHUNK * 4));
-        most = std::max(1, n);
+        ORMI_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem));
+        per_sm[threads / 32] = most = std::max(1, n);
     }
     const int grid = (int)std::min<int64_t>(THREADS ? p.rows : (p.rows + 7) / 8, (int64_t)ctx->num_sms * most);
     if (!dry) kernel<<<grid, threads, smem, ctx->stream>>>(p);
@@ -506,11 +547,13 @@ int launch_norm_back_row(ormi_b200_ctx* ctx, const NormBackParams& p, int thread
 
 template <typename T, bool AL>
 int launch_norm_back_rows(ormi_b200_ctx* ctx, const NormBackParams& p, bool dry) {
-    const int pieces = (p.cols + Piece<T, AL>::CHUNK - 1) / Piece<T, AL>::CHUNK, threads = (pieces + 1) / 2 * 32;
-    if (pieces <= 2) return launch_norm_back_row<T, AL, 0>(ctx, p, 256, dry);
-    if (threads <= 256) return launch_norm_back_row<T, AL, 256>(ctx, p, threads, dry);
-    if (threads <= 512) return launch_norm_back_row<T, AL, 512>(ctx, p, threads, dry);
-    return launch_norm_back_row<T, AL, 1024>(ctx, p, threads, dry);
+    // One piece per thread up to 512 threads, so that the registers allow two blocks of them; a piece of 8 bf16 values takes
+    // twice the registers of one of 4.  Three rows of copies per block, two where that would leave one block per SM.
+    const int pieces = (p.cols + Piece<T, AL>::CHUNK - 1) / Piece<T, AL>::CHUNK, warps2 = (pieces + 1) / 2;
+    if (pieces <= 2) return launch_norm_back_row<T, AL, 0, 2, 3>(ctx, p, 256, dry);
+    if (pieces <= 16) return launch_norm_back_row<T, AL, 512, 1, 3>(ctx, p, pieces * 32, dry);
+    if (warps2 <= 16) return launch_norm_back_row<T, AL, 512, 2, sizeof(T) == 4 ? 2 : 3>(ctx, p, warps2 * 32, dry);
+    return launch_norm_back_row<T, AL, 1024, 2, 2>(ctx, p, warps2 * 32, dry);
 }
 
 template <typename T>
