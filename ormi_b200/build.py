@@ -12,7 +12,7 @@ LIB = os.path.join(HERE, "libormi_b200.so")
 CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 
 SOURCES = ["abi.cu", "runtime.cu", "fusion.cpp", "codegen.cpp", "gemm_ffma.cu", "gemm_tcgen05.cu", "gemm_tc.cu", "colsum_static.cu", "comm.cu",
-           "rmsnorm.cu", "adamw.cu", "attention.cu", "attention_tc.cu", "attention_back_tc.cu"]
+           "rmsnorm.cu", "adamw.cu", "attention.cu", "attention_tc.cu", "attention_back_tc.cu", "attention_few.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-cudart", "static",

@@ -19,10 +19,14 @@
 
 #include "op_math.cuh"
 #include "operators.h"
+#include "tc.cuh"
 
 namespace ormi_b200 {
 namespace {
 
+#ifndef AB
+#define AB 4
+#endif
 constexpr int kThreads = 256;
 constexpr int kChunk = 4096;                 // elements per block: 32 blocks of 128 that share a scale
 
@@ -65,8 +69,6 @@ __device__ __forceinline__ float to_e4m3_grid(float a, uint32_t u) {
     return __uint_as_float((__float_as_uint(a) + (u << 4)) & 0xfff00000u);
 }
 
-__device__ __forceinline__ float codes_per_unit(float top) { return top > 0.f ? __fmul_rn(1.f / top, 448.f) : 0.f; }
-
 struct Rates { float lr, inv_bc1, inv_sqrt_bc2, gs; uint32_t key; };
 
 // The step number and what follows from it: from the host, or from the device counter of a captured step.
@@ -88,12 +90,12 @@ __device__ __forceinline__ Rates rates_of(const Common& c) {
 __device__ __forceinline__ float next_m(const Common& c, float m, float g) { return __fadd_rn(__fmul_rn(c.b1, m), __fmul_rn(c.c1, g)); }
 __device__ __forceinline__ float next_v(const Common& c, float v, float g) { return __fadd_rn(__fmul_rn(c.b2, v), __fmul_rn(__fmul_rn(c.c2, g), g)); }
 
+__device__ __forceinline__ float quick_inverse(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+
 // The quotient is an approximate one (2 ulp of the update, which is a small part of the parameter): an exact division costs
 // as much as the rest of the update.
 __device__ __forceinline__ float updated(float p, float m, float root, float decay, const Rates& r, float eps) {
-    float inv;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(root * r.inv_sqrt_bc2 + eps));
-    return p - (r.lr * decay * p + r.lr * (m * r.inv_bc1) * inv);
+    return p - (r.lr * decay * p + r.lr * r.inv_bc1 * m * quick_inverse(root * r.inv_sqrt_bc2 + eps));
 }
 
 // Four gradients from element i on.
@@ -119,7 +121,7 @@ __global__ void __launch_bounds__(kThreads) adamw_f32(const __grid_constant__ Ba
     if (threadIdx.x == 0) shared_rates = rates_of(b.c);
     __syncthreads();
     const Rates r = shared_rates;
-    const Tensor& t = tensor_of(b, blockIdx.x);
+    const Tensor t = tensor_of(b, blockIdx.x);
     const int64_t base = (int64_t)((int)blockIdx.x - t.first_chunk) * kChunk, end = min(base + kChunk, t.n);
     float* pm = (float*)t.m;
     float* pv = (float*)t.v;
@@ -158,32 +160,64 @@ __global__ void __launch_bounds__(kThreads) adamw_f32(const __grid_constant__ Ba
     }
 }
 
-// The 128 elements that share a scale, 4 per lane: new parameters in p, new states as codes.  The hash of element `at(k)`
-// decides its rounding.
-template <typename At>
-__device__ __forceinline__ void step_block(const Common& c, const Rates& r, float decay, uint32_t key, const float (&g)[4], const float (&cm)[4], const float (&cv)[4], float sm, float sv,
-                                           float (&p)[4], float (&qm)[4], float (&qv)[4], float& hi_m, float& hi_v, At&& at) {
-    float m[4], root[4];
+// The 128 elements that share a scale, 4 per lane: new parameters in p, new states as codes.  `h` are the elements' hashes.
+// Two elements per instruction where there is such an instruction: this kernel is bound by instructions as much as by memory.
+__device__ __forceinline__ void step_block(const Common& c, const Rates& r, float decay, const uint32_t (&h)[4], const float (&g)[4], const float (&cm)[4], const float (&cv)[4], float sm, float sv,
+                                           float (&p)[4], float (&qm)[4], float (&qv)[4], float& hi_m, float& hi_v) {
+    using namespace tc;
+    float2 m[2], root[2];
     uint32_t top_m = 0, top_v = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const float grad = __fmul_rn(g[k], r.gs), old = __fmul_rn(cv[k], sv);
-        m[k] = next_m(c, __fmul_rn(cm[k], sm), grad);
-        root[k] = sqrtf(next_v(c, __fmul_rn(old, old), grad));
-        p[k] = updated(p[k], m[k], root[k], decay, r, c.eps);
-        top_m = max(top_m, mag(m[k]));
-        top_v = max(top_v, mag(root[k]));
+    for (int k = 0; k < 2; ++k) {
+        const float2 grad = mul2(make_float2(g[2 * k], g[2 * k + 1]), both(r.gs)), old = mul2(make_float2(cv[2 * k], cv[2 * k + 1]), both(sv));
+        m[k] = add2(mul2(both(c.b1), mul2(make_float2(cm[2 * k], cm[2 * k + 1]), both(sm))), mul2(both(c.c1), grad));
+        const float2 v = add2(mul2(both(c.b2), mul2(old, old)), mul2(mul2(both(c.c2), grad), grad));
+        root[k] = make_float2(sqrtf(v.x), sqrtf(v.y));
+        const float2 den = fma2(root[k], both(r.inv_sqrt_bc2), both(c.eps));
+        const float2 up = mul2(mul2(m[k], both(r.lr * r.inv_bc1)), make_float2(quick_inverse(den.x), quick_inverse(den.y)));
+        const float2 now = make_float2(p[2 * k], p[2 * k + 1]), off = fma2(now, both(r.lr * decay), up);
+        p[2 * k] = now.x - off.x;
+        p[2 * k + 1] = now.y - off.y;
+        top_m = max(max(top_m, mag(m[k].x)), mag(m[k].y));
+        top_v = max(max(top_v, __float_as_uint(root[k].x)), __float_as_uint(root[k].y));
     }
     hi_m = __uint_as_float(__reduce_max_sync(0xffffffffu, top_m));
     hi_v = __uint_as_float(__reduce_max_sync(0xffffffffu, top_v));
-    const float up_m = codes_per_unit(hi_m), up_v = codes_per_unit(hi_v);
+    // codes per unit, 448 / top: one half of the warp divides for m, the other for sqrt(v)
+    const float mine = threadIdx.x & 16 ? hi_v : hi_m, up = mine > 0.f ? __fmul_rn(1.f / mine, 448.f) : 0.f;
+    const float2 up_m = both(__shfl_sync(0xffffffffu, up, 0)), up_v = both(__shfl_sync(0xffffffffu, up, 16));
+    uint32_t a[4], b[4], least = 0xffffffffu;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const float2 x = mul2(m[k], up_m), y = mul2(root[k], up_v);
+        // magnitudes as integers, at most 448 (a product of two roundings may lie just above)
+        a[2 * k] = min(mag(x.x), 0x43e00000u); a[2 * k + 1] = min(mag(x.y), 0x43e00000u);
+        b[2 * k] = min(__float_as_uint(y.x), 0x43e00000u); b[2 * k + 1] = min(__float_as_uint(y.y), 0x43e00000u);
+        least = min(min(least, min(a[2 * k], a[2 * k + 1])), min(b[2 * k], b[2 * k + 1]));
+    }
+    if (least >= 0x3c800000u) {                                 // 2^-6: everything has a full mantissa
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            a[k] = (a[k] + ((h[k] << 4) & 0xffff0u)) & 0xfff00000u;
+            b[k] = (b[k] + ((h[k] >> 12) & 0xffff0u)) & 0xfff00000u;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const bool some = k & 1 ? root[k / 2].y > 0.f : root[k / 2].x > 0.f;
+            a[k] = __float_as_uint(to_e4m3_grid(__uint_as_float(a[k]), h[k] & 0xffffu));
+            b[k] = __float_as_uint(to_e4m3_grid(some ? fmaxf(__uint_as_float(b[k]), 0x1p-9f) : 0.f, h[k] >> 16));
+        }
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const uint32_t h = mix32((uint32_t)at(k) ^ key);
-        const float a = fminf(__fmul_rn(fabsf(m[k]), up_m), 448.f), b = fminf(__fmul_rn(root[k], up_v), 448.f);
-        qm[k] = copysignf(to_e4m3_grid(a, h & 0xffffu), m[k]);
-        qv[k] = to_e4m3_grid(b < 0x1p-9f && root[k] > 0.f ? 0x1p-9f : b, h >> 16);
+        const float sign = k & 1 ? m[k / 2].y : m[k / 2].x;
+        qm[k] = __uint_as_float(a[k] | (__float_as_uint(sign) & 0x80000000u));
+        qv[k] = __uint_as_float(b[k]);
     }
+    // a state that is not a number stays one: the clamp above took it for a large value
+    if (!(hi_m < INFINITY)) { for (int k = 0; k < 4; ++k) qm[k] = NAN; }
+    if (!(hi_v < INFINITY)) { for (int k = 0; k < 4; ++k) qv[k] = NAN; }
 }
 
 __device__ __forceinline__ void codes4(uint32_t u, float (&v)[4]) {
@@ -197,39 +231,42 @@ __device__ __forceinline__ uint32_t to_codes4(const float (&v)[4]) {
 
 // States in 8 bits: a warp owns the 128 elements that share a scale; four in a row per lane where aligned, else 32 apart.
 template <int N>
-__global__ void __launch_bounds__(kThreads) adamw_e4m3(const __grid_constant__ Batch<N> b) {
+__global__ void __launch_bounds__(kThreads, AB) adamw_e4m3(const __grid_constant__ Batch<N> b) {
     __shared__ Rates shared_rates;
     if (threadIdx.x == 0) shared_rates = rates_of(b.c);
     __syncthreads();
     const Rates r = shared_rates;
-    const Tensor& t = tensor_of(b, blockIdx.x);
+    const Tensor t = tensor_of(b, blockIdx.x);
     const int64_t base = (int64_t)((int)blockIdx.x - t.first_chunk) * kChunk, end = min(base + kChunk, t.n);
     const uint32_t key = mix32(r.key + (uint32_t)t.index);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     e4m3* cm = (e4m3*)t.m;
     e4m3* cv = (e4m3*)t.v;
     if (t.vec && end - base == kChunk) {
+        // a warp takes four blocks, and asks for the next one's values before it works on this one
+        struct { float4 p, g; uint32_t m, v; float sm, sv; } now, next;
         constexpr int TURNS = kChunk / (kThreads / 32 * 128);
-        float4 pp[TURNS], gg[TURNS];
-        uint32_t um[TURNS], uv[TURNS];
-        float sm[TURNS], sv[TURNS];
+        auto first_of = [&](int k) { return base + (k * (kThreads / 32) + warp) * 128; };
+        auto fetch = [&](int k) {
+            const int64_t first = first_of(k), i = first + lane * 4;
+            next.p = *reinterpret_cast<const float4*>(t.param + i);
+            next.g = grads4(t, i);
+            next.m = *reinterpret_cast<const uint32_t*>(cm + i);
+            next.v = *reinterpret_cast<const uint32_t*>(cv + i);
+            next.sm = t.m_scales[first >> 7]; next.sv = t.v_scales[first >> 7];
+        };
+        fetch(0);
 #pragma unroll
         for (int k = 0; k < TURNS; ++k) {
-            const int64_t first = base + (k * (kThreads / 32) + warp) * 128, i = first + lane * 4;
-            pp[k] = *reinterpret_cast<const float4*>(t.param + i);
-            gg[k] = grads4(t, i);
-            um[k] = *reinterpret_cast<const uint32_t*>(cm + i);
-            uv[k] = *reinterpret_cast<const uint32_t*>(cv + i);
-            sm[k] = t.m_scales[first >> 7]; sv[k] = t.v_scales[first >> 7];
-        }
-#pragma unroll
-        for (int k = 0; k < TURNS; ++k) {
-            const int64_t first = base + (k * (kThreads / 32) + warp) * 128, i = first + lane * 4;
-            float p[4] = {pp[k].x, pp[k].y, pp[k].z, pp[k].w}, m[4], v[4], qm[4], qv[4], hi_m, hi_v;
-            const float g[4] = {gg[k].x, gg[k].y, gg[k].z, gg[k].w};
-            codes4(um[k], m);
-            codes4(uv[k], v);
-            step_block(b.c, r, t.decay, key, g, m, v, sm[k], sv[k], p, qm, qv, hi_m, hi_v, [&](int e) { return i + e; });
+            now = next;
+            if (k + 1 < TURNS) fetch(k + 1);
+            const int64_t first = first_of(k), i = first + lane * 4;
+            float p[4] = {now.p.x, now.p.y, now.p.z, now.p.w}, m[4], v[4], qm[4], qv[4], hi_m, hi_v;
+            const float g[4] = {now.g.x, now.g.y, now.g.z, now.g.w};
+            codes4(now.m, m);
+            codes4(now.v, v);
+            const uint32_t h[4] = {mix32((uint32_t)i ^ key), mix32((uint32_t)(i + 1) ^ key), mix32((uint32_t)(i + 2) ^ key), mix32((uint32_t)(i + 3) ^ key)};
+            step_block(b.c, r, t.decay, h, g, m, v, now.sm, now.sv, p, qm, qv, hi_m, hi_v);
             *reinterpret_cast<float4*>(t.param + i) = make_float4(p[0], p[1], p[2], p[3]);
             *reinterpret_cast<uint32_t*>(cm + i) = to_codes4(qm);
             *reinterpret_cast<uint32_t*>(cv + i) = to_codes4(qv);
@@ -251,7 +288,8 @@ __global__ void __launch_bounds__(kThreads) adamw_e4m3(const __grid_constant__ B
             m[e] = in ? float(cm[at(e)]) : 0.f;
             v[e] = in ? float(cv[at(e)]) : 0.f;
         }
-        step_block(b.c, r, t.decay, key, g, m, v, sm, sv, p, qm, qv, hi_m, hi_v, at);
+        const uint32_t h[4] = {mix32((uint32_t)at(0) ^ key), mix32((uint32_t)at(1) ^ key), mix32((uint32_t)at(2) ^ key), mix32((uint32_t)at(3) ^ key)};
+        step_block(b.c, r, t.decay, h, g, m, v, sm, sv, p, qm, qv, hi_m, hi_v);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (at(e) >= end) continue;

@@ -190,25 +190,42 @@ __global__ void __launch_bounds__(kThreads) attn_forward(AttnParams p) {
     }
 }
 
-// Joins the parts of a split: a warp per (batch, head, query).
+// Joins the parts of a split: a block per (batch, head, query), its four warps sharing the parts, a lane four columns.
 template <typename T>
-__global__ void __launch_bounds__(256) attn_join(AttnParams p) {
-    const int64_t lines = (int64_t)p.batch * p.heads * p.q_len, line = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (line >= lines) return;
-    const int lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(128) attn_join(AttnParams p) {
+    __shared__ float box[4][256];
+    __shared__ float sums[4];
+    const int64_t lines = (int64_t)p.batch * p.heads * p.q_len, line = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int t = line % p.q_len, h = line / p.q_len % p.heads, b = line / p.q_len / p.heads;
-    float top = -INFINITY, total = 0.f;
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_max[s * lines + line]);
+    float top = -INFINITY;
+    for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.part_max[s * lines + line]);
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float base = top == -INFINITY ? 0.f : top;
-    for (int s = 0; s < p.splits; ++s) total += p.part_sum[s * lines + line] * exp2f(p.part_max[s * lines + line] - base);
+    float total = 0.f;
+    for (int c = 0; c < p.dim; c += 128) {
+        float v[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+#pragma unroll 4
+        for (int s = warp; s < p.splits; s += 4) {
+            const float by = exp2f(p.part_max[s * lines + line] - base);
+            sum += by * p.part_sum[s * lines + line];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int d = c + lane + 32 * k;
+                if (d < p.dim) v[k] = fmaf(by, p.part_out[(s * lines + line) * p.dim + d], v[k]);
+            }
+        }
+        if (c == 0) total = sum;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) if (c + lane + 32 * k < p.dim) box[warp][c + lane + 32 * k] = v[k];
+    }
+    if (lane == 0) sums[warp] = total;
+    __syncthreads();
+    total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     const float by = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
     T* out = (T*)p.out + at(p.os, b, t, h);
-    for (int d = lane; d < p.dim; d += 32) {
-        float v = 0.f;
-        for (int s = 0; s < p.splits; ++s) v += p.part_out[(s * lines + line) * p.dim + d] * exp2f(p.part_max[s * lines + line] - base);
-        out[d] = from_f32<T>(v * by);
-    }
-    if (p.lse && lane == 0) p.lse[line] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
+    for (int d = threadIdx.x; d < p.dim; d += 128) out[d] = from_f32<T>(((box[0][d] + box[1][d]) + (box[2][d] + box[3][d])) * by);
+    if (p.lse && threadIdx.x == 0) p.lse[line] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
 }
 
 template <typename T>
@@ -339,11 +356,7 @@ void run_forward(ormi_b200_ctx* ctx, AttnParams& p) {
     attn_forward<T, BM, BN, DP><<<dim3(rows, pairs, p.splits), kThreads, smem, ctx->stream>>>(p);
     ORMI_CUDA(cudaGetLastError());
     count_launch(ctx);
-    if (p.splits > 1) {
-        attn_join<T><<<tiles(lines, 8), 256, 0, ctx->stream>>>(p);
-        ORMI_CUDA(cudaGetLastError());
-        count_launch(ctx);
-    }
+    if (p.splits > 1) attention_join(ctx, p, sizeof(T) == 4 ? ORMI_F32 : ORMI_BF16);
     part.release();
 }
 
@@ -383,6 +396,13 @@ void attention_simple(ormi_b200_ctx* ctx, AttnParams& p, int dtype) {
 
 void attention_backward_simple(ormi_b200_ctx* ctx, AttnParams& p, int dtype) {
     if (dtype == ORMI_F32) backward_by_size<float>(ctx, p); else backward_by_size<bf16>(ctx, p);
+}
+
+void attention_join(ormi_b200_ctx* ctx, const AttnParams& p, int dtype) {
+    const int64_t lines = (int64_t)p.batch * p.heads * p.q_len;
+    if (dtype == ORMI_F32) attn_join<float><<<tiles(lines, 1), 128, 0, ctx->stream>>>(p); else attn_join<bf16><<<tiles(lines, 1), 128, 0, ctx->stream>>>(p);
+    ORMI_CUDA(cudaGetLastError());
+    count_launch(ctx);
 }
 
 void attention_delta(ormi_b200_ctx* ctx, const AttnParams& p, int dtype) {
@@ -500,9 +520,10 @@ void attention(ormi_b200_ctx* ctx, const ormi_b200_attention_args& a) {
     if (!p.batch || !p.q_len || !p.heads) return;
     written(ctx, a.out);
     written(ctx, a.lse);
-    // few packed rows over the cache: a tile of 128 queries would be mostly padding
-    const bool few = (int64_t)p.q_len * p.group <= 16;
-    if (!few && attention_tc_supported(p, a.q.dtype)) attention_tc(ctx, p); else attention_simple(ctx, p, a.q.dtype);
+    // up to 64 packed rows: a tile of 128 queries of one head would be mostly padding
+    if (attention_few_supported(p, a.q.dtype)) attention_few(ctx, p);
+    else if (attention_tc_supported(p, a.q.dtype)) attention_tc(ctx, p);
+    else attention_simple(ctx, p, a.q.dtype);
 }
 
 void attention_backward_check(const ormi_b200_attention_backward_args& a) {

@@ -49,12 +49,11 @@ __device__ __forceinline__ int key_end(const RowMask& m, int pos) {
     return m.causal ? min(m.keys, max(pos < 0x7fffffff ? pos + 1 : pos, m.prefix)) : m.keys;
 }
 
-// Score of a visible pair in base 2 from the raw product; `capped` receives what the cap made of it, over the cap.
-// tanh(x) = 1 - 2 / (exp(2x) + 1): absolute error of a few 1e-7, so a score is off by that times the cap.
-__device__ __forceinline__ float tanh_exp(float x) { return 1.f - __fdividef(2.f, exp2f(x * (2.f * kLog2e)) + 1.f); }
-
 void attention_simple(ormi_b200_ctx* ctx, AttnParams& p, int dtype);
 void attention_backward_simple(ormi_b200_ctx* ctx, AttnParams& p, int dtype);
+bool attention_few_supported(const AttnParams& p, int dtype);
+void attention_few(ormi_b200_ctx* ctx, AttnParams& p);
+void attention_join(ormi_b200_ctx* ctx, const AttnParams& p, int dtype);
 void attention_delta(ormi_b200_ctx* ctx, const AttnParams& p, int dtype);
 
 }  // namespace ormi_b200

@@ -348,12 +348,12 @@ void launch_by_mask(ormi_b200_ctx* ctx, const CUtensorMap* maps, const TcParams&
 
 }  // namespace
 
-// A 4-D map (head_dim, position, head, batch) with boxes of 64 values x 128 positions: reads behind any extent give zero.
-void head_map(ormi_b200_ctx* ctx, CUtensorMap* map, const void* ptr, const Strides4& s, int batch, int len, int heads, int dim) {
+// A 4-D map (head_dim, position, head, batch) with boxes of 64 values x `rows` positions: reads behind any extent give zero.
+void head_map(ormi_b200_ctx* ctx, CUtensorMap* map, const void* ptr, const Strides4& s, int batch, int len, int heads, int dim, int rows) {
     cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)len, (cuuint64_t)heads, (cuuint64_t)batch};
     // the stride of an extent of one is never used, but is checked
     cuuint64_t strides[3] = {(cuuint64_t)(len > 1 ? s.t * 2 : 16), (cuuint64_t)(heads > 1 ? s.h * 2 : 16), (cuuint64_t)(batch > 1 ? s.b * 2 : 16)};
-    cuuint32_t box[4] = {64, (cuuint32_t)kTile, 1, 1}, one[4] = {1, 1, 1, 1};
+    cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, one[4] = {1, 1, 1, 1};
     ctx->drv.check(ctx->drv.TensorMapEncodeTiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
                    "cuTensorMapEncodeTiled");

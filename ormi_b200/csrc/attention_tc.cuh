@@ -70,7 +70,7 @@ bool attention_backward_tc_supported(const AttnParams& p, int dtype);
 void attention_backward_tc(ormi_b200_ctx* ctx, AttnParams& p);
 
 // host side (attention_tc.cu)
-void head_map(ormi_b200_ctx* ctx, CUtensorMap* map, const void* ptr, const Strides4& s, int batch, int len, int heads, int dim);
+void head_map(ormi_b200_ctx* ctx, CUtensorMap* map, const void* ptr, const Strides4& s, int batch, int len, int heads, int dim, int rows = kTile);
 bool map_allowed(const void* ptr, const Strides4& s, int batch, int len, int heads);
 TcParams tc_params(ormi_b200_ctx* ctx, const AttnParams& p, int2* bounds);
 size_t bounds_bytes(const AttnParams& p);

@@ -34,6 +34,8 @@ _TYPES.update({"torch." + k: v for k, v in list(_TYPES.items())})
 _by_dtype: dict = {}                       # dtype object -> code, filled as types are met
 
 _VIEW = struct.Struct("=Qii8q")            # ormi_b200_view
+_VIEW_PACK = _VIEW.pack
+_tensor_types: set = set()                 # types with the tensor protocol, filled as they are met
 _ABSENT = bytes(_VIEW.size)
 _ZEROS = (0, 0, 0, 0)
 
@@ -123,6 +125,18 @@ def _pack(x, dev_index: int) -> bytes:
     """``x`` as an ormi_b200_view."""
     if x is None:
         return _ABSENT
+    kind = type(x)
+    if kind in _tensor_types:                  # the common case first: a call's arguments cost more time than its launch
+        code = _by_dtype.get(x.dtype)
+        if code is not None and x.get_device() == dev_index:
+            shape, strides = x.shape, x.stride()
+            n = len(shape)
+            if n == 2:
+                return _VIEW_PACK(x.data_ptr(), code, 2, shape[0], shape[1], 0, 0, strides[0], strides[1], 0, 0)
+            if n == 4:
+                return _VIEW_PACK(x.data_ptr(), code, 4, *shape, *strides)
+            if n == 1:
+                return _VIEW_PACK(x.data_ptr(), code, 1, shape[0], 0, 0, 0, strides[0], 0, 0, 0)
     if isinstance(x, View):
         ptr, code, shape, strides = x.ptr, x.dtype, x.shape, x.strides
     elif hasattr(x, "data_ptr"):
@@ -133,6 +147,7 @@ def _pack(x, dev_index: int) -> bytes:
             if code is None:
                 raise TypeError(f"{dt} is not a type of these operators (float32, bfloat16, float8_e4m3fn, int32)")
             _by_dtype[dt] = code
+        _tensor_types.add(kind)
         if x.get_device() != dev_index:
             raise ValueError(f"a tensor on {x.device} where the device is cuda:{dev_index}")
         ptr, shape, strides = x.data_ptr(), x.shape, x.stride()
