@@ -15,6 +15,7 @@
 // written order give the same codes on any machine.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
 #include "op_math.cuh"
@@ -24,9 +25,6 @@
 namespace ormi_b200 {
 namespace {
 
-#ifndef AB
-#define AB 4
-#endif
 constexpr int kThreads = 256;
 constexpr int kChunk = 4096;                 // elements per block: 32 blocks of 128 that share a scale
 
@@ -231,7 +229,7 @@ __device__ __forceinline__ uint32_t to_codes4(const float (&v)[4]) {
 
 // States in 8 bits: a warp owns the 128 elements that share a scale; four in a row per lane where aligned, else 32 apart.
 template <int N>
-__global__ void __launch_bounds__(kThreads, AB) adamw_e4m3(const __grid_constant__ Batch<N> b) {
+__global__ void __launch_bounds__(kThreads, 4) adamw_e4m3(const __grid_constant__ Batch<N> b) {
     __shared__ Rates shared_rates;
     if (threadIdx.x == 0) shared_rates = rates_of(b.c);
     __syncthreads();
@@ -243,30 +241,46 @@ __global__ void __launch_bounds__(kThreads, AB) adamw_e4m3(const __grid_constant
     e4m3* cm = (e4m3*)t.m;
     e4m3* cv = (e4m3*)t.v;
     if (t.vec && end - base == kChunk) {
-        // a warp takes four blocks, and asks for the next one's values before it works on this one
-        struct { float4 p, g; uint32_t m, v; float sm, sv; } now, next;
+        // A warp takes four blocks.  All their values are asked for at once, into shared memory (cp.async, every lane its own
+        // pieces: nobody waits for anybody), so that 160 KB per SM are on their way without holding registers (134 million parameters:
+        // 379 us, 5710 GB/s; loads into registers, two blocks per SM: 457 us).
         constexpr int TURNS = kChunk / (kThreads / 32 * 128);
+        __shared__ __align__(16) struct { float4 p[kThreads], g[kThreads]; uint32_t m[kThreads], v[kThreads]; } box[TURNS];
         auto first_of = [&](int k) { return base + (k * (kThreads / 32) + warp) * 128; };
-        auto fetch = [&](int k) {
-            const int64_t first = first_of(k), i = first + lane * 4;
-            next.p = *reinterpret_cast<const float4*>(t.param + i);
-            next.g = grads4(t, i);
-            next.m = *reinterpret_cast<const uint32_t*>(cm + i);
-            next.v = *reinterpret_cast<const uint32_t*>(cv + i);
-            next.sm = t.m_scales[first >> 7]; next.sv = t.v_scales[first >> 7];
+        auto copy = [](void* to, const void* from, auto bytes) {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(tc::smem_u32(to)), "l"(from), "n"(decltype(bytes)::value) : "memory");
         };
-        fetch(0);
+        using B4 = std::integral_constant<int, 4>; using B8 = std::integral_constant<int, 8>; using B16 = std::integral_constant<int, 16>;
+        float sm[TURNS], sv[TURNS];
 #pragma unroll
         for (int k = 0; k < TURNS; ++k) {
-            now = next;
-            if (k + 1 < TURNS) fetch(k + 1);
             const int64_t first = first_of(k), i = first + lane * 4;
-            float p[4] = {now.p.x, now.p.y, now.p.z, now.p.w}, m[4], v[4], qm[4], qv[4], hi_m, hi_v;
-            const float g[4] = {now.g.x, now.g.y, now.g.z, now.g.w};
-            codes4(now.m, m);
-            codes4(now.v, v);
+            copy(&box[k].p[threadIdx.x], t.param + i, B16{});
+            if (t.grad_f32) copy(&box[k].g[threadIdx.x], (const float*)t.grad + i, B16{}); else copy(&box[k].g[threadIdx.x], (const bf16*)t.grad + i, B8{});
+            copy(&box[k].m[threadIdx.x], cm + i, B4{});
+            copy(&box[k].v[threadIdx.x], cv + i, B4{});
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            sm[k] = t.m_scales[first >> 7]; sv[k] = t.v_scales[first >> 7];
+        }
+#pragma unroll
+        for (int k = 0; k < TURNS; ++k) {
+            if (k == 0) asm volatile("cp.async.wait_group 3;" ::: "memory");
+            else if (k == 1) asm volatile("cp.async.wait_group 2;" ::: "memory");
+            else if (k == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+            else asm volatile("cp.async.wait_group 0;" ::: "memory");
+            const int64_t first = first_of(k), i = first + lane * 4;
+            const float4 pp = box[k].p[threadIdx.x];
+            float4 gg = box[k].g[threadIdx.x];
+            if (!t.grad_f32) {
+                const uint32_t lo = __float_as_uint(gg.x), hi = __float_as_uint(gg.y);
+                gg = make_float4(bf16_lo(lo), bf16_hi(lo), bf16_lo(hi), bf16_hi(hi));
+            }
+            float p[4] = {pp.x, pp.y, pp.z, pp.w}, m[4], v[4], qm[4], qv[4], hi_m, hi_v;
+            const float g[4] = {gg.x, gg.y, gg.z, gg.w};
+            codes4(box[k].m[threadIdx.x], m);
+            codes4(box[k].v[threadIdx.x], v);
             const uint32_t h[4] = {mix32((uint32_t)i ^ key), mix32((uint32_t)(i + 1) ^ key), mix32((uint32_t)(i + 2) ^ key), mix32((uint32_t)(i + 3) ^ key)};
-            step_block(b.c, r, t.decay, h, g, m, v, now.sm, now.sv, p, qm, qv, hi_m, hi_v);
+            step_block(b.c, r, t.decay, h, g, m, v, sm[k], sv[k], p, qm, qv, hi_m, hi_v);
             *reinterpret_cast<float4*>(t.param + i) = make_float4(p[0], p[1], p[2], p[3]);
             *reinterpret_cast<uint32_t*>(cm + i) = to_codes4(qm);
             *reinterpret_cast<uint32_t*>(cv + i) = to_codes4(qv);

@@ -20,25 +20,29 @@ constexpr int kThreads = 256;               // 16 x 16 threads over a tile
 
 __device__ __forceinline__ int64_t at(const Strides4& s, int b, int t, int h) { return (int64_t)b * s.b + (int64_t)t * s.t + (int64_t)h * s.h; }
 
-// Rows [first, first + R) of a [.., dim] operand into shared memory as fp32, zero behind `limit` rows and behind dim.
+// Rows [first, first + R) of a [.., dim] operand into shared memory as fp32, zero behind `limit` rows and behind dim: a warp per
+// row, so that finding a row is not every element's work.
 template <typename T, int R, int DP, typename F>
 __device__ __forceinline__ void load_rows(float (*dst)[DP + 4], int first, int limit, int dim, F&& row_ptr) {
-    for (int i = threadIdx.x; i < R * DP; i += kThreads) {
-        const int r = i / DP, d = i % DP;
-        float v = 0.f;
-        if (first + r < limit && d < dim) v = to_f32(((const T*)row_ptr(first + r))[d]);
-        dst[r][d] = v;
+    const int lane = threadIdx.x & 31;
+#pragma unroll 4
+    for (int r = threadIdx.x >> 5; r < R; r += kThreads / 32) {
+        const bool in = first + r < limit;
+        const T* row = in ? (const T*)row_ptr(first + r) : nullptr;
+#pragma unroll
+        for (int d = lane; d < DP; d += 32) dst[r][d] = in && d < dim ? to_f32(row[d]) : 0.f;
     }
 }
 
 // acc[i][j] = A[ty + 16 i] . B[tx + 16 j]
 template <int RI, int RJ, int DP>
-__device__ __forceinline__ void dot_tile(const float (*A)[DP + 4], const float (*B)[DP + 4], int ty, int tx, float (&acc)[RI][RJ]) {
+__device__ __forceinline__ void dot_tile(const float (*A)[DP + 4], const float (*B)[DP + 4], int dim, int ty, int tx, float (&acc)[RI][RJ]) {
 #pragma unroll
     for (int i = 0; i < RI; ++i)
 #pragma unroll
         for (int j = 0; j < RJ; ++j) acc[i][j] = 0.f;
-    for (int d = 0; d < DP; d += 4) {
+#pragma unroll 2
+    for (int d = 0; d < dim; d += 4) {
         float4 a[RI], b[RJ];
 #pragma unroll
         for (int i = 0; i < RI; ++i) a[i] = *(const float4*)&A[ty + 16 * i][d];
@@ -144,7 +148,7 @@ __global__ void __launch_bounds__(kThreads) attn_forward(AttnParams p) {
         load_rows<T, BN, DP>(V, n * BN, m.keys, p.dim, [&](int j) { return (const T*)p.v + at(p.vs, b, j, kvh); });
         __syncthreads();
         float s[RI][RJ];
-        dot_tile<RI, RJ, DP>(Q, K, ty, tx, s);
+        dot_tile<RI, RJ, DP>(Q, K, p.dim, ty, tx, s);
 #pragma unroll
         for (int i = 0; i < RI; ++i) {
             float big = top[i];
@@ -286,8 +290,8 @@ __global__ void __launch_bounds__(kThreads) attn_backward(AttnParams p) {
         if (QUERY) load_keys(key0); else load_queries(row0);
         __syncthreads();
         float s[RI][RI], g[RI][RI];
-        dot_tile<RI, RI, DP>(Q, K, ty, tx, s);
-        dot_tile<RI, RI, DP>(G, V, ty, tx, g);
+        dot_tile<RI, RI, DP>(Q, K, p.dim, ty, tx, s);
+        dot_tile<RI, RI, DP>(G, V, p.dim, ty, tx, g);
 #pragma unroll
         for (int i = 0; i < RI; ++i) {
             const RowOf o = row_of(p, m, kvh, row0 + ty + 16 * i);
@@ -360,32 +364,37 @@ void run_forward(ormi_b200_ctx* ctx, AttnParams& p) {
     part.release();
 }
 
+// Tiles of 64 rows have the best ratio of arithmetic to shared memory; where they would leave SMs idle, smaller ones spread the
+// work (half the arithmetic per load, four times the blocks), and up to 16 rows would be mostly padding in them.
+bool spread(ormi_b200_ctx* ctx, const AttnParams& p, int64_t rows) { return (rows + 63) / 64 * p.batch * p.kv_heads < ctx->num_sms; }
+
 template <typename T>
 void forward_by_size(ormi_b200_ctx* ctx, AttnParams& p) {
-    // up to 16 packed rows: a tile of 16, which wastes less of the arithmetic on padding
-    const bool few = (int64_t)p.q_len * p.group <= 16;
-    if (p.dim <= 64) { if (few) run_forward<T, 16, 64, 64>(ctx, p); else run_forward<T, 64, 64, 64>(ctx, p); }
-    else if (p.dim <= 128) { if (few) run_forward<T, 16, 64, 128>(ctx, p); else run_forward<T, 64, 64, 128>(ctx, p); }
-    else { if (few) run_forward<T, 16, 32, 256>(ctx, p); else run_forward<T, 64, 32, 256>(ctx, p); }
+    const int64_t rows = (int64_t)p.q_len * p.group;
+    const int tile = rows <= 16 ? 16 : spread(ctx, p, rows) ? 32 : 64;
+    if (p.dim <= 64) { if (tile == 16) run_forward<T, 16, 64, 64>(ctx, p); else if (tile == 32) run_forward<T, 32, 64, 64>(ctx, p); else run_forward<T, 64, 64, 64>(ctx, p); }
+    else if (p.dim <= 128) { if (tile == 16) run_forward<T, 16, 64, 128>(ctx, p); else if (tile == 32) run_forward<T, 32, 64, 128>(ctx, p); else run_forward<T, 64, 64, 128>(ctx, p); }
+    else { if (tile == 16) run_forward<T, 16, 32, 256>(ctx, p); else run_forward<T, 64, 32, 256>(ctx, p); }
 }
 
-template <typename T, int B, int DP>
+template <typename T, int B, int DP, bool QUERY>
 void run_backward(ormi_b200_ctx* ctx, AttnParams& p) {
     const int smem = (4 * B * (DP + 4) + 2 * B * (B + 4)) * 4;
-    allow_smem(attn_backward<T, B, DP, false>, smem);
-    allow_smem(attn_backward<T, B, DP, true>, smem);
-    const int pairs = p.batch * p.kv_heads;
-    if (p.k_len) attn_backward<T, B, DP, false><<<dim3(tiles(p.k_len, B), pairs), kThreads, smem, ctx->stream>>>(p);
-    if (p.q_len) attn_backward<T, B, DP, true><<<dim3(tiles((int64_t)p.q_len * p.group, B), pairs), kThreads, smem, ctx->stream>>>(p);
+    auto kernel = attn_backward<T, B, DP, QUERY>;
+    const int64_t rows = QUERY ? (int64_t)p.q_len * p.group : p.k_len;
+    if (!rows) return;
+    allow_smem(kernel, smem);
+    kernel<<<dim3(tiles(rows, B), p.batch * p.kv_heads), kThreads, smem, ctx->stream>>>(p);
     ORMI_CUDA(cudaGetLastError());
-    count_launch(ctx, (p.k_len > 0) + (p.q_len > 0));
+    count_launch(ctx);
 }
 
-template <typename T>
+template <typename T, bool QUERY>
 void backward_by_size(ormi_b200_ctx* ctx, AttnParams& p) {
-    if (p.dim <= 64) run_backward<T, 64, 64>(ctx, p);
-    else if (p.dim <= 128) run_backward<T, 64, 128>(ctx, p);
-    else run_backward<T, 32, 256>(ctx, p);
+    const bool small = spread(ctx, p, QUERY ? (int64_t)p.q_len * p.group : p.k_len);
+    if (p.dim <= 64) { if (small) run_backward<T, 32, 64, QUERY>(ctx, p); else run_backward<T, 64, 64, QUERY>(ctx, p); }
+    else if (p.dim <= 128) { if (small) run_backward<T, 32, 128, QUERY>(ctx, p); else run_backward<T, 64, 128, QUERY>(ctx, p); }
+    else run_backward<T, 32, 256, QUERY>(ctx, p);
 }
 
 }  // namespace
@@ -395,7 +404,8 @@ void attention_simple(ormi_b200_ctx* ctx, AttnParams& p, int dtype) {
 }
 
 void attention_backward_simple(ormi_b200_ctx* ctx, AttnParams& p, int dtype) {
-    if (dtype == ORMI_F32) backward_by_size<float>(ctx, p); else backward_by_size<bf16>(ctx, p);
+    if (dtype == ORMI_F32) { backward_by_size<float, false>(ctx, p); backward_by_size<float, true>(ctx, p); }
+    else { backward_by_size<bf16, false>(ctx, p); backward_by_size<bf16, true>(ctx, p); }
 }
 
 void attention_join(ormi_b200_ctx* ctx, const AttnParams& p, int dtype) {
