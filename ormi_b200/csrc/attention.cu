@@ -557,8 +557,12 @@ void attention_backward(ormi_b200_ctx* ctx, const ormi_b200_attention_backward_a
     for (auto* v : {&a.dq, &a.dk, &a.dv}) written(ctx, *v);
     Scratch delta(ctx, (size_t)p.batch * p.heads * p.q_len * 4);
     p.delta = (float*)delta.ptr;
-    attention_delta(ctx, p, a.forward.q.dtype);
-    if (attention_backward_tc_supported(p, a.forward.q.dtype)) attention_backward_tc(ctx, p); else attention_backward_simple(ctx, p, a.forward.q.dtype);
+    if (attention_backward_tc_supported(p, a.forward.q.dtype)) {
+        attention_backward_tc(ctx, p);
+    } else {
+        attention_delta(ctx, p, a.forward.q.dtype);
+        attention_backward_simple(ctx, p, a.forward.q.dtype);
+    }
     delta.release();
 }
 

@@ -1,14 +1,16 @@
 // Backward attention on the tensor cores: bf16, head_dim up to 128.
 //
 // Two kernels, so that no gradient is summed with atomics and results do not depend on the order of blocks:
-//   attn_back_kv   a block owns 128 keys of one key/value head and walks the tiles of 128 queries that see any of them, over
-//                  all query heads that share the head.  Scores are computed transposed (rows = keys), so that
-//                  probabilities and score gradients, rounded to bf16 in tensor memory, are the A operands of
-//                  dV += P^T dO and dK += dS^T Q directly.
-//   attn_back_q    a block owns 128 queries of one head and walks the tiles of keys: dQ += dS K.
+//   attn_back_q    a block owns 128 queries of one head and walks the tiles of 128 keys: dQ += dS K.  It also writes
+//                  delta = rowsum(dO O), which the second kernel reads.
+//   attn_back_kv   a block owns 128 keys of one key/value head and walks the tiles of 128 queries, over all query heads that
+//                  share the head.  Scores are computed transposed (rows = keys), so that probabilities and score
+//                  gradients, rounded to bf16 in tensor memory, are the A operands of dV += P^T dO and dK += dS^T Q directly.
 // The price is that both compute the scores (7 products instead of 5).  Warp 0 loads, warp 1 issues the products, warp 2
-// fetches the queries' statistics (or blanks the keys behind key_len), 8 warps do the arithmetic: two warpgroups, each half
-// of the columns of a tile.
+// fetches the queries' statistics (or blanks the keys behind key_len), and two warpgroups do the arithmetic, each half of the
+// columns of a tile: while they work on the gradients of a tile the tensor cores multiply its probabilities and compute
+// the next scores, and the other way round.  (Tiles of 64, one warpgroup each, were slower: a product of 64 columns takes
+// the tensor cores as long as one of 128.)
 #include <algorithm>
 
 #include "attention_tc.cuh"
@@ -28,7 +30,7 @@ template <int DP> struct BackShape {
     static constexpr int kSmem = 1024 + (2 + 2 * kStages) * kOperand + kMaxTiles * 2 + kStages * (int)sizeof(Stat) + 256;
 };
 
-// The tiles whose class is not kSkip, in order, with bit 15 set where each pair has to be looked at; by one warp.
+// The tiles whose class is not kSkip, in order, class in the top two bits; by one warp.
 template <typename F>
 __device__ __forceinline__ int list_tiles(unsigned short* list, int tiles, F&& class_of) {
     const int lane = threadIdx.x & 31;
@@ -36,11 +38,12 @@ __device__ __forceinline__ int list_tiles(unsigned short* list, int tiles, F&& c
     for (int first = 0; first < tiles; first += 32) {
         const int c = first + lane < tiles ? class_of(first + lane) : kSkip;
         const unsigned hit = __ballot_sync(0xffffffffu, c != kSkip);
-        if (c != kSkip) list[n + __popc(hit & ((1u << lane) - 1))] = (unsigned short)((first + lane) | (c == kPartial ? 0x8000 : 0));
+        if (c != kSkip) list[n + __popc(hit & ((1u << lane) - 1))] = (unsigned short)((first + lane) | c << 14);
         n += __popc(hit);
     }
     return n;
 }
+__device__ __forceinline__ int tile_of(unsigned short entry) { return entry & 0x3fff; }
 
 // 32 columns of tensor memory to 32 bf16 values of a row, times `by`.
 __device__ __forceinline__ void store_row32(bf16* out, int x, int dim, const uint32_t* o, float by) {
@@ -59,8 +62,23 @@ __device__ __forceinline__ void store_row32(bf16* out, int x, int dim, const uin
 // A operand of 128 bf16 columns that two warpgroups wrote into the first halves of their own 64 columns.
 template <int DP>
 __device__ __forceinline__ void product_halves(uint32_t d, uint32_t a, uint32_t b, uint32_t accumulate) {
+    const uint64_t db = desc_mn<kTile>(b);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) mma_ts(d, a + (k / 4) * 64 + (k % 4) * 8, desc(b, true) + ((k * 2048) >> 4), idesc(DP, true), accumulate || k > 0);
+    for (int k = 0; k < 8; ++k) mma_ts(d, a + (k / 4) * 64 + (k % 4) * 8, db + ((k * 2048) >> 4), idesc(DP, true), accumulate || k > 0);
+}
+
+__device__ __forceinline__ void leave(Abort& ab, int warp, uint32_t tmem) {
+    __syncwarp();
+    if (ab.flag) {                                             // let copies that are still in flight land before the block goes away
+        const unsigned long long t0 = global_ns();
+        while (global_ns() - t0 < 200000ull) { }
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
 }
 
 template <int DP, bool CAP, bool BIAS, bool DOCS>
@@ -95,7 +113,7 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     if (warp == 0) {
         const int n = key0 >= m.keys ? 0 : list_tiles(list, (p.a.q_len + kTile - 1) / kTile, [&](int t) {
             const int first = t * kTile, last = min(first + kTile, p.a.q_len) - 1;
-            return tile_class(p, b, t, key_end(m, m.start + first), key_end(m, m.start + last), key0 / kTile);
+            return tile_class<2, 2>(p, b, 2 * t, key_end(m, m.start + first), key_end(m, m.start + last), key0 / kUnit);
         });
         if (lane == 0) list_size = n;
     }
@@ -114,100 +132,114 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = tmem_slot, s_at = tmem, dp_at = tmem + 128, dv_at = tmem + 256, dk_at = tmem + 384;
+    // all of tensor memory is this block's, so it starts at column 0 (checked: every address below is a constant)
+    constexpr uint32_t tmem = 0, s_at = tmem, dp_at = tmem + 128, dv_at = tmem + 256, dk_at = tmem + 384;
+    const bool whole = tmem_slot == tmem;
+    if (!whole && threadIdx.x == 0) atomicCAS(p.err, 0, 20);
     const int per_head = list_size, total = per_head * p.a.group;
 
-    if (warp == 0) {
-        if (lane == 0 && total) {
-            mbar_expect_tx(kv_full, 2 * OP);
-            for (int x = 0; x < DP / 64; ++x) {
-                tma_load_4d(k_at + x * kBox, &map_k, kv_full, 64 * x, key0, kvh, b);
-                tma_load_4d(v_at + x * kBox, &map_v, kv_full, 64 * x, key0, kvh, b);
+    if (!whole) {
+    } else if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 0) {
+            if (lane == 0 && total) {
+                mbar_expect_tx(kv_full, 2 * OP);
+                for (int x = 0; x < DP / 64; ++x) {
+                    tma_load_4d(k_at + x * box_bytes(kTile), &map_k, kv_full, 64 * x, key0, kvh, b);
+                    tma_load_4d(v_at + x * box_bytes(kTile), &map_v, kv_full, 64 * x, key0, kvh, b);
+                }
+                bool ok = true;
+                int i = 0;
+                for (; i < total && ok; ++i) {
+                    const int s = i % ST, h = kvh * p.a.group + i / per_head, q0 = tile_of(list[i % per_head]) * kTile;
+                    ok = mbar_wait(empty(s), (i / ST & 1) ^ 1, ab, 31);
+                    if (!ok) break;
+                    mbar_expect_tx(q_full(s), OP);
+                    for (int x = 0; x < DP / 64; ++x) tma_load_4d(q_at(s) + x * box_bytes(kTile), &map_q, q_full(s), 64 * x, q0, h, b);
+                    mbar_expect_tx(do_full(s), OP);
+                    for (int x = 0; x < DP / 64; ++x) tma_load_4d(do_at(s) + x * box_bytes(kTile), &map_do, do_full(s), 64 * x, q0, h, b);
+                }
+                for (int k = 0; k < ST && ok; ++k, ++i) ok = mbar_wait(empty(i % ST), (i / ST & 1) ^ 1, ab, 31);
             }
-            bool ok = true;
-            int i = 0;
-            for (; i < total && ok; ++i) {
-                const int s = i % ST, h = kvh * p.a.group + i / per_head, q0 = (list[i % per_head] & 0x7fff) * kTile;
-                ok = mbar_wait(empty(s), (i / ST & 1) ^ 1, ab, 31);
-                if (!ok) break;
-                mbar_expect_tx(q_full(s), OP);
-                for (int x = 0; x < DP / 64; ++x) tma_load_4d(q_at(s) + x * kBox, &map_q, q_full(s), 64 * x, q0, h, b);
-                mbar_expect_tx(do_full(s), OP);
-                for (int x = 0; x < DP / 64; ++x) tma_load_4d(do_at(s) + x * kBox, &map_do, do_full(s), 64 * x, q0, h, b);
+        } else if (warp == 1) {
+            if (total) {
+                bool ok = warp_wait(kv_full, 0, ab, 32);
+                auto scores = [&](int i) {
+                    ok = ok && warp_wait(q_full(i % ST), i / ST & 1, ab, 33);
+                    if (!ok) return;
+                    fence_after();
+                    if (elect()) {
+                        product_nt<DP, kTile>(s_at, k_at, q_at(i % ST));
+                        commit(s_full);
+                    }
+                };
+                auto gaps = [&](int i) {
+                    ok = ok && warp_wait(do_full(i % ST), i / ST & 1, ab, 34);
+                    if (!ok) return;
+                    fence_after();
+                    if (elect()) {
+                        product_nt<DP, kTile>(dp_at, v_at, do_at(i % ST));
+                        commit(dp_full);
+                    }
+                };
+                scores(0);
+                gaps(0);
+                // P sits in the scores' columns and dS in the columns of dP: the next tile's products follow their readers in order
+                for (int i = 0; i < total && ok; ++i) {
+                    ok = warp_wait(p_ready, i & 1, ab, 35);
+                    if (!ok) break;
+                    fence_after();
+                    if (elect()) product_halves<DP>(dv_at, s_at, do_at(i % ST), i > 0);
+                    if (i + 1 < total) scores(i + 1);
+                    ok = ok && warp_wait(ds_ready, i & 1, ab, 36);
+                    if (!ok) break;
+                    fence_after();
+                    if (elect()) {
+                        product_halves<DP>(dk_at, dp_at, q_at(i % ST), i > 0);
+                        commit(empty(i % ST));
+                    }
+                    if (i + 1 < total) gaps(i + 1);
+                }
+                if (elect()) commit(done);
             }
-            for (int k = 0; k < ST && ok; ++k, ++i) ok = mbar_wait(empty(i % ST), (i / ST & 1) ^ 1, ab, 31);
+        } else if (warp == 2) {
+            // the queries' statistics; a row that sees nothing, or does not exist, gets an infinite one: its probabilities vanish
+            for (int i = 0; i < total; ++i) {
+                const int s = i % ST, h = kvh * p.a.group + i / per_head, q0 = tile_of(list[i % per_head]) * kTile;
+                float l[4], d[4];
+                int e[4], doc[4];
+    #pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int t = q0 + k * 32 + lane;
+                    const bool live = t < p.a.q_len;
+                    const int64_t line = ((int64_t)b * p.a.heads + h) * p.a.q_len + t;
+                    l[k] = live ? p.a.lse[line] * kLog2e : INFINITY;
+                    if (l[k] == -INFINITY) l[k] = INFINITY;
+                    d[k] = live ? p.a.delta[line] : 0.f;
+                    e[k] = live ? key_end(m, m.start + t) : 0;
+                    doc[k] = DOCS && live ? m.q_docs[t] : 0;
+                }
+                if (!warp_wait(stat_empty(s), (i / ST & 1) ^ 1, ab, 37)) break;
+    #pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    stats[s].lse2[k * 32 + lane] = -l[k]; stats[s].delta[k * 32 + lane] = -d[k];
+                    stats[s].end[k * 32 + lane] = e[k];
+                    if (DOCS) stats[s].doc[k * 32 + lane] = doc[k];
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(stat_full(s));
+            }
         }
-    } else if (warp == 1) {
-        if (lane == 0 && total) {
-            bool ok = mbar_wait(kv_full, 0, ab, 32);
-            auto scores = [&](int i) {
-                ok = ok && mbar_wait(q_full(i % ST), i / ST & 1, ab, 33);
-                if (!ok) return;
-                fence_after();
-                product_nt<DP, kTile>(s_at, k_at, q_at(i % ST), 0);
-                commit(s_full);
-            };
-            auto gaps = [&](int i) {
-                ok = ok && mbar_wait(do_full(i % ST), i / ST & 1, ab, 34);
-                if (!ok) return;
-                fence_after();
-                product_nt<DP, kTile>(dp_at, v_at, do_at(i % ST), 0);
-                commit(dp_full);
-            };
-            scores(0);
-            gaps(0);
-            // P sits in the scores' columns and dS in the columns of dP: the next tile's products follow their readers in order
-            for (int i = 0; i < total && ok; ++i) {
-                ok = mbar_wait(p_ready, i & 1, ab, 35);
-                if (!ok) break;
-                fence_after();
-                product_halves<DP>(dv_at, s_at, do_at(i % ST), i > 0);
-                if (i + 1 < total) scores(i + 1);
-                ok = ok && mbar_wait(ds_ready, i & 1, ab, 36);
-                if (!ok) break;
-                fence_after();
-                product_halves<DP>(dk_at, dp_at, q_at(i % ST), i > 0);
-                commit(empty(i % ST));
-                if (i + 1 < total) gaps(i + 1);
-            }
-            commit(done);
-        }
-    } else if (warp == 2) {
-        // the queries' statistics; a row that sees nothing, or does not exist, gets an infinite one: its probabilities vanish
-        for (int i = 0; i < total; ++i) {
-            const int s = i % ST, h = kvh * p.a.group + i / per_head, q0 = (list[i % per_head] & 0x7fff) * kTile;
-            float l[4], d[4];
-            int e[4], doc[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int t = q0 + k * 32 + lane;
-                const bool live = t < p.a.q_len;
-                const int64_t line = ((int64_t)b * p.a.heads + h) * p.a.q_len + t;
-                l[k] = live ? p.a.lse[line] * kLog2e : INFINITY;
-                if (l[k] == -INFINITY) l[k] = INFINITY;
-                d[k] = live ? p.a.delta[line] : 0.f;
-                e[k] = live ? key_end(m, m.start + t) : 0;
-                doc[k] = DOCS && live ? m.q_docs[t] : 0;
-            }
-            if (!warp_wait(stat_empty(s), (i / ST & 1) ^ 1, ab, 37)) break;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                stats[s].lse2[k * 32 + lane] = -l[k]; stats[s].delta[k * 32 + lane] = -d[k];
-                stats[s].end[k * 32 + lane] = e[k];
-                if (DOCS) stats[s].doc[k * 32 + lane] = doc[k];
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(stat_full(s));
-        }
-    } else if (warp >= 4) {
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int w = warp / 4 - 1, row = threadIdx.x & 127, key = key0 + row;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         const bool live = key < m.keys;
         const int my_doc = DOCS && live ? m.k_docs[key] : 0;
         bool ok = true;
         for (int i = 0; i < total; ++i) {
-            const int s = i % ST, entry = list[i % per_head], q0 = (entry & 0x7fff) * kTile;
-            const bool partial = entry & 0x8000;
+            const int s = i % ST, entry = list[i % per_head], q0 = tile_of(entry) * kTile;
+            const int cls = entry >> 14;
             const Stat& st = stats[s];
             const float slope = BIAS ? p.a.slopes[kvh * p.a.group + i / per_head] * kLog2e : 0.f;
             const float ahead = (float)(m.start + q0 + 64 * w - key);
@@ -236,10 +268,10 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                     a[k] = CAP || BIAS ? add2(z[c + k], a[k]) : fma2(z[c + k], both(p.scale_log2), a[k]);
                     z[c + k] = make_float2(ex2(a[k].x), ex2(a[k].y));
                 }
-                if (partial) {
+                if (cls >= kPartial) {
                     const int4 e = *reinterpret_cast<const int4*>(&st.end[64 * w + 2 * c]);
                     int4 d = make_int4(my_doc, my_doc, my_doc, my_doc);
-                    if (DOCS) d = *reinterpret_cast<const int4*>(&st.doc[64 * w + 2 * c]);
+                    if (DOCS) { if (cls == kDocs) d = *reinterpret_cast<const int4*>(&st.doc[64 * w + 2 * c]); }
                     if ((key >= e.x) | (d.x != my_doc)) { z[c].x = 0.f; if (CAP) g[c].x = 0.f; }
                     if ((key >= e.y) | (d.y != my_doc)) { z[c].y = 0.f; if (CAP) g[c].y = 0.f; }
                     if ((key >= e.z) | (d.z != my_doc)) { z[c + 1].x = 0.f; if (CAP) g[c + 1].x = 0.f; }
@@ -263,7 +295,7 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             ld32(dp_at + lanes + 64 * w, reinterpret_cast<uint32_t*>(gap));
             ld32(dp_at + lanes + 64 * w + 32, reinterpret_cast<uint32_t*>(gap) + 32);
             wait_ld();
-            if (partial) {                              // a masked pair's V may hold anything
+            if (cls >= kPartial) {                      // a masked pair's V may hold anything
 #pragma unroll
                 for (int c = 0; c < 32; ++c) { if (g[c].x == 0.f) gap[c].x = 0.f; if (g[c].y == 0.f) gap[c].y = 0.f; }
             }
@@ -295,17 +327,7 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             }
         }
     }
-    __syncwarp();
-    if (ab.flag) {                                             // let copies that are still in flight land before the block goes away
-        const unsigned long long t0 = global_ns();
-        while (global_ns() - t0 < 200000ull) { }
-    }
-    fence_before();
-    __syncthreads();
-    if (warp == 1) {
-        fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
-    }
+    leave(ab, warp, tmem_slot);
 }
 
 template <int DP, bool CAP, bool BIAS, bool DOCS>
@@ -320,7 +342,8 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     const uint32_t q_at = base, do_at = base + OP;
     auto k_at = [&](int s) { return base + (2 + 2 * s) * OP; };
     auto v_at = [&](int s) { return base + (3 + 2 * s) * OP; };
-    int* docs = reinterpret_cast<int*>(mem + (2 + 2 * ST) * OP);                 // 64 for each compute warp
+    float* deltas = reinterpret_cast<float*>(mem + (2 + 2 * ST) * OP);           // of the 128 queries
+    int* docs = reinterpret_cast<int*>(deltas + kTile);                          // 64 for each compute warp
     unsigned short* list = reinterpret_cast<unsigned short*>(docs + 8 * 64);
     const uint32_t bars = smem_u32(list + kMaxTiles);
     const uint32_t q_full = bars, dp_full = bars + 8, ds_ready = bars + 16, done = bars + 24, blank_go = bars + 32, blanked = bars + 40;
@@ -340,7 +363,7 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     const int blank_tile = m.keys < p.a.k_len && m.keys % kTile ? m.keys / kTile : -1;
     if (warp == 0) {
         const int lo = key_end(m, m.start + q0), hi = key_end(m, m.start + min(q0 + kTile, p.a.q_len) - 1);
-        const int n = list_tiles(list, (max(hi, 0) + kTile - 1) / kTile, [&](int j) { return tile_class(p, b, q0 / kTile, lo, hi, j); });
+        const int n = list_tiles(list, (max(hi, 0) + kTile - 1) / kTile, [&](int j) { return tile_class<2, 2>(p, b, q0 / kUnit, lo, hi, 2 * j); });
         if (lane == 0) list_size = n;
     }
     if (threadIdx.x == 0) {
@@ -358,94 +381,128 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = tmem_slot, dp_at = tmem + 256, dq_at = tmem + 384;
+    constexpr uint32_t tmem = 0, dp_at = tmem + 256, dq_at = tmem + 384;         // as above
+    const bool whole = tmem_slot == tmem;
+    if (!whole && threadIdx.x == 0) atomicCAS(p.err, 0, 20);
     auto s_at = [&](int x) { return tmem + 128 * x; };
     const int total = list_size;
 
-    if (warp == 0) {
-        if (lane == 0 && total) {
-            mbar_expect_tx(q_full, 2 * OP);
-            for (int x = 0; x < DP / 64; ++x) {
-                tma_load_4d(q_at + x * kBox, &map_q, q_full, 64 * x, q0, h, b);
-                tma_load_4d(do_at + x * kBox, &map_do, q_full, 64 * x, q0, h, b);
-            }
-            bool ok = true;
-            int i = 0;
-            for (; i < total && ok; ++i) {
-                const int s = i % ST, key0 = (list[i] & 0x7fff) * kTile;
-                ok = mbar_wait(empty(s), (i / ST & 1) ^ 1, ab, 41);
-                if (!ok) break;
-                mbar_expect_tx(k_full(s), OP);
-                for (int x = 0; x < DP / 64; ++x) tma_load_4d(k_at(s) + x * kBox, &map_k, k_full(s), 64 * x, key0, kvh, b);
-                mbar_expect_tx(v_full(s), OP);
-                for (int x = 0; x < DP / 64; ++x) tma_load_4d(v_at(s) + x * kBox, &map_v, v_full(s), 64 * x, key0, kvh, b);
-            }
-            for (int k = 0; k < ST && ok; ++k, ++i) ok = mbar_wait(empty(i % ST), (i / ST & 1) ^ 1, ab, 41);
-        }
-    } else if (warp == 1) {
-        if (lane == 0 && total) {
-            bool ok = mbar_wait(q_full, 0, ab, 42);
-            auto scores = [&](int i) {
-                ok = ok && mbar_wait(k_full(i % ST), i / ST & 1, ab, 43);
-                if (ok && (list[i] & 0x7fff) == blank_tile) {            // warp 2 blanks the rows behind key_len first
-                    mbar_arrive(blank_go);
-                    ok = mbar_wait(blanked, 0, ab, 43);
+    if (!whole) {
+    } else if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 0) {
+            if (lane == 0 && total) {
+                mbar_expect_tx(q_full, 2 * OP);
+                for (int x = 0; x < DP / 64; ++x) {
+                    tma_load_4d(q_at + x * box_bytes(kTile), &map_q, q_full, 64 * x, q0, h, b);
+                    tma_load_4d(do_at + x * box_bytes(kTile), &map_do, q_full, 64 * x, q0, h, b);
                 }
-                ok = ok && mbar_wait(s_empty(i & 1), (i / 2 & 1) ^ 1, ab, 44);
-                if (!ok) return;
-                fence_after();
-                product_nt<DP, kTile>(s_at(i & 1), q_at, k_at(i % ST), 0);
-                commit(s_full(i & 1));
-            };
-            auto gaps = [&](int i) {
-                ok = ok && mbar_wait(v_full(i % ST), i / ST & 1, ab, 45);
-                if (!ok) return;
-                fence_after();
-                product_nt<DP, kTile>(dp_at, do_at, v_at(i % ST), 0);
-                commit(dp_full);
-            };
-            scores(0);
-            gaps(0);
-            for (int i = 0; i < total && ok; ++i) {
-                if (i + 1 < total) scores(i + 1);                        // runs while the gradients of tile i are computed
-                ok = ok && mbar_wait(ds_ready, i & 1, ab, 46);
-                if (!ok) break;
-                fence_after();
-                product_halves<DP>(dq_at, dp_at, k_at(i % ST), i > 0);
-                commit(empty(i % ST));
-                if (i + 1 < total) gaps(i + 1);
+                bool ok = true;
+                int i = 0;
+                for (; i < total && ok; ++i) {
+                    const int s = i % ST, key0 = tile_of(list[i]) * kTile;
+                    ok = mbar_wait(empty(s), (i / ST & 1) ^ 1, ab, 41);
+                    if (!ok) break;
+                    mbar_expect_tx(k_full(s), OP);
+                    for (int x = 0; x < DP / 64; ++x) tma_load_4d(k_at(s) + x * box_bytes(kTile), &map_k, k_full(s), 64 * x, key0, kvh, b);
+                    mbar_expect_tx(v_full(s), OP);
+                    for (int x = 0; x < DP / 64; ++x) tma_load_4d(v_at(s) + x * box_bytes(kTile), &map_v, v_full(s), 64 * x, key0, kvh, b);
+                }
+                for (int k = 0; k < ST && ok; ++k, ++i) ok = mbar_wait(empty(i % ST), (i / ST & 1) ^ 1, ab, 41);
             }
-            commit(done);
-        }
-    } else if (warp == 2) {
-        if (total && blank_tile >= 0 && (list[total - 1] & 0x7fff) == blank_tile) {
-            const int s = (total - 1) % ST;
-            if (warp_wait(blank_go, 0, ab, 47)) {
-                for (int x = 0; x < DP / 64; ++x)
-                    for (int i = m.keys % kTile * 8 + lane; i < kTile * 8; i += 32)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(k_at(s) + x * kBox + i * 16), "r"(0) : "memory");
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(blanked);
+        } else if (warp == 1) {
+            if (total) {
+                bool ok = warp_wait(q_full, 0, ab, 42);
+                auto scores = [&](int i) {
+                    ok = ok && warp_wait(k_full(i % ST), i / ST & 1, ab, 43);
+                    if (ok && tile_of(list[i]) == blank_tile) {            // warp 2 blanks the rows behind key_len first
+                        if (lane == 0) mbar_arrive(blank_go);
+                        ok = warp_wait(blanked, 0, ab, 43);
+                    }
+                    ok = ok && warp_wait(s_empty(i & 1), (i / 2 & 1) ^ 1, ab, 44);
+                    if (!ok) return;
+                    fence_after();
+                    if (elect()) {
+                        product_nt<DP, kTile>(s_at(i & 1), q_at, k_at(i % ST));
+                        commit(s_full(i & 1));
+                    }
+                };
+                auto gaps = [&](int i) {
+                    ok = ok && warp_wait(v_full(i % ST), i / ST & 1, ab, 45);
+                    if (!ok) return;
+                    fence_after();
+                    if (elect()) {
+                        product_nt<DP, kTile>(dp_at, do_at, v_at(i % ST));
+                        commit(dp_full);
+                    }
+                };
+                scores(0);
+                gaps(0);
+                for (int i = 0; i < total && ok; ++i) {
+                    if (i + 1 < total) scores(i + 1);                        // runs while the gradients of tile i are computed
+                    ok = ok && warp_wait(ds_ready, i & 1, ab, 46);
+                    if (!ok) break;
+                    fence_after();
+                    if (elect()) {
+                        product_halves<DP>(dq_at, dp_at, k_at(i % ST), i > 0);
+                        commit(empty(i % ST));
+                    }
+                    if (i + 1 < total) gaps(i + 1);
+                }
+                if (elect()) commit(done);
+            }
+        } else if (warp == 2) {
+            if (total && blank_tile >= 0 && tile_of(list[total - 1]) == blank_tile) {
+                const int s = (total - 1) % ST;
+                if (warp_wait(blank_go, 0, ab, 47)) {
+                    for (int x = 0; x < DP / 64; ++x)
+                        for (int i = m.keys % kTile * 8 + lane; i < kTile * 8; i += 32)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(k_at(s) + x * box_bytes(kTile) + i * 16), "r"(0) : "memory");
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(blanked);
+                }
             }
         }
-    } else if (warp >= 4) {
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        // delta of the block's queries: DP / 8 lanes per row, 16 bytes each
+        constexpr int LPR = DP / 8;
+        const int64_t lines = ((int64_t)b * p.a.heads + h) * p.a.q_len;
+#pragma unroll 2
+        for (int r = (warp - 4) * (32 / LPR) + lane / LPR; r < kTile; r += 8 * (32 / LPR)) {
+            const int t = q0 + r, d = lane % LPR * 8;
+            float sum = 0.f;
+            if (t < p.a.q_len && d < p.a.dim) {
+                const uint4 x = *reinterpret_cast<const uint4*>((const bf16*)p.a.out + (int64_t)b * p.a.os.b + (int64_t)t * p.a.os.t + (int64_t)h * p.a.os.h + d);
+                const uint4 y = *reinterpret_cast<const uint4*>((const bf16*)p.a.dout + (int64_t)b * p.a.dos.b + (int64_t)t * p.a.dos.t + (int64_t)h * p.a.dos.h + d);
+                const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sum = fmaf(bf16_hi(xs[k]), bf16_hi(ys[k]), fmaf(bf16_lo(xs[k]), bf16_lo(ys[k]), sum));
+            }
+#pragma unroll
+            for (int o = LPR / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (d == 0) {
+                deltas[r] = sum;
+                if (t < p.a.q_len) p.a.delta[lines + t] = sum;
+            }
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");           // the eight compute warps; nothing before it can give up
         const int w = warp / 4 - 1, t = q0 + (threadIdx.x & 127);
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         const bool live = t < p.a.q_len;
         const int pos = m.start + t, end = live ? key_end(m, pos) : 0;
         const int my_doc = DOCS && live ? m.q_docs[t] : 0;
         const float slope = BIAS ? p.a.slopes[h] * kLog2e : 0.f;
-        const int64_t line = ((int64_t)b * p.a.heads + h) * p.a.q_len + t;
-        float lse2 = live ? p.a.lse[line] * kLog2e : INFINITY;
+        float lse2 = live ? p.a.lse[lines + t] * kLog2e : INFINITY;
         if (lse2 == -INFINITY) lse2 = INFINITY;
-        const float delta = live ? p.a.delta[line] : 0.f;
+        const float delta = deltas[threadIdx.x & 127];
         int* my_docs = docs + (warp - 4) * 64;
         bool ok = true;
         for (int i = 0; i < total; ++i) {
-            const int entry = list[i], key0 = (entry & 0x7fff) * kTile + 64 * w;
-            const bool partial = entry & 0x8000;
-            if (DOCS && partial) {
+            const int entry = list[i], key0 = tile_of(entry) * kTile + 64 * w;
+            const int cls = entry >> 14;
+            if (DOCS && cls == kDocs) {
                 __syncwarp();
                 for (int k = lane; k < 64; k += 32) my_docs[k] = key0 + k < p.a.k_len ? m.k_docs[key0 + k] : 0;
                 __syncwarp();
@@ -473,11 +530,21 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                 z[c] = make_float2(ex2(z[c].x), ex2(z[c].y));
                 g[c] = CAP ? mul2(g[c], z[c]) : z[c];
             }
-            if (partial) {
+            if (DOCS && cls == kDocs) {
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                    const int4 d = *reinterpret_cast<const int4*>(&my_docs[2 * c]);
+                    if (d.x != my_doc) g[c].x = 0.f;
+                    if (d.y != my_doc) g[c].y = 0.f;
+                    if (d.z != my_doc) g[c + 1].x = 0.f;
+                    if (d.w != my_doc) g[c + 1].y = 0.f;
+                }
+            }
+            if (cls >= kPartial) {
 #pragma unroll
                 for (int c = 0; c < 32; ++c) {
-                    if ((2 * c >= left) | (DOCS && my_docs[2 * c] != my_doc)) g[c].x = 0.f;
-                    if ((2 * c + 1 >= left) | (DOCS && my_docs[2 * c + 1] != my_doc)) g[c].y = 0.f;
+                    if (2 * c >= left) g[c].x = 0.f;
+                    if (2 * c + 1 >= left) g[c].y = 0.f;
                 }
             }
             ok = warp_wait(dp_full, i & 1, ab, 49);
@@ -487,7 +554,7 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
             ld32(dp_at + lanes + 64 * w, reinterpret_cast<uint32_t*>(gap));
             ld32(dp_at + lanes + 64 * w + 32, reinterpret_cast<uint32_t*>(gap) + 32);
             wait_ld();
-            if (partial) {                              // a masked pair's V may hold anything
+            if (cls >= kPartial) {                      // a masked pair's V may hold anything
 #pragma unroll
                 for (int c = 0; c < 32; ++c) { if (g[c].x == 0.f) gap[c].x = 0.f; if (g[c].y == 0.f) gap[c].y = 0.f; }
             }
@@ -516,17 +583,7 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
             }
         }
     }
-    __syncwarp();
-    if (ab.flag) {
-        const unsigned long long t0 = global_ns();
-        while (global_ns() - t0 < 200000ull) { }
-    }
-    fence_before();
-    __syncthreads();
-    if (warp == 1) {
-        fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
-    }
+    leave(ab, warp, tmem_slot);
 }
 
 template <int DP, bool CAP, bool BIAS, bool DOCS>
@@ -536,8 +593,8 @@ void launch_backward(ormi_b200_ctx* ctx, const CUtensorMap* maps, const TcParams
     auto q = attn_back_q<DP, CAP, BIAS, DOCS>;
     ORMI_CUDA(cudaFuncSetAttribute(kv, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     ORMI_CUDA(cudaFuncSetAttribute(q, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kv<<<dim3(p.a.batch * p.a.kv_heads, (p.a.k_len + kTile - 1) / kTile), kThreads, smem, ctx->stream>>>(maps[0], maps[1], maps[2], maps[3], p);
     q<<<dim3(p.a.batch * p.a.heads, (p.a.q_len + kTile - 1) / kTile), kThreads, smem, ctx->stream>>>(maps[0], maps[1], maps[2], maps[3], p);
+    kv<<<dim3(p.a.batch * p.a.kv_heads, (p.a.k_len + kTile - 1) / kTile), kThreads, smem, ctx->stream>>>(maps[0], maps[1], maps[2], maps[3], p);
     ORMI_CUDA(cudaGetLastError());
     count_launch(ctx, 2);
 }

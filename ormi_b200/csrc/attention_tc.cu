@@ -62,7 +62,7 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     // classes of the tiles, and which union tile holds the last valid key in its middle
     for (int j = threadIdx.x; j < tiles; j += kThreads) {
         int c = 0;
-        for (int w = 0; w < 2; ++w) c |= tile_class(p, b, q0 / kTile + w, lo[w], hi[w], j) << (2 * w);
+        for (int w = 0; w < 2; ++w) c |= tile_class<2, 2>(p, b, q0 / kUnit + 2 * w, lo[w], hi[w], 2 * j) << (2 * w);
         cls[j] = (unsigned char)c;
     }
     const int blank_tile = m.keys < p.a.k_len && m.keys % kTile ? m.keys / kTile : -1;
@@ -81,17 +81,21 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = tmem_slot;
+    // all of tensor memory is this block's, so it starts at column 0 (checked: every address below is a constant)
+    constexpr uint32_t tmem = 0;
+    const bool whole = tmem_slot == tmem;
+    if (!whole && threadIdx.x == 0) atomicCAS(p.err, 0, 20);
     auto s_at = [&](int w) { return tmem + w * 128; };
     auto o_at = [&](int w) { return tmem + 256 + w * 128; };
 
-    if (warp < 4) {
+    if (!whole) {
+    } else if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == 0 && lane == 0) {
             // ---------------------------------------------------------------- loads
             mbar_expect_tx(q_full, 2 * OP);
             for (int w = 0; w < 2; ++w)
-                for (int x = 0; x < DP / 64; ++x) tma_load_4d(q_at + w * OP + x * kBox, &map_q, q_full, 64 * x, q0 + w * kTile, h, b);
+                for (int x = 0; x < DP / 64; ++x) tma_load_4d(q_at + w * OP + x * box_bytes(kTile), &map_q, q_full, 64 * x, q0 + w * kTile, h, b);
             int seq = 0;
             bool ok = true;
             for (int j = 0; j < tiles && ok; ++j) {
@@ -101,53 +105,60 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     ok = mbar_wait(kv_empty(s), (seq / ST & 1) ^ 1, ab, 21);
                     if (!ok) break;
                     mbar_expect_tx(kv_full(s), OP);
-                    for (int x = 0; x < DP / 64; ++x) tma_load_4d(ring + s * OP + x * kBox, kv ? &map_v : &map_k, kv_full(s), 64 * x, j * kTile, kvh, b);
+                    for (int x = 0; x < DP / 64; ++x) tma_load_4d(ring + s * OP + x * box_bytes(kTile), kv ? &map_v : &map_k, kv_full(s), 64 * x, j * kTile, kvh, b);
                 }
             }
             // nothing of this block's is in flight when it leaves
             ok = ok && mbar_wait(q_full, 0, ab, 21);
             for (int i = 0; i < ST && ok; ++i, ++seq) ok = mbar_wait(kv_empty(seq % ST), (seq / ST & 1) ^ 1, ab, 21);
-        } else if (warp == 1 && lane == 0) {
+        } else if (warp == 1) {
             // ---------------------------------------------------------------- products
             int u = -1, prev = 0, prev_j = -1, used_p[2] = {0, 0};
-            bool ok = mbar_wait(q_full, 0, ab, 22);
+            bool ok = warp_wait(q_full, 0, ab, 22);
             for (int j = 0; j <= tiles && ok; ++j) {
                 const int c = j < tiles ? cls[j] : 0;
                 if (!c && j < tiles) continue;
                 if (c) ++u;
                 const int k_seq = 2 * u, v_seq = (c ? 2 * (u - 1) : 2 * u) + 1;      // K of this tile, V of the one before
+                const uint32_t k_buf = ring + (k_seq % ST) * OP, v_buf = ring + (v_seq % ST) * OP;
                 bool have_k = false, have_v = false;
-                for (int w = 0; w < 2 && ok; ++w) {
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    if (!ok) break;
                     if (prev >> (2 * w) & 3) {
                         if (!have_v) {
-                            ok = mbar_wait(kv_full(v_seq % ST), v_seq / ST & 1, ab, 23);
+                            ok = warp_wait(kv_full(v_seq % ST), v_seq / ST & 1, ab, 23);
                             if (ok && prev_j == blank_tile) {              // warp 2 may begin: these rows have landed
-                                mbar_arrive(blank_go);
-                                ok = mbar_wait(v_blank, 0, ab, 24);
+                                if (lane == 0) mbar_arrive(blank_go);
+                                ok = warp_wait(v_blank, 0, ab, 24);
                             }
                             have_v = true;
                         }
-                        ok = ok && mbar_wait(p_full(w), used_p[w] & 1, ab, 25);
+                        ok = ok && warp_wait(p_full(w), used_p[w] & 1, ab, 25);
                         if (!ok) break;
                         fence_after();
-                        product_tn<DP>(o_at(w), s_at(w), ring + (v_seq % ST) * OP, used_p[w] > 0);
+                        if (elect()) product_tn<DP, kTile>(o_at(w), s_at(w), v_buf, used_p[w] > 0);
                         ++used_p[w];
                     }
                     if (c >> (2 * w) & 3) {
-                        if (!have_k) { ok = mbar_wait(kv_full(k_seq % ST), k_seq / ST & 1, ab, 26); have_k = true; }
+                        if (!have_k) { ok = warp_wait(kv_full(k_seq % ST), k_seq / ST & 1, ab, 26); have_k = true; }
                         if (!ok) break;
                         fence_after();
-                        product_nt<DP, kTile>(s_at(w), q_at + w * OP, ring + (k_seq % ST) * OP, 0);
-                        commit(s_full(w));
+                        if (elect()) {
+                            product_nt<DP, kTile>(s_at(w), q_at + w * OP, k_buf);
+                            commit(s_full(w));
+                        }
                     }
                 }
                 if (!ok) break;
-                if (prev) commit(kv_empty(v_seq % ST));
-                if (c) commit(kv_empty(k_seq % ST));
+                if (elect()) {
+                    if (prev) commit(kv_empty(v_seq % ST));
+                    if (c) commit(kv_empty(k_seq % ST));
+                }
                 prev = c;
                 prev_j = j;
             }
-            commit(o_full);
+            if (elect()) commit(o_full);
         } else if (warp == 2 && blank_tile >= 0 && blank_tile < tiles && cls[blank_tile]) {
             // ---------------------------------------------------------------- rows of V behind key_len: zero, whatever they held
             // (the issuer says when V has landed: a parity wait of this warp's own on the ring could be a phase late or early)
@@ -158,7 +169,7 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 const int first = m.keys % kTile;
                 for (int x = 0; x < DP / 64; ++x)
                     for (int i = first * 8 + lane; i < kTile * 8; i += 32)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(ring + s * OP + x * kBox + i * 16), "r"(0) : "memory");
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(ring + s * OP + x * box_bytes(kTile) + i * 16), "r"(0) : "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(v_blank);
@@ -182,7 +193,7 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             const int c = cls[j] >> (2 * w) & 3;
             if (!c) continue;
             const int key0 = j * kTile;
-            if (DOCS && c == kPartial) {
+            if (DOCS && c == kDocs) {
                 __syncwarp();
                 for (int i = lane; i < kTile; i += 32) my_docs[i] = key0 + i < p.a.k_len ? m.k_docs[key0 + i] : 0;
                 __syncwarp();
@@ -215,12 +226,22 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     }
                 }
             }
-            if (c == kPartial) {
+            if (DOCS && c == kDocs) {
+#pragma unroll
+                for (int i = 0; i < 64; i += 2) {
+                    const int4 d = *reinterpret_cast<const int4*>(&my_docs[2 * i]);
+                    if (d.x != my_doc) z[i].x = -INFINITY;
+                    if (d.y != my_doc) z[i].y = -INFINITY;
+                    if (d.z != my_doc) z[i + 1].x = -INFINITY;
+                    if (d.w != my_doc) z[i + 1].y = -INFINITY;
+                }
+            }
+            if (c >= kPartial) {
                 const int left = end - key0;
 #pragma unroll
                 for (int i = 0; i < 64; ++i) {
-                    if ((2 * i >= left) | (DOCS && my_docs[2 * i] != my_doc)) z[i].x = -INFINITY;
-                    if ((2 * i + 1 >= left) | (DOCS && my_docs[2 * i + 1] != my_doc)) z[i].y = -INFINITY;
+                    if (2 * i >= left) z[i].x = -INFINITY;
+                    if (2 * i + 1 >= left) z[i].y = -INFINITY;
                 }
             }
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -300,28 +321,26 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     __syncthreads();
     if (warp == 1) {
         fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_slot), "r"(512) : "memory");
     }
 }
 
-// Smallest and largest document of every tile of 128 positions, of the queries and then of the keys: a warp per tile.
+// Smallest and largest document of every unit of 64 positions, of the queries and then of the keys: a warp per unit.
 __global__ void __launch_bounds__(256) attn_doc_bounds(TcParams p, int2* bounds) {
     int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int64_t q_count = (int64_t)p.a.batch * p.q_tiles;
-    if (at >= q_count + (int64_t)p.a.batch * p.k_tiles) return;
+    const int64_t q_count = (int64_t)p.a.batch * p.q_units;
+    if (at >= q_count + (int64_t)p.a.batch * p.k_units) return;
     bounds += at;
     const bool keys = at >= q_count;
     if (keys) at -= q_count;
-    const int tiles = keys ? p.k_tiles : p.q_tiles, len = keys ? p.a.k_len : p.a.q_len;
-    const int32_t* docs = (keys ? p.a.k_docs : p.a.q_docs) + at / tiles * len;
-    const int j = at % tiles, lane = threadIdx.x & 31;
+    const int units = keys ? p.k_units : p.q_units, len = keys ? p.a.k_len : p.a.q_len;
+    const int32_t* docs = (keys ? p.a.k_docs : p.a.q_docs) + at / units * len;
+    const int first = at % units * kUnit + (threadIdx.x & 31);
     int lo = INT32_MAX, hi = INT32_MIN;
-    for (int i = j * kTile + lane; i < min((j + 1) * kTile, len); i += 32) {
-        lo = min(lo, docs[i]); hi = max(hi, docs[i]);
-    }
+    for (int i = first; i < min(first + kUnit, len); i += 32) { lo = min(lo, docs[i]); hi = max(hi, docs[i]); }
     lo = __reduce_min_sync(0xffffffffu, lo);
     hi = __reduce_max_sync(0xffffffffu, hi);
-    if (lane == 0) *bounds = make_int2(lo, hi);
+    if ((threadIdx.x & 31) == 0) *bounds = make_int2(lo, hi);
 }
 
 template <int DP, bool CAP, bool BIAS, bool DOCS>
@@ -366,15 +385,15 @@ bool map_allowed(const void* ptr, const Strides4& s, int batch, int len, int hea
 }
 
 size_t bounds_bytes(const AttnParams& p) {
-    return p.k_docs ? (size_t)p.batch * ((p.q_len + kTile - 1) / kTile + 1 + (p.k_len + kTile - 1) / kTile) * sizeof(int2) : 0;
+    // (the forward kernel looks at two tiles of queries, of which the second may not exist)
+    return p.k_docs ? (size_t)p.batch * (units_of(p.q_len + kTile) + units_of(p.k_len)) * sizeof(int2) : 0;
 }
 
 TcParams tc_params(ormi_b200_ctx* ctx, const AttnParams& a, int2* bounds) {
     TcParams p{};
     p.a = a;
-    p.q_tiles = (a.q_len + kTile - 1) / kTile;
-    p.q_tiles += p.q_tiles & 1;                                  // a block looks at two tiles of queries
-    p.k_tiles = (a.k_len + kTile - 1) / kTile;
+    p.q_units = units_of(a.q_len + kTile);
+    p.k_units = units_of(a.k_len);
     p.scale_log2 = a.scale * kLog2e;
     p.cap_log2 = a.cap * kLog2e;
     if (a.cap > 0.f) {
@@ -385,8 +404,8 @@ TcParams tc_params(ormi_b200_ctx* ctx, const AttnParams& a, int2* bounds) {
     p.err = device_error_word(ctx);
     ctx->gemm_err_pending = true;
     if (a.k_docs) {
-        int2* kb = bounds + (size_t)a.batch * p.q_tiles;
-        attn_doc_bounds<<<(int)(((int64_t)a.batch * (p.q_tiles + p.k_tiles) + 7) / 8), 256, 0, ctx->stream>>>(p, bounds);
+        int2* kb = bounds + (size_t)a.batch * p.q_units;
+        attn_doc_bounds<<<(int)(((int64_t)a.batch * (p.q_units + p.k_units) + 7) / 8), 256, 0, ctx->stream>>>(p, bounds);
         ORMI_CUDA(cudaGetLastError());
         count_launch(ctx);
         p.q_bounds = bounds; p.k_bounds = kb;

@@ -6,30 +6,34 @@
 
 namespace ormi_b200 {
 
-constexpr int kTile = 128;                       // queries, and keys, of a tile
-constexpr int kMaxTiles = 8192;                  // tiles of keys (or queries) that a block keeps a class for: 2^20 positions
-enum TileClass { kSkip = 0, kFull = 1, kPartial = 2 };   // no pair visible; every pair; look at each
+constexpr int kTile = 128, kUnit = 64;           // positions of a tile, and of half of one
+constexpr int kMaxTiles = 8192;                  // tiles (forward) or units (backward) that a block keeps a class for
+enum TileClass { kSkip = 0, kFull = 1, kPartial = 2, kDocs = 3 };   // no pair visible; every pair; look at positions; and at documents too
 
 struct TcParams {
     AttnParams a;
-    const int2 *q_bounds, *k_bounds;             // smallest and largest document of every tile, [batch][tiles]; NULL without documents
-    int q_tiles, k_tiles;
+    const int2 *q_bounds, *k_bounds;             // smallest and largest document of every unit, [batch][units]; NULL without documents
+    int q_units, k_units;                        // even
     float scale_log2, cap_log2;                  // scale * log2(e), cap * log2(e)
     float x_per_raw, exp_per_raw, poly_limit;    // with a cap: scale / cap, 2 log2(e) scale / cap, the largest |raw| for the polynomial
     int* err;
 };
 
-// Class of (queries first .. first + 127, tile of keys j).  `lo` and `hi`: key_end of the first and the last row that exists.
-__device__ __forceinline__ int tile_class(const TcParams& p, int b, int q_tile, int lo, int hi, int j) {
-    const int key0 = j * kTile;
+// Class of QU units of queries from q_unit on against KU units of keys from k_unit on.  `lo` and `hi`: key_end of the first
+// query and of the last one that exists.
+template <int QU, int KU>
+__device__ __forceinline__ int tile_class(const TcParams& p, int b, int q_unit, int lo, int hi, int k_unit) {
+    const int key0 = k_unit * kUnit;
     if (key0 >= hi) return kSkip;
-    int c = key0 + kTile <= lo ? kFull : kPartial;
-    if (p.k_bounds) {
-        const int2 q = p.q_bounds[(int64_t)b * p.q_tiles + q_tile], k = p.k_bounds[(int64_t)b * p.k_tiles + j];
-        if (k.y < q.x || k.x > q.y) return kSkip;
-        if (!(k.x == k.y && q.x == q.y)) c = kPartial;
-    }
-    return c;
+    const int c = key0 + KU * kUnit <= lo ? kFull : kPartial;
+    if (!p.k_bounds) return c;
+    const int2* qb = p.q_bounds + (int64_t)b * p.q_units + q_unit;
+    const int2* kb = p.k_bounds + (int64_t)b * p.k_units + k_unit;
+    int2 q = qb[0], k = kb[0];
+    if (QU == 2) q = make_int2(min(q.x, qb[1].x), max(q.y, qb[1].y));
+    if (KU == 2) k = make_int2(min(k.x, kb[1].x), max(k.y, kb[1].y));
+    if (k.y < q.x || k.x > q.y) return kSkip;
+    return k.x == k.y && q.x == q.y ? c : kDocs;
 }
 
 // Raw products to base-2 scores under a cap, in place: z = cap tanh(x), x = raw * scale / cap; `dcap`, when given, receives
@@ -74,5 +78,6 @@ void head_map(ormi_b200_ctx* ctx, CUtensorMap* map, const void* ptr, const Strid
 bool map_allowed(const void* ptr, const Strides4& s, int batch, int len, int heads);
 TcParams tc_params(ormi_b200_ctx* ctx, const AttnParams& p, int2* bounds);
 size_t bounds_bytes(const AttnParams& p);
+template <typename T> inline int units_of(T len) { return (int)((len + kTile - 1) / kTile) * 2; }
 
 }  // namespace ormi_b200

@@ -43,19 +43,17 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
                  ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-// Shared-memory matrix descriptor, 128-byte swizzle.  The tiles here are boxes of 64 values (128 bytes) x 128 rows, 16 KB,
-// one box for every 64 values of a row.
+// Shared-memory matrix descriptor, 128-byte swizzle.  Operands are boxes of 64 values (128 bytes) x `rows` rows, one box for
+// every 64 values of a row.
 //   K-major (the product runs along the 64 values): 8-row groups 1024 bytes apart; the next 16 k are 32 bytes on.
 //   MN-major (the product runs along the rows): 8-row groups 1024 bytes apart, the next 64 columns one box on; the next 16
 //   k are 2048 bytes on.
-constexpr int kBox = 16384;
-__device__ __forceinline__ uint64_t desc(uint32_t addr, bool mn_major) {
-    uint64_t d = (addr & 0x3FFFF) >> 4;
-    d |= (uint64_t)(mn_major ? (kBox >> 4) : 1) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
+__host__ __device__ constexpr int box_bytes(int rows) { return rows * 128; }
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+template <int ROWS> __device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(ROWS * 128 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 // bf16 operands, fp32 accumulation, M = 128.
 __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
@@ -70,21 +68,30 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                  ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate) : "memory");
 }
-// D[128 x N] (+)= A[128 x DP] . B[N x DP]^T, both K-major boxes.
+// D[128 x N] = A[128 x DP] . B[N x DP]^T, both K-major, A in boxes of 128 rows and B in boxes of N.
 template <int DP, int N>
-__device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t b, uint32_t accumulate) {
+__device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t b) {
+    const uint64_t da = desc_k(a), db = desc_k(b);
 #pragma unroll
-    for (int k = 0; k < DP / 16; ++k) {
-        const uint32_t off = (k / 4) * kBox + (k % 4) * 32;
-        mma_ss(d, desc(a, false) + (off >> 4), desc(b, false) + (off >> 4), idesc(N, false), accumulate || k > 0);
-    }
+    for (int k = 0; k < DP / 16; ++k)
+        mma_ss(d, da + (((k / 4) * (128 * 128) + (k % 4) * 32) >> 4), db + (((k / 4) * (N * 128) + (k % 4) * 32) >> 4), idesc(N, false), k > 0);
 }
-// D[128 x DP] (+)= A[128 x 128] . B[128 x DP], A in tensor memory, B's rows along the product.
-template <int DP>
+// D[128 x DP] (+)= A[128 x K] . B[K x DP], A in tensor memory, B in boxes of K rows, which run along the product.
+template <int DP, int K>
 __device__ __forceinline__ void product_tn(uint32_t d, uint32_t a, uint32_t b, uint32_t accumulate) {
+    const uint64_t db = desc_mn<K>(b);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) mma_ts(d, a + k * 8, desc(b, true) + ((k * 2048) >> 4), idesc(DP, true), accumulate || k > 0);
+    for (int k = 0; k < K / 16; ++k) mma_ts(d, a + k * 8, db + ((k * 2048) >> 4), idesc(DP, true), accumulate || k > 0);
 }
+// True in one lane of a converged warp.  The products are issued by a whole warp that runs its loop together and elects a
+// lane around the instructions only: their descriptors then live in uniform registers.  (Issued from a branch that a single
+// thread took, every product cost 60-70 cycles of moving its operands there, more than the product itself.)
+__device__ __forceinline__ bool elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 // Arrives on `bar` once every tcgen05 operation this thread has issued is complete.
 __device__ __forceinline__ void commit(uint32_t bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
