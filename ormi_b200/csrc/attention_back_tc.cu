@@ -45,20 +45,6 @@ __device__ __forceinline__ int list_tiles(unsigned short* list, int tiles, F&& c
 }
 __device__ __forceinline__ int tile_of(unsigned short entry) { return entry & 0x3fff; }
 
-// 32 columns of tensor memory to 32 bf16 values of a row, times `by`.
-__device__ __forceinline__ void store_row32(bf16* out, int x, int dim, const uint32_t* o, float by) {
-#pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-        if (x + i >= dim) break;
-        uint4 v;
-        v.x = pack_bf16x2(__uint_as_float(o[i]) * by, __uint_as_float(o[i + 1]) * by);
-        v.y = pack_bf16x2(__uint_as_float(o[i + 2]) * by, __uint_as_float(o[i + 3]) * by);
-        v.z = pack_bf16x2(__uint_as_float(o[i + 4]) * by, __uint_as_float(o[i + 5]) * by);
-        v.w = pack_bf16x2(__uint_as_float(o[i + 6]) * by, __uint_as_float(o[i + 7]) * by);
-        *reinterpret_cast<uint4*>(out + x + i) = v;
-    }
-}
-
 // A operand of 128 bf16 columns that two warpgroups wrote into the first halves of their own 64 columns.
 template <int DP>
 __device__ __forceinline__ void product_halves(uint32_t d, uint32_t a, uint32_t b, uint32_t accumulate) {
@@ -317,13 +303,14 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             // warpgroup 0 writes dV, warpgroup 1 dK; keys that nobody sees get zero
             fence_after();
             const Strides4& os = w ? p.a.dks : p.a.dvs;
-            bf16* out = (bf16*)(w ? p.a.dk : p.a.dv) + (int64_t)b * os.b + (int64_t)key * os.t + (int64_t)kvh * os.h;
+            const int first = key0 + (warp & 3) * 32;
+            bf16* out = (bf16*)(w ? p.a.dk : p.a.dv) + (int64_t)b * os.b + (int64_t)first * os.t + (int64_t)kvh * os.h;
 #pragma unroll 1
             for (int x = 0; x < DP; x += 32) {
                 uint32_t o[32];
                 if (total) { ld32((w ? dk_at : dv_at) + lanes + x, o); wait_ld(); }
                 else for (int i = 0; i < 32; ++i) o[i] = 0;
-                if (key < p.a.k_len) store_row32(out, x, p.a.dim, o, w ? p.a.scale : 1.f);
+                store_block32(k_at + (warp - 4) * 2048, o, w ? p.a.scale : 1.f, p.a.k_len - first, p.a.dim - x, [&](int r) { return out + r * os.t + x; });
             }
         }
     }
@@ -467,19 +454,26 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // delta of the block's queries: DP / 8 lanes per row, 16 bytes each
-        constexpr int LPR = DP / 8;
+        constexpr int LPR = DP / 8, RPW = 32 / LPR, TURNS = kTile / (8 * RPW);
         const int64_t lines = ((int64_t)b * p.a.heads + h) * p.a.q_len;
-#pragma unroll 2
-        for (int r = (warp - 4) * (32 / LPR) + lane / LPR; r < kTile; r += 8 * (32 / LPR)) {
-            const int t = q0 + r, d = lane % LPR * 8;
-            float sum = 0.f;
-            if (t < p.a.q_len && d < p.a.dim) {
-                const uint4 x = *reinterpret_cast<const uint4*>((const bf16*)p.a.out + (int64_t)b * p.a.os.b + (int64_t)t * p.a.os.t + (int64_t)h * p.a.os.h + d);
-                const uint4 y = *reinterpret_cast<const uint4*>((const bf16*)p.a.dout + (int64_t)b * p.a.dos.b + (int64_t)t * p.a.dos.t + (int64_t)h * p.a.dos.h + d);
-                const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+        const int d = lane % LPR * 8;
+        uint4 xs[TURNS], ys[TURNS];                               // everything is asked for first
 #pragma unroll
-                for (int k = 0; k < 4; ++k) sum = fmaf(bf16_hi(xs[k]), bf16_hi(ys[k]), fmaf(bf16_lo(xs[k]), bf16_lo(ys[k]), sum));
+        for (int k = 0; k < TURNS; ++k) {
+            const int t = q0 + (k * 8 + warp - 4) * RPW + lane / LPR;
+            xs[k] = ys[k] = make_uint4(0, 0, 0, 0);
+            if (t < p.a.q_len && d < p.a.dim) {
+                xs[k] = *reinterpret_cast<const uint4*>((const bf16*)p.a.out + (int64_t)b * p.a.os.b + (int64_t)t * p.a.os.t + (int64_t)h * p.a.os.h + d);
+                ys[k] = *reinterpret_cast<const uint4*>((const bf16*)p.a.dout + (int64_t)b * p.a.dos.b + (int64_t)t * p.a.dos.t + (int64_t)h * p.a.dos.h + d);
             }
+        }
+#pragma unroll
+        for (int k = 0; k < TURNS; ++k) {
+            const int r = (k * 8 + warp - 4) * RPW + lane / LPR, t = q0 + r;
+            const uint32_t x[4] = {xs[k].x, xs[k].y, xs[k].z, xs[k].w}, y[4] = {ys[k].x, ys[k].y, ys[k].z, ys[k].w};
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum = fmaf(bf16_hi(x[e]), bf16_hi(y[e]), fmaf(bf16_lo(x[e]), bf16_lo(y[e]), sum));
 #pragma unroll
             for (int o = LPR / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             if (d == 0) {
@@ -573,13 +567,14 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         if (ok && total) ok = warp_wait(done, 0, ab, 50);
         if (ok) {
             fence_after();
-            bf16* out = (bf16*)p.a.dq + (int64_t)b * p.a.dqs.b + (int64_t)t * p.a.dqs.t + (int64_t)h * p.a.dqs.h;
+            const int first = q0 + (warp & 3) * 32;
+            bf16* out = (bf16*)p.a.dq + (int64_t)b * p.a.dqs.b + (int64_t)first * p.a.dqs.t + (int64_t)h * p.a.dqs.h;
 #pragma unroll 1
             for (int x = w * (DP / 2); x < (w + 1) * (DP / 2); x += 32) {          // a half of the columns each
                 uint32_t o[32];
                 if (total) { ld32(dq_at + lanes + x, o); wait_ld(); }
                 else for (int i = 0; i < 32; ++i) o[i] = 0;
-                if (live) store_row32(out, x, p.a.dim, o, p.a.scale);
+                store_block32(q_at + (warp - 4) * 2048, o, p.a.scale, p.a.q_len - first, p.a.dim - x, [&](int r) { return out + r * p.a.dqs.t + x; });
             }
         }
     }

@@ -10,6 +10,7 @@
 // O is rescaled only when a row's maximum has grown by more than 2^8 since the last time: probabilities up to 256 lose
 // nothing in fp32 sums nor, relatively, in bf16.
 #include <algorithm>
+#include <cmath>
 
 #include "attention_tc.cuh"
 
@@ -286,27 +287,19 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             if (lane == 0) mbar_arrive(p_full(w));
             ++n;
         }
-        if (ok && n) ok = warp_wait(o_full, 0, ab, 29);
+        if (ok) ok = warp_wait(o_full, 0, ab, 29);
         if (ok) {
             fence_after();
             const float by = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
-            bf16* out = (bf16*)p.a.out + (int64_t)b * p.a.os.b + (int64_t)t * p.a.os.t + (int64_t)h * p.a.os.h;
+            // the rings are idle now: their memory stages the rows
+            const int t0 = q0 + w * kTile + (warp & 3) * 32;
+            bf16* out = (bf16*)p.a.out + (int64_t)b * p.a.os.b + (int64_t)t0 * p.a.os.t + (int64_t)h * p.a.os.h;
 #pragma unroll 1
             for (int x = 0; x < DP; x += 32) {
                 uint32_t o[32];
                 if (n) { ld32(o_at(w) + lanes + x, o); wait_ld(); }
                 else for (int i = 0; i < 32; ++i) o[i] = 0;
-                if (!live) continue;
-#pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    if (x + i >= p.a.dim) break;
-                    uint4 v;
-                    v.x = pack_bf16x2(__uint_as_float(o[i]) * by, __uint_as_float(o[i + 1]) * by);
-                    v.y = pack_bf16x2(__uint_as_float(o[i + 2]) * by, __uint_as_float(o[i + 3]) * by);
-                    v.z = pack_bf16x2(__uint_as_float(o[i + 4]) * by, __uint_as_float(o[i + 5]) * by);
-                    v.w = pack_bf16x2(__uint_as_float(o[i + 6]) * by, __uint_as_float(o[i + 7]) * by);
-                    *reinterpret_cast<uint4*>(out + x + i) = v;
-                }
+                store_block32(ring + (warp - 4) * 2048, o, by, p.a.q_len - t0, p.a.dim - x, [&](int r) { return out + r * p.a.os.t + x; });
             }
             if (live && p.a.lse) p.a.lse[((int64_t)b * p.a.heads + h) * p.a.q_len + t] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
         }
@@ -397,9 +390,14 @@ TcParams tc_params(ormi_b200_ctx* ctx, const AttnParams& a, int2* bounds) {
     p.scale_log2 = a.scale * kLog2e;
     p.cap_log2 = a.cap * kLog2e;
     if (a.cap > 0.f) {
-        p.x_per_raw = a.scale / a.cap;
-        p.exp_per_raw = 2.f * kLog2e * a.scale / a.cap;
-        p.poly_limit = 0.5f * a.cap / a.scale;
+        const double k = (double)a.scale / a.cap, c = (double)a.scale * 1.4426950408889634;
+        static const double p3[3] = {0.9999996059266845, -0.33321928380355686, 0.12841935404930116}, p5[5] = {0.9999999870693153, -0.3333307189419646, 0.13324828997681853, -0.052989241174570344, 0.017141319046484527};
+        for (int i = 0; i < 3; ++i) p.poly3[i] = (float)(c * p3[i] * std::pow(k, 2 * i));
+        for (int i = 0; i < 5; ++i) p.poly5[i] = (float)(c * p5[i] * std::pow(k, 2 * i));
+        p.limit3 = (float)std::min(0.25 / k, 1e15);               // (a square that overflows has no business here)
+        p.limit5 = (float)std::min(0.5 / k, 1e15);
+        p.exp_per_raw = (float)(2 * 1.4426950408889634 * k);
+        p.minus_inv_cap2 = -1.f / (p.cap_log2 * p.cap_log2);
     }
     p.err = device_error_word(ctx);
     ctx->gemm_err_pending = true;
