@@ -270,19 +270,33 @@ class AdamW:
                 codes.append(code)
             blob.append(_ADAM_TENSOR.pack(*ptrs, count, codes[1], decay[i]))
         self.dev, self.n, self.blob = dev, n, b"".join(blob)
+        self._grads = [(_FLAT.unpack(_pack(g, dev.index))[1], G.numel(g.shape)) for g in lists[1]]
         self.betas, self.eps, self.seed = betas, float(eps), int(seed)
         self.steps_done = 0
         self._keepalive = lists
 
-    def step(self, lr: float = 0.0, *, step: int | None = None, grad_scale=None, device_lr=None, device_step=None):
-        """One update.  ``step`` counts from 1 and defaults to one more than the last one.  ``grad_scale`` and ``device_lr``
-        (replaces ``lr``): f32 device scalars.  ``device_step``: address of a 64-bit device counter of the steps done,
+    def step(self, lr: float = 0.0, *, step: int | None = None, grads=None, grad_scale=None, device_lr=None, device_step=None):
+        """One update.  ``step`` counts from 1 and defaults to one more than the last one.  ``grads``: this step's gradients
+        where they are not the buffers of the constructor (same types and sizes).  ``grad_scale`` and ``device_lr`` (replaces
+        ``lr``): f32 device scalars.  ``device_step``: address of a 64-bit device counter of the steps done,
         which the call reads and increments, for steps that are captured and replayed."""
+        blob = self.blob
+        if grads is not None:
+            if len(grads) != self.n:
+                raise ValueError("every list names one buffer for each parameter")
+            blob = bytearray(blob)
+            for i, g in enumerate(grads):
+                ptr, code, ndim, *dims = _FLAT.unpack(_pack(g, self.dev.index))
+                shape = dims[:ndim]
+                if (code, G.numel(shape)) != self._grads[i] or any(a != 1 and b != c for a, b, c in zip(shape, dims[4:4 + ndim], G.calc_contiguous_strides(shape))):
+                    raise ValueError(f"tensor {i}: the gradient has another type or size, or is not contiguous")
+                struct.pack_into("=Q", blob, i * _ADAM_TENSOR.size + 8, ptr)
+            blob = bytes(blob)
         if device_step is None:
             self.steps_done = self.steps_done + 1 if step is None else int(step)
         config = _ADAM_CONFIG.pack(lr, self.betas[0], self.betas[1], self.eps, self.steps_done, _scalar(device_step, 8, self.dev), _scalar(device_lr, 4, self.dev),
                                    _scalar(grad_scale, 4, self.dev), self.seed & 0xffffffff, self.state_bits)
-        check(lib.ormi_b200_adamw(self.dev.handle, self.blob, self.n, config))
+        check(lib.ormi_b200_adamw(self.dev.handle, blob, self.n, config))
 
 
 def _scalar(x, size: int, dev) -> int:

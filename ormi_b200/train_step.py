@@ -8,7 +8,8 @@ module adds is the host loop a data-parallel job needs around ``ormi_b200_realiz
   waits for each bucket only where its sums are first read (``ormi_b200_comm_mark`` / ``ormi_b200_comm_wait``);
 * each phase is flattened once; every later step patches the device pointers of its inputs into the flattened
   graph and hands it to the backend again (plan and kernels come from the caches), so a step costs a few C calls;
-* parameters ping-pong: the update phase returns fresh buffers that become the next step's leaves.
+* parameters ping-pong: the update phase returns fresh buffers that become the next step's leaves (SGD), or they are
+  updated in place by one launch over all of them (AdamW, ormi_b200/ops.py).
 
 Sharding rule (rows of x and t are split evenly over the ranks, weights are replicated): each rank's loss is
 scaled by 1 / (global_batch * D), so the *sum* of the local gradients over ranks is the gradient of the global
@@ -22,6 +23,7 @@ from typing import Callable, Sequence
 import numpy as np
 
 from . import graph as G
+from . import ops
 from . import workloads as W
 from ._lib import lib, check
 
@@ -132,11 +134,17 @@ class MLPTrainer:
 
     so bucket 1 hides behind the dW2 GEMM and bucket 2 behind the next step's first GEMM.  `flush` applies the
     update that is still pending after the last step.
+
+    ``optimizer="adamw"`` puts an in-place AdamW step (``adamw``: keyword arguments of :class:`ormi_b200.ops.AdamW` such as
+    ``betas``, ``eps``, ``weight_decay``, ``seed``, and ``state_bits`` 32 or 8) where U2 and U1 stand; the biases are not
+    decayed.  In "bf16" matmul arithmetic the same launch rewrites the weights' bf16 copies.
     """
 
     def __init__(self, dev, x, t, w1, b1, w2, b2, lr: float, global_batch: int | None = None, world: int = 1,
-                 overlap: bool = True, bf16_matmuls: bool | None = None):
-        self.dev, self.world, self.overlap = dev, world, overlap
+                 overlap: bool = True, bf16_matmuls: bool | None = None, optimizer: str = "sgd", adamw: dict | None = None):
+        if optimizer not in ("sgd", "adamw"):
+            raise ValueError(f'optimizer is "sgd" or "adamw", not {optimizer!r}')
+        self.dev, self.world, self.overlap, self.lr = dev, world, overlap, lr
         if bf16_matmuls is None:
             bf16_matmuls = dev.get_option("matmul") == "bf16"
         B, D = x.shape[0], t.shape[1]
@@ -158,7 +166,14 @@ class MLPTrainer:
             # writes their bf16 copies along (the flag is ignored by the other arithmetics)
             node.twin16 = k in ("w1", "w2")
             return node
-        if world == 1:
+        self._adamw = {}
+        if optimizer == "adamw":
+            for group in (("w1", "b1"), ("w2", "b2")) if world > 1 else (tuple(self.names),):
+                self._adamw[group] = self._make_adamw(group, {k: params[k] for k in group}, dict(adamw or {}))
+        if world == 1 and self._adamw:
+            p.intermediates = "free"
+            p.add_phase([loss] + [grads[k] for k in self.names])
+        elif world == 1:
             # one realize call per step whose roots are all that is read afterwards
             p.intermediates = "free"
             ups = [weight_update(W.sgd_update(params[k], lr), k) for k in self.names]
@@ -181,17 +196,40 @@ class MLPTrainer:
             # h is read by two matmuls of later phases and by nothing else: in "bf16" arithmetic it leaves phase F as a
             # bf16 matrix only (the backend hands back what it made; with other arithmetics the flag is not set)
             taps["h"].bf16 = bf16_matmuls
-            p.add_phase([taps["h"]])                             # F
-            p.add_phase([up["w2"], up["b2"]])                    # U2
-            p.add_phase([loss, grads["w1"], grads["b1"]])        # B1
-            p.add_phase([grads["w2"], grads["b2"]])              # B2
-            p.add_phase([up["w1"], up["b1"]])                    # U1
+            phases = [("F", [taps["h"]]), ("U2", [up["w2"], up["b2"]]), ("B1", [loss, grads["w1"], grads["b1"]]),
+                      ("B2", [grads["w2"], grads["b2"]]), ("U1", [up["w1"], up["b1"]])]
+            self._phase = {}
+            for name, roots in phases:
+                if self._adamw and name in ("U1", "U2"):
+                    continue
+                self._phase[name] = len(p.phases)
+                p.add_phase(roots)
             self._pending = None          # (dW2, db2) of the last step, still to be applied
         self.loss_ptr = None
         self.steps_done = 0
         self._initial = set(self.names)   # parameters still in the buffers the constructor uploaded
         # the build pass above already ran one step worth of kernels but did not move the parameters
         dev.sync()
+
+    def _make_adamw(self, group, params, options):
+        """The optimizer over a group of parameters; its states start at zero."""
+        dev, bits = self.dev, options.pop("state_bits", 32)
+        if bits not in (32, 8):
+            raise ValueError("state_bits is 32 or 8")
+        decay = options.pop("weight_decay", 0.0)
+        nodes = [params[k] for k in group]
+        kind = "f32" if bits == 32 else "e4m3"
+        states = [[ops.zeros(dev, [n.numel()], kind) for n in nodes] for _ in range(2)]
+        if bits == 8:
+            for name in ("m_scales", "v_scales"):
+                options[name] = [ops.zeros(dev, [-(-n.numel() // 128)]) for n in nodes]
+        flat = [ops.view(n.data.dev_ptr, [n.numel()]) for n in nodes]
+        return ops.AdamW(dev, flat, [ops.view(0x100, [n.numel()]) for n in nodes], *states,     # gradients come with every step
+                         weight_decay=[decay if k in ("w1", "w2") else 0.0 for k in group], **options)
+
+    def _adamw_step(self, group, grads):
+        """AdamW on `group` in place; `grads`: (address, bytes) of this step's gradients."""
+        self._adamw[group].step(lr=self.lr, grads=[ops.view(ptr, [nbytes // 4]) for ptr, nbytes in grads])
 
     def _allreduce(self, entries, slot):
         n = len(entries)
@@ -219,15 +257,22 @@ class MLPTrainer:
         """U2: the second layer's update with the gradients the previous step left behind."""
         p = self.prog
         self._wait(2)
-        res = p.run_phase(1, outs)
-        self._replace("w2", res[0])
-        self._replace("b2", res[1])
+        if self._adamw:
+            if self._pending is None:
+                return set()
+            self._adamw_step(("w2", "b2"), self._pending)
+            new = set()
+        else:
+            res = p.run_phase(self._phase["U2"], outs)
+            self._replace("w2", res[0])
+            self._replace("b2", res[1])
+            new = {res[0][0], res[1][0]}
         if self._pending is not None:
             for buf in self._pending:
                 self.dev.free(*buf)
             self._pending = None
         p.ext_ptr["gw2"], p.ext_ptr["gb2"] = self._zero["w2"], self._zero["b2"]
-        return {res[0][0], res[1][0]}
+        return new
 
     def step(self):
         p, dev = self.prog, self.dev
@@ -236,26 +281,33 @@ class MLPTrainer:
             res = p.run_phase(0, outs)
             loss = res[0]
             keep = {loss[0]}
-            for i, k in enumerate(self.names):
-                self._replace(k, res[1 + i])
-                keep.add(res[1 + i][0])
+            if self._adamw:
+                self._adamw_step(tuple(self.names), [res[1 + i] for i in range(len(self.names))])
+            else:
+                for i, k in enumerate(self.names):
+                    self._replace(k, res[1 + i])
+                    keep.add(res[1 + i][0])
         else:
-            p.run_phase(0, outs)                                   # F
+            p.run_phase(self._phase["F"], outs)                    # F
             keep = self._apply_pending(outs)                       # U2
-            res = p.run_phase(2, outs)                             # B1
+            res = p.run_phase(self._phase["B1"], outs)             # B1
             loss, dw1, db1 = res[0], res[1], res[2]
             self._allreduce([dw1, db1, loss], 1)
-            res = p.run_phase(3, outs)                             # B2
+            res = p.run_phase(self._phase["B2"], outs)             # B2
             dw2, db2 = res[0], res[1]
             self._allreduce([dw2, db2], 2)
             self._wait(1)
-            p.ext_ptr["gw1"], p.ext_ptr["gb1"] = dw1, db1
-            res = p.run_phase(4, outs)                             # U1
-            self._replace("w1", res[0])
-            self._replace("b1", res[1])
+            if self._adamw:
+                self._adamw_step(("w1", "b1"), (dw1, db1))
+                keep |= {dw2[0], db2[0], loss[0]}
+            else:
+                p.ext_ptr["gw1"], p.ext_ptr["gb1"] = dw1, db1
+                res = p.run_phase(self._phase["U1"], outs)         # U1
+                self._replace("w1", res[0])
+                self._replace("b1", res[1])
+                keep |= {res[0][0], res[1][0], dw2[0], db2[0], loss[0]}
             self._pending = (dw2, db2)
             p.ext_ptr["gw2"], p.ext_ptr["gb2"] = dw2, db2
-            keep |= {res[0][0], res[1][0], dw2[0], db2[0], loss[0]}
         # everything else this step produced goes back to the pool (stream-ordered: kernels already queued finish first)
         for ptr, nbytes in outs.get("owned", []):
             if ptr not in keep:

@@ -746,3 +746,208 @@ def test_adamw_with_a_device_counter_captured_and_replayed(device):
         step.destroy()
     finally:
         dev.close()
+
+
+# ---- together, and inside the training loop
+
+@gpu
+@pytest.mark.parametrize("matmul", ["fp32", "bf16"])
+def test_a_block_of_operators_trains_as_its_formulas_say(matmul):
+    """Norm, projection, attention, projection, norm, their gradients and an AdamW step, the products through the lazy graph."""
+    from ormi_b200.runtime import Device
+    dev = Device(0)
+    dev.set_option("matmul", matmul)
+    try:
+        B, N, W, H, HK, D = 2, 40, 128, 4, 2, 32
+        T, E = B * N, (H + 2 * HK) * D
+        rng = np.random.default_rng(5)
+        host = {k: rng.standard_normal(s).astype(np.float32) * c for k, s, c in (
+            ("x", (T, W), 1.0), ("r", (T, W), 1.0), ("g1", (W,), 1.0), ("wqkv", (W, E), W ** -0.5), ("wo", (H * D, W), (H * D) ** -0.5), ("g2", (W,), 1.0), ("c", (T, W), 1.0))}
+        docs = np.repeat(np.arange(2), N // 2)[None].repeat(B, 0).astype(np.int32)
+        masks = dict(causal=True, cap=8.0)
+
+        leaf = lambda b: G.Node(G.OpEnum.LEAF, data=b, requires_grad=True)      # noqa: E731
+        x, r, c = (dev.upload(host[k]) for k in ("x", "r", "c"))
+        g1, g2 = dev.upload(host["g1"]), dev.upload(host["g2"])
+        wqkv, wo = dev.leaf(host["wqkv"], True), dev.leaf(host["wo"], True)
+        d = ops.upload(dev, docs, "i32")
+        s1, h1, s2, h2, a = (dev.buffer([T, n]) for n in (W, W, W, W, H * D))
+        rstd1, rstd2, lse = dev.buffer([T]), dev.buffer([T]), dev.buffer([B, H, N])
+        heads = lambda b, first, n, width: ops.view(b.dev_ptr + first * D * 4, (B, N, n, D), "f32", (N * width, width, D, 1))      # noqa: E731
+        parts = lambda b: (heads(b, 0, H, E), heads(b, H, HK, E), heads(b, H + HK, HK, E))      # noqa: E731
+
+        ops.rmsnorm(dev, x, g1, h1, residual=r, residual_out=s1, rstd=rstd1)
+        h1n = leaf(h1)
+        qkv = G.matmul(h1n, wqkv)
+        dev.realize([qkv])
+        ops.attention(dev, *parts(qkv.data), heads(a, 0, H, H * D), lse, q_docs=d, k_docs=d, **masks)
+        an = leaf(a)
+        o = G.matmul(an, wo)
+        dev.realize([o])
+        ops.rmsnorm(dev, o, g2, h2, residual=s1, residual_out=s2, rstd=rstd2)
+
+        ds2, ds1, dg1, dg2, dqkv = dev.buffer([T, W]), dev.buffer([T, W]), dev.buffer([W]), dev.buffer([W]), dev.buffer([T, E])
+        ops.rmsnorm_backward(dev, c, s2, g2, rstd2, ds2, dg2)
+        o.grad = leaf(ds2)
+        G.compute_gradients(o)
+        dev.realize([an.grad, wo.grad])
+        ops.attention_backward(dev, heads(an.grad.data, 0, H, H * D), *parts(qkv.data), heads(a, 0, H, H * D), lse, *parts(dqkv), q_docs=d, k_docs=d, **masks)
+        qkv.grad = leaf(dqkv)
+        G.compute_gradients(qkv)
+        dev.realize([h1n.grad, wqkv.grad])
+        ops.rmsnorm_backward(dev, h1n.grad, s1, g1, rstd1, ds1, dg1, dresidual=ds2)
+
+        t = {k: torch.tensor(v, dtype=F8, requires_grad=True) for k, v in host.items()}
+        norm = lambda v, g: v / torch.sqrt(v.square().mean(-1, keepdim=True) + 1e-6) * g      # noqa: E731
+        z1 = t["x"] + t["r"]
+        q, k, v = (norm(z1, t["g1"]) @ t["wqkv"]).view(B, N, H + 2 * HK, D).split([H, HK, HK], 2)
+        k, v = (y.repeat_interleave(H // HK, 2) for y in (k, v))
+        z = 8.0 * torch.tanh(torch.einsum("bqhd,bkhd->bhqk", q, k) * D ** -0.5 / 8.0)
+        td = torch.tensor(docs)
+        seen = torch.tril(torch.ones(N, N, dtype=torch.bool))[None] & (td[:, :, None] == td[:, None, :])
+        att = torch.einsum("bhqk,bkhd->bqhd", torch.softmax(z.masked_fill(~seen[:, None], -math.inf), -1), v).reshape(T, H * D)
+        z2 = att @ t["wo"] + z1
+        out = norm(z2, t["g2"])
+        (out * t["c"]).sum().backward()
+        # fp32: a few hundred roundings of 2^-24 against the largest value; bf16 products: the framework's own bound for them
+        tol = 1e-4 if matmul == "fp32" else 3e-2
+        for name, got, want in (("h2", dev.download(h2), out), ("dx", dev.download(ds1), t["x"].grad), ("dr", dev.download(ds1), t["r"].grad), ("dg1", dev.download(dg1), t["g1"].grad),
+                                ("dg2", dev.download(dg2), t["g2"].grad), ("dwo", dev.numpy(wo.grad), t["wo"].grad), ("dwqkv", dev.numpy(wqkv.grad), t["wqkv"].grad)):
+            want = want.detach().numpy()
+            assert np.abs(got - want).max() <= tol * np.abs(want).max(), (name, np.abs(got - want).max() / np.abs(want).max())
+
+        params, grads = [wqkv, wo, g1, g2], [wqkv.grad, wo.grad, dg1, dg2]
+        states = [[ops.zeros(dev, p.shape) for p in params] for _ in range(2)]
+        before = [dev.download(p.data if isinstance(p, G.Node) else p) for p in params]
+        gh = [dev.download(g.data if isinstance(g, G.Node) else g) for g in grads]
+        ops.AdamW(dev, params, grads, *states, weight_decay=[0.1, 0.1, 0.0, 0.0]).step(lr=0.01)
+        for p, old, g, wd in zip(params, before, gh, (0.1, 0.1, 0.0, 0.0)):
+            want = old.astype(np.float64) * (1 - 0.01 * wd) - 0.01 * g / (np.abs(g.astype(np.float64)) + 1e-8)      # the first step: m / sqrt(v) is the sign
+            got = dev.download(p.data if isinstance(p, G.Node) else p)
+            assert np.abs(got - want).max() < 1e-5
+        # the next forward product sees the new weights (in "bf16" arithmetic through the copy that the optimizer rewrote)
+        again = G.matmul(leaf(h1), wqkv)
+        got = dev.numpy(again)
+        want = dev.download(h1).astype(np.float64) @ dev.download(wqkv.data).astype(np.float64)
+        assert np.abs(got - want).max() <= (1e-5 if matmul == "fp32" else 2e-2) * np.abs(want).max()
+    finally:
+        dev.close()
+
+
+def mlp(seed=3, B=96, D=64, F=128):
+    rng = np.random.default_rng(seed)
+    f = lambda *s: rng.standard_normal(s).astype(np.float32)      # noqa: E731
+    return f(B, D), f(B, D), f(D, F) / D ** 0.5, f(F) * 0.1, f(F, D) / F ** 0.5, f(D) * 0.1
+
+
+def mlp_grads(x, t, w1, b1, w2, b2):
+    p = [torch.tensor(v, dtype=F8, requires_grad=True) for v in (w1, b1, w2, b2)]
+    z = torch.tensor(x, dtype=F8) @ p[0] + p[1]
+    h = 0.5 * z * (1 + torch.tanh(math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)))
+    loss = ((h @ p[2] + p[3] - torch.tensor(t, dtype=F8)) ** 2).sum() / (x.shape[0] * t.shape[1])
+    loss.backward()
+    return float(loss.detach()), [v.grad.numpy() for v in p]
+
+
+@gpu
+@pytest.mark.parametrize("matmul, sharded", [("fp32", False), ("bf16", False), ("fp32", True)])
+def test_mlp_trainer_with_adamw(matmul, sharded, monkeypatch):
+    """Four steps of the training loop against AdamW in 64 bits.  `sharded`: the schedule of several ranks, run by one whose sums
+    over ranks are its own."""
+    from ormi_b200.runtime import Device
+    from ormi_b200.train_step import MLPTrainer
+    if sharded:
+        monkeypatch.setattr(MLPTrainer, "_allreduce", lambda self, entries, slot: None)
+        monkeypatch.setattr(MLPTrainer, "_wait", lambda self, slot: None)
+    dev = Device(0)
+    dev.set_option("matmul", matmul)
+    try:
+        x, t, *params = mlp()
+        lr, b1, b2, eps, wd = 0.01, 0.9, 0.99, 1e-3, 0.1
+        tr = MLPTrainer(dev, x, t, *params, lr=lr, world=2 if sharded else 1, global_batch=x.shape[0], optimizer="adamw", adamw=dict(betas=(b1, b2), eps=eps, weight_decay=wd))
+        p, m, v = [q.astype(np.float64) for q in params], [0.0] * 4, [0.0] * 4
+        for step in range(1, 5):
+            tr.step()
+            loss, grads = mlp_grads(x, t, *p)
+            assert abs(tr.loss() - loss) <= (1e-4 if matmul == "fp32" else 3e-2) * loss
+            for i, g in enumerate(grads):
+                m[i] = b1 * m[i] + (1 - b1) * g
+                v[i] = b2 * v[i] + (1 - b2) * g * g
+                p[i] = p[i] - lr * (wd if i in (0, 2) else 0.0) * p[i] - lr * (m[i] / (1 - b1 ** step)) / (np.sqrt(v[i] / (1 - b2 ** step)) + eps)
+        # an update is at most lr; relative errors of the gradients (1e-5 of the largest; bf16 products: 2e-2) pass through it against eps
+        tol = 4 * lr * (1e-3 if matmul == "fp32" else 0.3)
+        for name, want, old in zip(("w1", "b1", "w2", "b2"), p, params):
+            got = tr.parameter(name).reshape(want.shape)
+            assert np.abs(got - want).max() <= tol, name
+            assert np.abs(got - old).max() > lr
+    finally:
+        dev.close()
+
+
+@gpu
+def test_mlp_trainer_with_adamw_in_8_bits_stays_near_32(device):
+    from ormi_b200.train_step import MLPTrainer
+    x, t, *params = mlp()
+    losses = {}
+    for bits in (32, 8):
+        tr = MLPTrainer(device, x, t, *params, lr=0.003, optimizer="adamw", adamw=dict(state_bits=bits, betas=(0.9, 0.99)))
+        for _ in range(10):
+            tr.step()
+        losses[bits] = tr.loss()
+        assert all(np.isfinite(tr.parameter(k)).all() for k in ("w1", "b1", "w2", "b2"))
+    assert abs(losses[8] - losses[32]) < 0.1 * losses[32]
+
+
+def test_mlp_trainer_refuses_unknown_optimizers():
+    from ormi_b200.train_step import MLPTrainer
+    with pytest.raises(ValueError, match="optimizer"):
+        MLPTrainer(NODEV, *mlp(), lr=0.1, optimizer="adam")
+
+
+@gpu
+def test_captured_block_replays_with_new_inputs_and_weights():
+    """A captured forward and backward pass with an AdamW step: replays read the buffers' new contents, update in place, and a bf16
+    copy made of a captured output outside is not used after a replay."""
+    from ormi_b200.runtime import Device
+    dev = Device(0)
+    try:
+        b, n, h, d = 1, 200, 4, 64
+        q, k, v = qkv(b, n, n, h, h, d, BF)
+        out, lse, dout = torch.empty_like(q), torch.empty(b, h, n, device="cuda"), randn(b, n, h, d, dtype=BF, seed=9)
+        grads = [torch.empty_like(q) for _ in range(3)]
+        w = torch.randn(n * h * d, device="cuda")
+        m, s2 = torch.zeros_like(w), torch.zeros_like(w)
+        count = torch.zeros(1, dtype=torch.int64, device="cuda")
+        opt = ops.AdamW(dev, [w], [grads[0].view(-1)], [m], [s2])
+
+        def step():
+            ops.attention(dev, q, k, v, out, lse, causal=True)
+            ops.attention_backward(dev, dout, q, k, v, out, lse, *grads, causal=True)
+            opt.step(lr=0.01, device_step=count)
+        torch.cuda.synchronize()
+        step()
+        dev.sync()
+        with dev.capture() as one:
+            step()
+        step()                                           # the first graph keeps its scratch: a second one needs a plain run of its own
+        dev.sync()
+        with dev.capture() as two:
+            step()
+        q.copy_(randn(b, n, h, d, dtype=BF, seed=77))
+        torch.cuda.synchronize()
+        one.launch()
+        two.launch()
+        dev.sync()
+        assert int(count) == 4
+        ref = Attention(q, k, v, causal=True)
+        want, bound, _, _ = ref.forward()
+        close("out", out, want, bound)
+        for (name, (want, bound)), got in zip(ref.backward(dout, out, lse).items(), grads):
+            close(name, got, want, bound)
+        one.destroy()
+        two.launch()
+        dev.sync()
+        assert int(count) == 5
+        two.destroy()
+    finally:
+        dev.close()
