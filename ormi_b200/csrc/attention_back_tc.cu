@@ -320,25 +320,29 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
 template <int DP, bool CAP, bool BIAS, bool DOCS>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-            const __grid_constant__ CUtensorMap map_do, const __grid_constant__ TcParams p) {
+            const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_o, const __grid_constant__ TcParams p) {
     using Shape = BackShape<DP>;
-    constexpr int ST = Shape::kStages, OP = Shape::kOperand;
+    // K is read twice, by the scores and a whole tile later by dQ; V once: three slots and one (six and two of half the size)
+    constexpr int KS = Shape::kStages * 3 / 2, VS = Shape::kStages / 2, OP = Shape::kOperand;
     extern __shared__ unsigned char raw[];
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     unsigned char* mem = raw + (base - smem_u32(raw));
     const uint32_t q_at = base, do_at = base + OP;
-    auto k_at = [&](int s) { return base + (2 + 2 * s) * OP; };
-    auto v_at = [&](int s) { return base + (3 + 2 * s) * OP; };
-    float* deltas = reinterpret_cast<float*>(mem + (2 + 2 * ST) * OP);           // of the 128 queries
-    int* docs = reinterpret_cast<int*>(deltas + kTile);                          // 64 for each compute warp
+    auto k_at = [&](int s) { return base + (2 + s) * OP; };
+    auto v_at = [&](int s) { return base + (2 + KS + s) * OP; };
+    const uint32_t o_at = k_at(KS - 1);                                          // O's tile, until delta has been computed
+    float* deltas = reinterpret_cast<float*>(mem + (2 + KS + VS) * OP);          // of the 128 queries: two halves
+    int* docs = reinterpret_cast<int*>(deltas + 2 * kTile);                      // 64 for each compute warp
     unsigned short* list = reinterpret_cast<unsigned short*>(docs + 8 * 64);
     const uint32_t bars = smem_u32(list + kMaxTiles);
     const uint32_t q_full = bars, dp_full = bars + 8, ds_ready = bars + 16, done = bars + 24, blank_go = bars + 32, blanked = bars + 40;
     auto s_full = [&](int x) { return bars + 48 + 8 * x; };
     auto s_empty = [&](int x) { return bars + 64 + 8 * x; };
-    auto k_full = [&](int s) { return bars + 80 + 8 * s; };
-    auto v_full = [&](int s) { return bars + 80 + 8 * (ST + s); };
-    auto empty = [&](int s) { return bars + 80 + 8 * (2 * ST + s); };
+    const uint32_t o_full = bars + 80, o_read = bars + 88;
+    auto k_full = [&](int s) { return bars + 96 + 8 * s; };
+    auto k_empty = [&](int s) { return bars + 96 + 8 * (KS + s); };
+    auto v_full = [&](int s) { return bars + 96 + 8 * (2 * KS + s); };
+    auto v_empty = [&](int s) { return bars + 96 + 8 * (2 * KS + VS + s); };
     __shared__ uint32_t tmem_slot;
     __shared__ int list_size;
     __shared__ Abort ab;
@@ -357,7 +361,9 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         ab.flag = 0; ab.err = p.err;
         mbar_init(q_full, 1); mbar_init(dp_full, 1); mbar_init(ds_ready, 8); mbar_init(done, 1); mbar_init(blank_go, 1); mbar_init(blanked, 1);
         for (int x = 0; x < 2; ++x) { mbar_init(s_full(x), 1); mbar_init(s_empty(x), 8); }
-        for (int s = 0; s < ST; ++s) { mbar_init(k_full(s), 1); mbar_init(v_full(s), 1); mbar_init(empty(s), 1); }
+        mbar_init(o_full, 1); mbar_init(o_read, 8);
+        for (int s = 0; s < KS; ++s) { mbar_init(k_full(s), 1); mbar_init(k_empty(s), 1); }
+        for (int s = 0; s < VS; ++s) { mbar_init(v_full(s), 1); mbar_init(v_empty(s), 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -378,30 +384,47 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     } else if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == 0) {
-            if (lane == 0 && total) {
+            if (lane == 0) {
+                // (O is needed even where no key is seen: delta is written for every query)
+                mbar_expect_tx(o_full, OP);
+                for (int x = 0; x < DP / 64; ++x) tma_load_4d(o_at + x * box_bytes(kTile), &map_o, o_full, 64 * x, q0, h, b);
                 mbar_expect_tx(q_full, 2 * OP);
                 for (int x = 0; x < DP / 64; ++x) {
-                    tma_load_4d(q_at + x * box_bytes(kTile), &map_q, q_full, 64 * x, q0, h, b);
                     tma_load_4d(do_at + x * box_bytes(kTile), &map_do, q_full, 64 * x, q0, h, b);
+                    tma_load_4d(q_at + x * box_bytes(kTile), &map_q, q_full, 64 * x, q0, h, b);
                 }
                 bool ok = true;
-                int i = 0;
-                for (; i < total && ok; ++i) {
-                    const int s = i % ST, key0 = tile_of(list[i]) * kTile;
-                    ok = mbar_wait(empty(s), (i / ST & 1) ^ 1, ab, 41);
-                    if (!ok) break;
+                auto load_k = [&](int i) {
+                    const int s = i % KS;
+                    ok = ok && mbar_wait(k_empty(s), (i / KS & 1) ^ 1, ab, 41) && (i != KS - 1 || mbar_wait(o_read, 0, ab, 41));
+                    if (!ok) return;
                     mbar_expect_tx(k_full(s), OP);
-                    for (int x = 0; x < DP / 64; ++x) tma_load_4d(k_at(s) + x * box_bytes(kTile), &map_k, k_full(s), 64 * x, key0, kvh, b);
+                    for (int x = 0; x < DP / 64; ++x) tma_load_4d(k_at(s) + x * box_bytes(kTile), &map_k, k_full(s), 64 * x, tile_of(list[i]) * kTile, kvh, b);
+                };
+                auto load_v = [&](int i) {
+                    const int s = i % VS;
+                    ok = ok && mbar_wait(v_empty(s), (i / VS & 1) ^ 1, ab, 41);
+                    if (!ok) return;
                     mbar_expect_tx(v_full(s), OP);
-                    for (int x = 0; x < DP / 64; ++x) tma_load_4d(v_at(s) + x * box_bytes(kTile), &map_v, v_full(s), 64 * x, key0, kvh, b);
+                    for (int x = 0; x < DP / 64; ++x) tma_load_4d(v_at(s) + x * box_bytes(kTile), &map_v, v_full(s), 64 * x, tile_of(list[i]) * kTile, kvh, b);
+                };
+                // in the order in which the slots come free: V of a tile when the one before has been multiplied, K a tile ahead of it
+                if (total) { load_k(0); load_v(0); }
+                if (total > 1) load_k(1);
+                for (int i = 1; i < total && ok; ++i) {
+                    load_v(i);
+                    if (i + 1 < total) load_k(i + 1);
                 }
-                for (int k = 0; k < ST && ok; ++k, ++i) ok = mbar_wait(empty(i % ST), (i / ST & 1) ^ 1, ab, 41);
+                // nothing of this block's is in flight when it leaves
+                ok = ok && mbar_wait(q_full, 0, ab, 41) && mbar_wait(o_read, 0, ab, 41);
+                for (int k = 0; k < KS; ++k) ok = ok && mbar_wait(k_empty((total + k) % KS), ((total + k) / KS & 1) ^ 1, ab, 41);
+                for (int k = 0; k < VS; ++k) ok = ok && mbar_wait(v_empty((total + k) % VS), ((total + k) / VS & 1) ^ 1, ab, 41);
             }
         } else if (warp == 1) {
             if (total) {
                 bool ok = warp_wait(q_full, 0, ab, 42);
                 auto scores = [&](int i) {
-                    ok = ok && warp_wait(k_full(i % ST), i / ST & 1, ab, 43);
+                    ok = ok && warp_wait(k_full(i % KS), i / KS & 1, ab, 43);
                     if (ok && tile_of(list[i]) == blank_tile) {            // warp 2 blanks the rows behind key_len first
                         if (lane == 0) mbar_arrive(blank_go);
                         ok = warp_wait(blanked, 0, ab, 43);
@@ -410,17 +433,18 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                     if (!ok) return;
                     fence_after();
                     if (elect()) {
-                        product_nt<DP, kTile>(s_at(i & 1), q_at, k_at(i % ST));
+                        product_nt<DP, kTile>(s_at(i & 1), q_at, k_at(i % KS));
                         commit(s_full(i & 1));
                     }
                 };
                 auto gaps = [&](int i) {
-                    ok = ok && warp_wait(v_full(i % ST), i / ST & 1, ab, 45);
+                    ok = ok && warp_wait(v_full(i % VS), i / VS & 1, ab, 45);
                     if (!ok) return;
                     fence_after();
                     if (elect()) {
-                        product_nt<DP, kTile>(dp_at, do_at, v_at(i % ST));
+                        product_nt<DP, kTile>(dp_at, do_at, v_at(i % VS));
                         commit(dp_full);
+                        commit(v_empty(i % VS));
                     }
                 };
                 scores(0);
@@ -431,8 +455,8 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                     if (!ok) break;
                     fence_after();
                     if (elect()) {
-                        product_halves<DP>(dq_at, dp_at, k_at(i % ST), i > 0);
-                        commit(empty(i % ST));
+                        product_halves<DP>(dq_at, dp_at, k_at(i % KS), i > 0);
+                        commit(k_empty(i % KS));
                     }
                     if (i + 1 < total) gaps(i + 1);
                 }
@@ -440,7 +464,7 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
             }
         } else if (warp == 2) {
             if (total && blank_tile >= 0 && tile_of(list[total - 1]) == blank_tile) {
-                const int s = (total - 1) % ST;
+                const int s = (total - 1) % KS;
                 if (warp_wait(blank_go, 0, ab, 47)) {
                     for (int x = 0; x < DP / 64; ++x)
                         for (int i = m.keys % kTile * 8 + lane; i < kTile * 8; i += 32)
@@ -453,35 +477,7 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        // delta of the block's queries: DP / 8 lanes per row, 16 bytes each
-        constexpr int LPR = DP / 8, RPW = 32 / LPR, TURNS = kTile / (8 * RPW);
         const int64_t lines = ((int64_t)b * p.a.heads + h) * p.a.q_len;
-        const int d = lane % LPR * 8;
-        uint4 xs[TURNS], ys[TURNS];                               // everything is asked for first
-#pragma unroll
-        for (int k = 0; k < TURNS; ++k) {
-            const int t = q0 + (k * 8 + warp - 4) * RPW + lane / LPR;
-            xs[k] = ys[k] = make_uint4(0, 0, 0, 0);
-            if (t < p.a.q_len && d < p.a.dim) {
-                xs[k] = *reinterpret_cast<const uint4*>((const bf16*)p.a.out + (int64_t)b * p.a.os.b + (int64_t)t * p.a.os.t + (int64_t)h * p.a.os.h + d);
-                ys[k] = *reinterpret_cast<const uint4*>((const bf16*)p.a.dout + (int64_t)b * p.a.dos.b + (int64_t)t * p.a.dos.t + (int64_t)h * p.a.dos.h + d);
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < TURNS; ++k) {
-            const int r = (k * 8 + warp - 4) * RPW + lane / LPR, t = q0 + r;
-            const uint32_t x[4] = {xs[k].x, xs[k].y, xs[k].z, xs[k].w}, y[4] = {ys[k].x, ys[k].y, ys[k].z, ys[k].w};
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum = fmaf(bf16_hi(x[e]), bf16_hi(y[e]), fmaf(bf16_lo(x[e]), bf16_lo(y[e]), sum));
-#pragma unroll
-            for (int o = LPR / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (d == 0) {
-                deltas[r] = sum;
-                if (t < p.a.q_len) p.a.delta[lines + t] = sum;
-            }
-        }
-        asm volatile("bar.sync 1, 256;" ::: "memory");           // the eight compute warps; nothing before it can give up
         const int w = warp / 4 - 1, t = q0 + (threadIdx.x & 127);
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         const bool live = t < p.a.q_len;
@@ -490,10 +486,30 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         const float slope = BIAS ? p.a.slopes[h] * kLog2e : 0.f;
         float lse2 = live ? p.a.lse[lines + t] * kLog2e : INFINITY;
         if (lse2 == -INFINITY) lse2 = INFINITY;
-        const float delta = deltas[threadIdx.x & 127];
+        // delta of the block's queries: a row per thread, half of the columns for each warpgroup, from the swizzled tiles
+        bool ok = warp_wait(q_full, 0, ab, 47) && warp_wait(o_full, 0, ab, 47);
+        float half = 0.f;
+        if (ok) {
+            const int row = threadIdx.x & 127;
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                const int c = w * (DP / 16) + k;                  // 16-byte chunk of the row
+                const uint32_t at = (c >> 3) * box_bytes(kTile) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+                uint32_t x[4], y[4];
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(o_at + at) : "memory");
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3]) : "r"(do_at + at) : "memory");
+#pragma unroll
+                for (int e = 0; e < 4; ++e) half = fmaf(bf16_hi(x[e]), bf16_hi(y[e]), fmaf(bf16_lo(x[e]), bf16_lo(y[e]), half));
+            }
+        }
+        deltas[w * kTile + (threadIdx.x & 127)] = half;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(o_read);                      // the third slot is free for keys
+        asm volatile("bar.sync 1, 256;" ::: "memory");           // the eight compute warps; all of them come here
+        const float delta = deltas[threadIdx.x & 127] + deltas[kTile + (threadIdx.x & 127)];
+        if (w == 0 && live) p.a.delta[lines + t] = delta;
         int* my_docs = docs + (warp - 4) * 64;
-        bool ok = true;
-        for (int i = 0; i < total; ++i) {
+        for (int i = 0; i < total && ok; ++i) {
             const int entry = list[i], key0 = tile_of(entry) * kTile + 64 * w;
             const int cls = entry >> 14;
             if (DOCS && cls == kDocs) {
@@ -588,7 +604,7 @@ void launch_backward(ormi_b200_ctx* ctx, const CUtensorMap* maps, const TcParams
     auto q = attn_back_q<DP, CAP, BIAS, DOCS>;
     ORMI_CUDA(cudaFuncSetAttribute(kv, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     ORMI_CUDA(cudaFuncSetAttribute(q, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    q<<<dim3(p.a.batch * p.a.heads, (p.a.q_len + kTile - 1) / kTile), kThreads, smem, ctx->stream>>>(maps[0], maps[1], maps[2], maps[3], p);
+    q<<<dim3(p.a.batch * p.a.heads, (p.a.q_len + kTile - 1) / kTile), kThreads, smem, ctx->stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], p);
     kv<<<dim3(p.a.batch * p.a.kv_heads, (p.a.k_len + kTile - 1) / kTile), kThreads, smem, ctx->stream>>>(maps[0], maps[1], maps[2], maps[3], p);
     ORMI_CUDA(cudaGetLastError());
     count_launch(ctx, 2);
@@ -616,11 +632,12 @@ bool attention_backward_tc_supported(const AttnParams& p, int dtype) {
 void attention_backward_tc(ormi_b200_ctx* ctx, AttnParams& a) {
     Scratch bounds(ctx, bounds_bytes(a));
     const TcParams p = tc_params(ctx, a, (int2*)bounds.ptr);
-    CUtensorMap maps[4];
+    CUtensorMap maps[5];
     head_map(ctx, &maps[0], a.q, a.qs, a.batch, a.q_len, a.heads, a.dim);
     head_map(ctx, &maps[1], a.k, a.ks, a.batch, a.k_len, a.kv_heads, a.dim);
     head_map(ctx, &maps[2], a.v, a.vs, a.batch, a.k_len, a.kv_heads, a.dim);
     head_map(ctx, &maps[3], a.dout, a.dos, a.batch, a.q_len, a.heads, a.dim);
+    head_map(ctx, &maps[4], a.out, a.os, a.batch, a.q_len, a.heads, a.dim);
     if (a.dim <= 64) launch_by_mask<64>(ctx, maps, p); else launch_by_mask<128>(ctx, maps, p);
     bounds.release();
 }
