@@ -6,6 +6,8 @@
 //   attn_back_kv   a block owns 128 keys of one key/value head and walks the tiles of 128 queries, over all query heads that
 //                  share the head.  Scores are computed transposed (rows = keys), so that probabilities and score
 //                  gradients, rounded to bf16 in tensor memory, are the A operands of dV += P^T dO and dK += dS^T Q directly.
+//                  Blocks of a cluster share the heads and add their dK and dV up through each other's shared memory, in a
+//                  fixed order: with four heads in one block the longest block took most of the launch.
 // The price is that both compute the scores (7 products instead of 5).  Warp 0 loads, warp 1 issues the products, warp 2
 // fetches the queries' statistics (or blanks the keys behind key_len), and two warpgroups do the arithmetic, each half of the
 // columns of a tile: while they work on the gradients of a tile the tensor cores multiply its probabilities and compute
@@ -93,10 +95,12 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     __shared__ Abort ab;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int b = blockIdx.x / p.a.kv_heads, kvh = blockIdx.x % p.a.kv_heads;
+    const int rank = blockIdx.x % p.cluster, head_group = blockIdx.x / p.cluster;
+    const int b = head_group / p.a.kv_heads, kvh = head_group % p.a.kv_heads;
+    const int heads = p.a.group / p.cluster, first_head = kvh * p.a.group + rank * heads;      // this block's query heads
     const int key0 = blockIdx.y * kTile;                                   // causal: the first keys are seen by most queries
     const RowMask m = row_mask(p.a, b);
-    if (warp == 0) {
+    if (warp == 2) {
         const int n = key0 >= m.keys ? 0 : list_tiles(list, (p.a.q_len + kTile - 1) / kTile, [&](int t) {
             const int first = t * kTile, last = min(first + kTile, p.a.q_len) - 1;
             return tile_class<2, 2>(p, b, 2 * t, key_end(m, m.start + first), key_end(m, m.start + last), key0 / kUnit);
@@ -110,6 +114,12 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         for (int s = 0; s < ST; ++s) { mbar_init(q_full(s), 1); mbar_init(do_full(s), 1); mbar_init(empty(s), 1); mbar_init(stat_full(s), 1); mbar_init(stat_empty(s), 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        // the resident operands do not depend on the list: they are on their way while it is being made
+        mbar_expect_tx(kv_full, 2 * OP);
+        for (int x = 0; x < DP / 64; ++x) {
+            tma_load_4d(k_at + x * box_bytes(kTile), &map_k, kv_full, 64 * x, key0, kvh, b);
+            tma_load_4d(v_at + x * box_bytes(kTile), &map_v, kv_full, 64 * x, key0, kvh, b);
+        }
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
@@ -122,22 +132,17 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     constexpr uint32_t tmem = 0, s_at = tmem, dp_at = tmem + 128, dv_at = tmem + 256, dk_at = tmem + 384;
     const bool whole = tmem_slot == tmem;
     if (!whole && threadIdx.x == 0) atomicCAS(p.err, 0, 20);
-    const int per_head = list_size, total = per_head * p.a.group;
+    const int per_head = list_size, total = per_head * heads;
 
     if (!whole) {
     } else if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == 0) {
-            if (lane == 0 && total) {
-                mbar_expect_tx(kv_full, 2 * OP);
-                for (int x = 0; x < DP / 64; ++x) {
-                    tma_load_4d(k_at + x * box_bytes(kTile), &map_k, kv_full, 64 * x, key0, kvh, b);
-                    tma_load_4d(v_at + x * box_bytes(kTile), &map_v, kv_full, 64 * x, key0, kvh, b);
-                }
+            if (lane == 0) {
                 bool ok = true;
                 int i = 0;
                 for (; i < total && ok; ++i) {
-                    const int s = i % ST, h = kvh * p.a.group + i / per_head, q0 = tile_of(list[i % per_head]) * kTile;
+                    const int s = i % ST, h = first_head + i / per_head, q0 = tile_of(list[i % per_head]) * kTile;
                     ok = mbar_wait(empty(s), (i / ST & 1) ^ 1, ab, 31);
                     if (!ok) break;
                     mbar_expect_tx(q_full(s), OP);
@@ -145,6 +150,7 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                     mbar_expect_tx(do_full(s), OP);
                     for (int x = 0; x < DP / 64; ++x) tma_load_4d(do_at(s) + x * box_bytes(kTile), &map_do, do_full(s), 64 * x, q0, h, b);
                 }
+                ok = ok && mbar_wait(kv_full, 0, ab, 31);             // nothing of this block's is in flight when it leaves
                 for (int k = 0; k < ST && ok; ++k, ++i) ok = mbar_wait(empty(i % ST), (i / ST & 1) ^ 1, ab, 31);
             }
         } else if (warp == 1) {
@@ -191,7 +197,7 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         } else if (warp == 2) {
             // the queries' statistics; a row that sees nothing, or does not exist, gets an infinite one: its probabilities vanish
             for (int i = 0; i < total; ++i) {
-                const int s = i % ST, h = kvh * p.a.group + i / per_head, q0 = tile_of(list[i % per_head]) * kTile;
+                const int s = i % ST, h = first_head + i / per_head, q0 = tile_of(list[i % per_head]) * kTile;
                 float l[4], d[4];
                 int e[4], doc[4];
     #pragma unroll
@@ -227,7 +233,7 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             const int s = i % ST, entry = list[i % per_head], q0 = tile_of(entry) * kTile;
             const int cls = entry >> 14;
             const Stat& st = stats[s];
-            const float slope = BIAS ? p.a.slopes[kvh * p.a.group + i / per_head] * kLog2e : 0.f;
+            const float slope = BIAS ? p.a.slopes[first_head + i / per_head] * kLog2e : 0.f;
             const float ahead = (float)(m.start + q0 + 64 * w - key);
             ok = warp_wait(stat_full(s), i / ST & 1, ab, 38) && warp_wait(s_full, i & 1, ab, 38);
             if (!ok) break;
@@ -236,24 +242,37 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             ld32(s_at + lanes + 64 * w, reinterpret_cast<uint32_t*>(z));
             ld32(s_at + lanes + 64 * w + 32, reinterpret_cast<uint32_t*>(z) + 32);
             wait_ld();
-            if (CAP) cap_scores<32, true>(p, z, g);
-            if (BIAS) {
-#pragma unroll
-                for (int c = 0; c < 32; ++c) {
+            // the capped score, its slope and the exponential of two columns: the polynomial runs on the FMA pipe while the
+            // special function unit is busy with the exponentials before it
+            auto expo = [&](int c, const float2& neg_lse2) {
+                if (CAP) g[c] = cap_slope(p, z[c]);
+                if (BIAS) {
                     if (!CAP) z[c] = mul2(z[c], both(p.scale_log2));
                     z[c] = make_float2(fmaf(-slope, fabsf(ahead + (float)(2 * c)), z[c].x), fmaf(-slope, fabsf(ahead + (float)(2 * c + 1)), z[c].y));
+                }
+                z[c] = CAP || BIAS ? add2(z[c], neg_lse2) : fma2(z[c], both(p.scale_log2), neg_lse2);
+                z[c] = make_float2(ex2(z[c].x), ex2(z[c].y));
+            };
+            if (!CAP || cap_is_polynomial<32>(p, z)) {
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                    const float4 l = *reinterpret_cast<const float4*>(&st.lse2[64 * w + 2 * c]);
+                    if (CAP) { z[c] = cap_polynomial(p, z[c]); z[c + 1] = cap_polynomial(p, z[c + 1]); }
+                    expo(c, make_float2(l.x, l.y));
+                    expo(c + 1, make_float2(l.z, l.w));
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                    const float4 l = *reinterpret_cast<const float4*>(&st.lse2[64 * w + 2 * c]);
+                    z[c] = cap_any(p, z[c]); z[c + 1] = cap_any(p, z[c + 1]);
+                    expo(c, make_float2(l.x, l.y));
+                    expo(c + 1, make_float2(l.z, l.w));
                 }
             }
             uint32_t pk[32];
 #pragma unroll
             for (int c = 0; c < 32; c += 2) {
-                const float4 l = *reinterpret_cast<const float4*>(&st.lse2[64 * w + 2 * c]);
-                float2 a[2] = {make_float2(l.x, l.y), make_float2(l.z, l.w)};
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    a[k] = CAP || BIAS ? add2(z[c + k], a[k]) : fma2(z[c + k], both(p.scale_log2), a[k]);
-                    z[c + k] = make_float2(ex2(a[k].x), ex2(a[k].y));
-                }
                 if (cls >= kPartial) {
                     const int4 e = *reinterpret_cast<const int4*>(&st.end[64 * w + 2 * c]);
                     int4 d = make_int4(my_doc, my_doc, my_doc, my_doc);
@@ -300,19 +319,62 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         }
         if (ok && total) ok = warp_wait(done, 0, ab, 40);
         if (ok) {
-            // warpgroup 0 writes dV, warpgroup 1 dK; keys that nobody sees get zero
+            // warpgroup 0 takes dV out of tensor memory, warpgroup 1 dK; keys that nobody sees get zero
             fence_after();
+            const int first = key0 + (warp & 3) * 32, row = threadIdx.x & 127;
             const Strides4& os = w ? p.a.dks : p.a.dvs;
-            const int first = key0 + (warp & 3) * 32;
             bf16* out = (bf16*)(w ? p.a.dk : p.a.dv) + (int64_t)b * os.b + (int64_t)first * os.t + (int64_t)kvh * os.h;
+            if (p.cluster == 1) {
+                store_rows<DP>((w ? dk_at : dv_at) + lanes, total > 0, base + (warp - 4) * (64 * DP), w ? p.a.scale : 1.f, p.a.k_len - first, p.a.dim, [&](int r) { return out + r * os.t; });
+            } else {
+                // into the idle operand buffers, for the cluster: rows of fp32, their 16-byte chunks c at c ^ row
+                const uint32_t to = base + w * (kTile * DP * 4) + row * (DP * 4);
 #pragma unroll 1
-            for (int x = 0; x < DP; x += 32) {
-                uint32_t o[32];
-                if (total) { ld32((w ? dk_at : dv_at) + lanes + x, o); wait_ld(); }
-                else for (int i = 0; i < 32; ++i) o[i] = 0;
-                store_block32(k_at + (warp - 4) * 2048, o, w ? p.a.scale : 1.f, p.a.k_len - first, p.a.dim - x, [&](int r) { return out + r * os.t + x; });
+                for (int x = 0; x < DP; x += 32) {
+                    uint32_t o[32];
+                    if (total) { ld32((w ? dk_at : dv_at) + lanes + x, o); wait_ld(); }
+                    else for (int i = 0; i < 32; ++i) o[i] = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + (((x / 4 + i) ^ (row & (DP / 4 - 1))) << 4)), "r"(o[4 * i]), "r"(o[4 * i + 1]), "r"(o[4 * i + 2]), "r"(o[4 * i + 3]) : "memory");
+                }
             }
         }
+    }
+    __syncwarp();
+    if (p.cluster > 1) {
+        auto meet = [&] {
+            asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+            asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+        };
+        meet();
+        if (whole && !ab.flag) {
+            // rows rank, rank + cluster, ... of both: the sum over the cluster's blocks in their order.  A lane holds four columns.
+            constexpr int LPR = DP / 4, RPW = 32 / LPR;
+            const int mine = kTile / p.cluster, c = lane % LPR;
+            const float by_k = p.a.scale;
+#pragma unroll 2
+            for (int i = warp * RPW + lane / LPR; i < 2 * mine; i += kThreads / 32 * RPW) {
+                const int which = i >= mine, row = (i - which * mine) * p.cluster + rank, key = key0 + row;
+                const uint32_t at = base + which * (kTile * DP * 4) + row * (DP * 4) + ((c ^ (row & (DP / 4 - 1))) << 4);
+                float4 v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (r >= p.cluster) continue;
+                    uint32_t peer;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(r));
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[r].x), "=f"(v[r].y), "=f"(v[r].z), "=f"(v[r].w) : "r"(peer));
+                }
+                if (key >= p.a.k_len || 4 * c >= p.a.dim) continue;
+                const Strides4& os = which ? p.a.dks : p.a.dvs;
+                const float by = which ? by_k : 1.f;
+                bf16* out = (bf16*)(which ? p.a.dk : p.a.dv) + (int64_t)b * os.b + (int64_t)key * os.t + (int64_t)kvh * os.h + 4 * c;
+                *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2((((v[0].x + v[1].x) + v[2].x) + v[3].x) * by, (((v[0].y + v[1].y) + v[2].y) + v[3].y) * by),
+                                                            pack_bf16x2((((v[0].z + v[1].z) + v[2].z) + v[3].z) * by, (((v[0].w + v[1].w) + v[2].w) + v[3].w) * by));
+            }
+        }
+        meet();                                                // nobody leaves while another reads its memory
     }
     leave(ab, warp, tmem_slot);
 }
@@ -352,7 +414,7 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     const int q0 = (int)(gridDim.y - 1 - blockIdx.y) * kTile;
     const RowMask m = row_mask(p.a, b);
     const int blank_tile = m.keys < p.a.k_len && m.keys % kTile ? m.keys / kTile : -1;
-    if (warp == 0) {
+    if (warp == 2) {
         const int lo = key_end(m, m.start + q0), hi = key_end(m, m.start + min(q0 + kTile, p.a.q_len) - 1);
         const int n = list_tiles(list, (max(hi, 0) + kTile - 1) / kTile, [&](int j) { return tile_class<2, 2>(p, b, q0 / kUnit, lo, hi, 2 * j); });
         if (lane == 0) list_size = n;
@@ -366,6 +428,14 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         for (int s = 0; s < VS; ++s) { mbar_init(v_full(s), 1); mbar_init(v_empty(s), 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        // (O is needed even where no key is seen: delta is written for every query)
+        mbar_expect_tx(o_full, OP);
+        for (int x = 0; x < DP / 64; ++x) tma_load_4d(o_at + x * box_bytes(kTile), &map_o, o_full, 64 * x, q0, h, b);
+        mbar_expect_tx(q_full, 2 * OP);
+        for (int x = 0; x < DP / 64; ++x) {
+            tma_load_4d(do_at + x * box_bytes(kTile), &map_do, q_full, 64 * x, q0, h, b);
+            tma_load_4d(q_at + x * box_bytes(kTile), &map_q, q_full, 64 * x, q0, h, b);
+        }
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
@@ -385,14 +455,6 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == 0) {
             if (lane == 0) {
-                // (O is needed even where no key is seen: delta is written for every query)
-                mbar_expect_tx(o_full, OP);
-                for (int x = 0; x < DP / 64; ++x) tma_load_4d(o_at + x * box_bytes(kTile), &map_o, o_full, 64 * x, q0, h, b);
-                mbar_expect_tx(q_full, 2 * OP);
-                for (int x = 0; x < DP / 64; ++x) {
-                    tma_load_4d(do_at + x * box_bytes(kTile), &map_do, q_full, 64 * x, q0, h, b);
-                    tma_load_4d(q_at + x * box_bytes(kTile), &map_q, q_full, 64 * x, q0, h, b);
-                }
                 bool ok = true;
                 auto load_k = [&](int i) {
                     const int s = i % KS;
@@ -529,9 +591,8 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
             if (lane == 0) mbar_arrive(s_empty(i & 1));
             const float ahead = (float)(pos - key0);
             const int left = end - key0;
-            if (CAP) cap_scores<32, true>(p, z, g);
-#pragma unroll
-            for (int c = 0; c < 32; ++c) {
+            auto expo = [&](int c) {                                  // as in attn_back_kv
+                if (CAP) g[c] = cap_slope(p, z[c]);
                 if (BIAS) {
                     if (!CAP) z[c] = mul2(z[c], both(p.scale_log2));
                     z[c] = make_float2(fmaf(-slope, fabsf(ahead - (float)(2 * c)), z[c].x), fmaf(-slope, fabsf(ahead - (float)(2 * c + 1)), z[c].y));
@@ -539,6 +600,13 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                 z[c] = CAP || BIAS ? add2(z[c], both(-lse2)) : fma2(z[c], both(p.scale_log2), both(-lse2));
                 z[c] = make_float2(ex2(z[c].x), ex2(z[c].y));
                 g[c] = CAP ? mul2(g[c], z[c]) : z[c];
+            };
+            if (!CAP || cap_is_polynomial<32>(p, z)) {
+#pragma unroll
+                for (int c = 0; c < 32; ++c) { if (CAP) z[c] = cap_polynomial(p, z[c]); expo(c); }
+            } else {
+#pragma unroll
+                for (int c = 0; c < 32; ++c) { z[c] = cap_any(p, z[c]); expo(c); }
             }
             if (DOCS && cls == kDocs) {
 #pragma unroll
@@ -585,13 +653,8 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
             fence_after();
             const int first = q0 + (warp & 3) * 32;
             bf16* out = (bf16*)p.a.dq + (int64_t)b * p.a.dqs.b + (int64_t)first * p.a.dqs.t + (int64_t)h * p.a.dqs.h;
-#pragma unroll 1
-            for (int x = w * (DP / 2); x < (w + 1) * (DP / 2); x += 32) {          // a half of the columns each
-                uint32_t o[32];
-                if (total) { ld32(dq_at + lanes + x, o); wait_ld(); }
-                else for (int i = 0; i < 32; ++i) o[i] = 0;
-                store_block32(q_at + (warp - 4) * 2048, o, p.a.scale, p.a.q_len - first, p.a.dim - x, [&](int r) { return out + r * p.a.dqs.t + x; });
-            }
+            const int x = w * (DP / 2);                                            // a half of the columns each
+            store_rows<DP / 2>(dq_at + lanes + x, total > 0, q_at + (warp - 4) * (32 * DP), p.a.scale, p.a.q_len - first, p.a.dim - x, [&](int r) { return out + r * p.a.dqs.t + x; });
         }
     }
     leave(ab, warp, tmem_slot);
@@ -605,7 +668,17 @@ void launch_backward(ormi_b200_ctx* ctx, const CUtensorMap* maps, const TcParams
     ORMI_CUDA(cudaFuncSetAttribute(kv, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     ORMI_CUDA(cudaFuncSetAttribute(q, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     q<<<dim3(p.a.batch * p.a.heads, (p.a.q_len + kTile - 1) / kTile), kThreads, smem, ctx->stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], p);
-    kv<<<dim3(p.a.batch * p.a.kv_heads, (p.a.k_len + kTile - 1) / kTile), kThreads, smem, ctx->stream>>>(maps[0], maps[1], maps[2], maps[3], p);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(p.a.batch * p.a.kv_heads * p.cluster, (p.a.k_len + kTile - 1) / kTile);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = smem;
+    config.stream = ctx->stream;
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = p.cluster; cluster.val.clusterDim.y = 1; cluster.val.clusterDim.z = 1;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    ORMI_CUDA(cudaLaunchKernelEx(&config, kv, maps[0], maps[1], maps[2], maps[3], p));
     ORMI_CUDA(cudaGetLastError());
     count_launch(ctx, 2);
 }
@@ -631,7 +704,13 @@ bool attention_backward_tc_supported(const AttnParams& p, int dtype) {
 
 void attention_backward_tc(ormi_b200_ctx* ctx, AttnParams& a) {
     Scratch bounds(ctx, bounds_bytes(a));
-    const TcParams p = tc_params(ctx, a, (int2*)bounds.ptr);
+    TcParams p = tc_params(ctx, a, (int2*)bounds.ptr);
+    // A block alone keeps its set-up (loads, tensor memory, first products: 5 us) for more tiles; a cluster spreads the work
+    // of a key/value head where blocks would leave SMs idle, and evens out the uneven lists that documents make (packed
+    // documents, 2 x 4096 tokens, 16 heads over 4: 279 us alone, 260 us in twos, 304 us in fours; without documents 431, 446
+    // and 513 us).
+    const int64_t blocks = (int64_t)a.batch * a.kv_heads * ((a.k_len + kTile - 1) / kTile);
+    p.cluster = a.group % 4 == 0 && blocks * 4 <= ctx->num_sms ? 4 : a.group % 2 == 0 && (blocks * 2 <= ctx->num_sms || a.k_docs) ? 2 : 1;
     CUtensorMap maps[5];
     head_map(ctx, &maps[0], a.q, a.qs, a.batch, a.q_len, a.heads, a.dim);
     head_map(ctx, &maps[1], a.k, a.ks, a.batch, a.k_len, a.kv_heads, a.dim);

@@ -60,12 +60,6 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         hi[w] = first < p.a.q_len ? key_end(m, m.start + last) : 0;
     }
     const int tiles = (max(max(hi[0], hi[1]), 0) + kTile - 1) / kTile;
-    // classes of the tiles, and which union tile holds the last valid key in its middle
-    for (int j = threadIdx.x; j < tiles; j += kThreads) {
-        int c = 0;
-        for (int w = 0; w < 2; ++w) c |= tile_class<2, 2>(p, b, q0 / kUnit + 2 * w, lo[w], hi[w], 2 * j) << (2 * w);
-        cls[j] = (unsigned char)c;
-    }
     const int blank_tile = m.keys < p.a.k_len && m.keys % kTile ? m.keys / kTile : -1;
     if (threadIdx.x == 0) {
         ab.flag = 0; ab.err = p.err;
@@ -74,10 +68,20 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         for (int s = 0; s < ST; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        // Q does not depend on the classes: it is on its way while they are being worked out
+        mbar_expect_tx(q_full, 2 * OP);
+        for (int w = 0; w < 2; ++w)
+            for (int x = 0; x < DP / 64; ++x) tma_load_4d(q_at + w * OP + x * box_bytes(kTile), &map_q, q_full, 64 * x, q0 + w * kTile, h, b);
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // classes of the tiles, and which union tile holds the last valid key in its middle
+    for (int j = threadIdx.x; j < tiles; j += kThreads) {
+        int c = 0;
+        for (int w = 0; w < 2; ++w) c |= tile_class<2, 2>(p, b, q0 / kUnit + 2 * w, lo[w], hi[w], 2 * j) << (2 * w);
+        cls[j] = (unsigned char)c;
     }
     fence_before();
     __syncthreads();
@@ -94,9 +98,6 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == 0 && lane == 0) {
             // ---------------------------------------------------------------- loads
-            mbar_expect_tx(q_full, 2 * OP);
-            for (int w = 0; w < 2; ++w)
-                for (int x = 0; x < DP / 64; ++x) tma_load_4d(q_at + w * OP + x * box_bytes(kTile), &map_q, q_full, 64 * x, q0 + w * kTile, h, b);
             int seq = 0;
             bool ok = true;
             for (int j = 0; j < tiles && ok; ++j) {
@@ -209,7 +210,15 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             // With neither cap nor bias the raw products go through max and exponential as they are, the scale (positive)
             // riding on the subtraction of the maximum.
             constexpr bool PLAIN = !CAP && !BIAS;
-            if (CAP) cap_scores<64, false>(p, z, nullptr);
+            if (CAP) {
+                if (cap_is_polynomial<64>(p, z)) {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) z[i] = cap_polynomial(p, z[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) z[i] = cap_any(p, z[i]);
+                }
+            }
             if (BIAS) {
                 const float ahead = (float)(pos - key0);
                 if (__all_sync(0xffffffffu, pos - key0 >= kTile - 1)) {          // every key at or before the query: the distance is linear
@@ -294,13 +303,7 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             // the rings are idle now: their memory stages the rows
             const int t0 = q0 + w * kTile + (warp & 3) * 32;
             bf16* out = (bf16*)p.a.out + (int64_t)b * p.a.os.b + (int64_t)t0 * p.a.os.t + (int64_t)h * p.a.os.h;
-#pragma unroll 1
-            for (int x = 0; x < DP; x += 32) {
-                uint32_t o[32];
-                if (n) { ld32(o_at(w) + lanes + x, o); wait_ld(); }
-                else for (int i = 0; i < 32; ++i) o[i] = 0;
-                store_block32(ring + (warp - 4) * 2048, o, by, p.a.q_len - t0, p.a.dim - x, [&](int r) { return out + r * p.a.os.t + x; });
-            }
+            store_rows<DP>(o_at(w) + lanes, n > 0, ring + (warp - 4) * (64 * DP), by, p.a.q_len - t0, p.a.dim, [&](int r) { return out + r * p.a.os.t; });
             if (live && p.a.lse) p.a.lse[((int64_t)b * p.a.heads + h) * p.a.q_len + t] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
         }
     }
@@ -391,11 +394,9 @@ TcParams tc_params(ormi_b200_ctx* ctx, const AttnParams& a, int2* bounds) {
     p.cap_log2 = a.cap * kLog2e;
     if (a.cap > 0.f) {
         const double k = (double)a.scale / a.cap, c = (double)a.scale * 1.4426950408889634;
-        static const double p3[3] = {0.9999996059266845, -0.33321928380355686, 0.12841935404930116}, p5[5] = {0.9999999870693153, -0.3333307189419646, 0.13324828997681853, -0.052989241174570344, 0.017141319046484527};
-        for (int i = 0; i < 3; ++i) p.poly3[i] = (float)(c * p3[i] * std::pow(k, 2 * i));
-        for (int i = 0; i < 5; ++i) p.poly5[i] = (float)(c * p5[i] * std::pow(k, 2 * i));
-        p.limit3 = (float)std::min(0.25 / k, 1e15);               // (a square that overflows has no business here)
-        p.limit5 = (float)std::min(0.5 / k, 1e15);
+        static const double terms[4] = {0.9999999028730692, -0.333313732975708, 0.1327115660233386, -0.04756107721454571};
+        for (int i = 0; i < 4; ++i) p.poly[i] = (float)(c * terms[i] * std::pow(k, 2 * i));
+        p.poly_limit = (float)std::min(0.4 / k, 1e9);             // (a power that overflows has no business here)
         p.exp_per_raw = (float)(2 * 1.4426950408889634 * k);
         p.minus_inv_cap2 = -1.f / (p.cap_log2 * p.cap_log2);
     }

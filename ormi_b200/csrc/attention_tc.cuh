@@ -15,8 +15,9 @@ struct TcParams {
     const int2 *q_bounds, *k_bounds;             // smallest and largest document of every unit, [batch][units]; NULL without documents
     int q_units, k_units;                        // even
     float scale_log2, cap_log2;                  // scale * log2(e), cap * log2(e)
-    // with a cap: 2 log2(e) scale / cap, -1 / cap_log2^2, the polynomials and the largest |raw| for them
-    float exp_per_raw, minus_inv_cap2, poly3[3], limit3, poly5[5], limit5;
+    // with a cap: 2 log2(e) scale / cap, -1 / cap_log2^2, the polynomial and the largest |raw| for it
+    float exp_per_raw, minus_inv_cap2, poly[4], poly_limit;
+    int cluster;                                 // backward pass: blocks that share the query heads of a key/value head
     int* err;
 };
 
@@ -37,69 +38,62 @@ __device__ __forceinline__ int tile_class(const TcParams& p, int b, int q_unit, 
     return k.x == k.y && q.x == q.y ? c : kDocs;
 }
 
-// Raw products to base-2 scores under a cap, in place: z = cap tanh(x), x = raw * scale / cap; `dcap`, when given, receives
-// 1 - tanh(x)^2.  Scores are a few units wide and caps tens of units, so |x| is small: tanh(x) / x is a polynomial in x^2
-// there (Chebyshev fits: three terms for |x| <= 1/4, relative error 4e-7; five for |x| <= 1/2, 1e-8), its coefficients
-// scaled on the host so that it takes raw^2 and gives z / raw.  A warp whose products leave that range takes
-// tanh(x) = 1 - 2 / (e^2x + 1): two operations of the special function unit, off by a few 1e-7 of the cap.
-template <int N, bool SLOPE>
-__device__ __forceinline__ void cap_scores(const TcParams& p, float2 (&z)[N], float2* dcap) {
+// Raw products to base-2 scores under a cap: z = cap tanh(x), x = raw * scale / cap; the derivative 1 - tanh(x)^2 follows from
+// z.  Scores are a few units wide and caps tens of units, so |x| is small: up to 0.4, tanh(x) / x is a polynomial of four
+// terms in x^2 (Chebyshev fit, relative error 1e-7), its coefficients scaled on the host so that it takes raw^2 and gives
+// z / raw.  A warp whose products leave that range takes tanh(x) = 1 - 2 / (e^2x + 1): two operations of the special
+// function unit, off by a few 1e-7 of the cap.
+template <int N>
+__device__ __forceinline__ bool cap_is_polynomial(const TcParams& p, const float2 (&z)[N]) {
     float big = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) big = tc::max3(big, fabsf(z[i].x), fabsf(z[i].y));
-    if (__all_sync(0xffffffffu, big <= p.limit3)) {
+    return __all_sync(0xffffffffu, big <= p.poly_limit);
+}
+__device__ __forceinline__ float2 cap_polynomial(const TcParams& p, const float2& raw) {
+    const float2 u = tc::mul2(raw, raw);
+    float2 t = tc::fma2(u, tc::both(p.poly[3]), tc::both(p.poly[2]));
+    t = tc::fma2(u, t, tc::both(p.poly[1]));
+    return tc::mul2(raw, tc::fma2(u, t, tc::both(p.poly[0])));
+}
+__device__ __forceinline__ float2 cap_any(const TcParams& p, const float2& raw) {
+    return make_float2(fmaf(-2.f * p.cap_log2, __fdividef(1.f, tc::ex2(raw.x * p.exp_per_raw) + 1.f), p.cap_log2),
+                       fmaf(-2.f * p.cap_log2, __fdividef(1.f, tc::ex2(raw.y * p.exp_per_raw) + 1.f), p.cap_log2));
+}
+__device__ __forceinline__ float2 cap_slope(const TcParams& p, const float2& z) { return tc::fma2(tc::mul2(z, z), tc::both(p.minus_inv_cap2), tc::both(1.f)); }
+
+// A warp's 32 rows x COLS columns of fp32 accumulators in tensor memory (a row per lane) as bf16 to global memory, times `by`:
+// through a staging buffer of the warp (32 x COLS x 2 bytes), so that neighbouring lanes write a whole row and not each lane
+// 16 bytes of its own.  have: false gives zeros.  row_ptr(r): where row r goes; columns from `cols` on and rows from `rows`
+// on are left out.
+template <int COLS, typename F>
+__device__ __forceinline__ void store_rows(uint32_t taddr, bool have, uint32_t stage, float by, int rows, int cols, F&& row_ptr) {
+    constexpr int LPR = COLS / 8, MASK = LPR < 8 ? LPR - 1 : 7;
+    const int lane = threadIdx.x & 31;
+    uint32_t o[COLS];
+    if (have) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float2 u = tc::mul2(z[i], z[i]);
-            z[i] = tc::mul2(z[i], tc::fma2(u, tc::fma2(u, tc::both(p.poly3[2]), tc::both(p.poly3[1])), tc::both(p.poly3[0])));
-        }
-    } else if (__all_sync(0xffffffffu, big <= p.limit5)) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float2 u = tc::mul2(z[i], z[i]);
-            float2 t = tc::fma2(u, tc::both(p.poly5[4]), tc::both(p.poly5[3]));
-            t = tc::fma2(u, t, tc::both(p.poly5[2]));
-            t = tc::fma2(u, t, tc::both(p.poly5[1]));
-            z[i] = tc::mul2(z[i], tc::fma2(u, t, tc::both(p.poly5[0])));
-        }
+        for (int x = 0; x < COLS; x += 32) tc::ld32(taddr + x, o + x);
+        tc::wait_ld();
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            // r = 1 / (e^2x + 1): tanh = 1 - 2 r, 1 - tanh^2 = 4 r (1 - r)
-            const float rx = __fdividef(1.f, tc::ex2(z[i].x * p.exp_per_raw) + 1.f), ry = __fdividef(1.f, tc::ex2(z[i].y * p.exp_per_raw) + 1.f);
-            if (SLOPE) dcap[i] = make_float2(4.f * rx * (1.f - rx), 4.f * ry * (1.f - ry));
-            z[i] = make_float2(fmaf(-2.f * p.cap_log2, rx, p.cap_log2), fmaf(-2.f * p.cap_log2, ry, p.cap_log2));
-        }
-        return;
+        for (int x = 0; x < COLS; ++x) o[x] = 0;
     }
-    if (SLOPE) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) dcap[i] = tc::fma2(tc::mul2(z[i], z[i]), tc::both(p.minus_inv_cap2), tc::both(1.f));
-    }
-}
-
-// A warp's 32 rows x 32 columns of fp32 accumulators (a row per lane) as bf16 to global memory, times `by`: through a 2 KB
-// staging buffer of the warp, so that four lanes write 64 bytes of a row together and not each lane 16 bytes of its own.
-// row_ptr(r): where row r's first of these columns goes; columns from `cols` on and rows from `rows` on are left out.
-template <typename F>
-__device__ __forceinline__ void store_block32(uint32_t stage, const uint32_t* o, float by, int rows, int cols, F&& row_ptr) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < LPR; ++i) {
         uint32_t v[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = pack_bf16x2(__uint_as_float(o[8 * i + 2 * k]) * by, __uint_as_float(o[8 * i + 2 * k + 1]) * by);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((i ^ (lane >> 1 & 3)) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * (COLS * 2) + ((i ^ (lane & MASK)) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
     }
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = 8 * i + (lane >> 2), c = lane & 3;
+    for (int k = 0; k < LPR; ++k) {
+        const int r = k * (32 / LPR) + lane / LPR, c = lane % LPR;
         uint4 v;
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(stage + r * 64 + ((c ^ (r >> 1 & 3)) << 4)) : "memory");
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(stage + r * (COLS * 2) + ((c ^ (r & MASK)) << 4)) : "memory");
         if (r < rows && 8 * c < cols) *reinterpret_cast<uint4*>((bf16*)row_ptr(r) + 8 * c) = v;
     }
-    __syncwarp();
 }
 
 bool attention_tc_supported(const AttnParams& p, int dtype);
