@@ -571,14 +571,24 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         const float delta = deltas[threadIdx.x & 127] + deltas[kTile + (threadIdx.x & 127)];
         if (w == 0 && live) p.a.delta[lines + t] = delta;
         int* my_docs = docs + (warp - 4) * 64;
+        int ahead_docs[2];                                       // documents of the tile to come, asked for a tile ahead
+        auto fetch = [&](int i) {
+            if (DOCS && list[i] >> 14 == kDocs) {
+                const int k = tile_of(list[i]) * kTile + 64 * w + lane;
+                ahead_docs[0] = k < p.a.k_len ? m.k_docs[k] : 0;
+                ahead_docs[1] = k + 32 < p.a.k_len ? m.k_docs[k + 32] : 0;
+            }
+        };
+        if (total) fetch(0);
         for (int i = 0; i < total && ok; ++i) {
             const int entry = list[i], key0 = tile_of(entry) * kTile + 64 * w;
             const int cls = entry >> 14;
             if (DOCS && cls == kDocs) {
                 __syncwarp();
-                for (int k = lane; k < 64; k += 32) my_docs[k] = key0 + k < p.a.k_len ? m.k_docs[key0 + k] : 0;
+                my_docs[lane] = ahead_docs[0]; my_docs[lane + 32] = ahead_docs[1];
                 __syncwarp();
             }
+            if (i + 1 < total) fetch(i + 1);
             ok = warp_wait(s_full(i & 1), i / 2 & 1, ab, 48);
             if (!ok) break;
             fence_after();

@@ -40,11 +40,12 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     unsigned char* cls = mem + (2 + ST) * OP;                  // two bits for each tile of queries
     int* docs = reinterpret_cast<int*>(cls + kMaxTiles);       // 128 for each softmax warp
     const uint32_t bars = smem_u32(docs + 8 * 128);
-    const uint32_t q_full = bars, o_full = bars + 8, v_blank = bars + 16, blank_go = bars + 248;
+    const uint32_t q_full = bars, v_blank = bars + 8, blank_go = bars + 16;
     auto s_full = [&](int w) { return bars + 24 + 8 * w; };
-    auto p_full = [&](int w) { return bars + 40 + 8 * w; };
-    auto kv_full = [&](int s) { return bars + 56 + 8 * s; };
-    auto kv_empty = [&](int s) { return bars + 56 + 8 * (ST + s); };
+    auto o_full = [&](int w) { return bars + 40 + 8 * w; };
+    auto p_full = [&](int w) { return bars + 56 + 8 * w; };
+    auto kv_full = [&](int s) { return bars + 72 + 8 * s; };
+    auto kv_empty = [&](int s) { return bars + 72 + 8 * (ST + s); };
     __shared__ uint32_t tmem_slot;
     __shared__ Abort ab;
 
@@ -63,8 +64,8 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const int blank_tile = m.keys < p.a.k_len && m.keys % kTile ? m.keys / kTile : -1;
     if (threadIdx.x == 0) {
         ab.flag = 0; ab.err = p.err;
-        mbar_init(q_full, 1); mbar_init(o_full, 1); mbar_init(v_blank, 1); mbar_init(blank_go, 1);
-        for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(p_full(w), 4); }
+        mbar_init(q_full, 1); mbar_init(v_blank, 1); mbar_init(blank_go, 1);
+        for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(o_full(w), 1); mbar_init(p_full(w), 4); }
         for (int s = 0; s < ST; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -115,7 +116,8 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             for (int i = 0; i < ST && ok; ++i, ++seq) ok = mbar_wait(kv_empty(seq % ST), (seq / ST & 1) ^ 1, ab, 21);
         } else if (warp == 1) {
             // ---------------------------------------------------------------- products
-            int u = -1, prev = 0, prev_j = -1, used_p[2] = {0, 0};
+            int u = -1, prev = 0, prev_j = -1, used_p[2] = {0, 0}, last[2] = {tiles - 1, tiles - 1};
+            for (int w = 0; w < 2; ++w) while (last[w] >= 0 && !(cls[last[w]] >> (2 * w) & 3)) --last[w];
             bool ok = warp_wait(q_full, 0, ab, 22);
             for (int j = 0; j <= tiles && ok; ++j) {
                 const int c = j < tiles ? cls[j] : 0;
@@ -139,7 +141,10 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                         ok = ok && warp_wait(p_full(w), used_p[w] & 1, ab, 25);
                         if (!ok) break;
                         fence_after();
-                        if (elect()) product_tn<DP, kTile>(o_at(w), s_at(w), v_buf, used_p[w] > 0);
+                        if (elect()) {
+                            product_tn<DP>(o_at(w), s_at(w), v_buf, used_p[w] > 0);
+                            if (prev_j == last[w]) commit(o_full(w));
+                        }
                         ++used_p[w];
                     }
                     if (c >> (2 * w) & 3) {
@@ -160,7 +165,6 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 prev = c;
                 prev_j = j;
             }
-            if (elect()) commit(o_full);
         } else if (warp == 2 && blank_tile >= 0 && blank_tile < tiles && cls[blank_tile]) {
             // ---------------------------------------------------------------- rows of V behind key_len: zero, whatever they held
             // (the issuer says when V has landed: a parity wait of this warp's own on the ring could be a phase late or early)
@@ -191,15 +195,26 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         float top = -INFINITY, total = 0.f;
         int n = 0;
         bool ok = true;
-        for (int j = 0; j < tiles; ++j) {
-            const int c = cls[j] >> (2 * w) & 3;
-            if (!c) continue;
-            const int key0 = j * kTile;
+        auto class_at = [&](int j) { return cls[j] >> (2 * w) & 3; };
+        auto next_tile = [&](int j) { do ++j; while (j < tiles && class_at(j) == kSkip); return j; };
+        int ahead[4];                                            // documents of the tile to come, asked for a tile ahead
+        auto fetch = [&](int j) {
+            if (DOCS && j < tiles && class_at(j) == kDocs)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) ahead[k] = j * kTile + k * 32 + lane < p.a.k_len ? m.k_docs[j * kTile + k * 32 + lane] : 0;
+        };
+        int next = next_tile(-1);
+        fetch(next);
+        while (next < tiles) {
+            const int j = next, c = class_at(j), key0 = j * kTile;
             if (DOCS && c == kDocs) {
                 __syncwarp();
-                for (int i = lane; i < kTile; i += 32) my_docs[i] = key0 + i < p.a.k_len ? m.k_docs[key0 + i] : 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) my_docs[k * 32 + lane] = ahead[k];
                 __syncwarp();
             }
+            next = next_tile(j);
+            fetch(next);
             ok = warp_wait(s_full(w), n & 1, ab, 28);
             if (!ok) break;
             fence_after();
@@ -296,14 +311,15 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             if (lane == 0) mbar_arrive(p_full(w));
             ++n;
         }
-        if (ok) ok = warp_wait(o_full, 0, ab, 29);
+        // (a warpgroup that saw no key still waits for its queries: their memory is written below)
+        if (ok) ok = n ? warp_wait(o_full(w), 0, ab, 29) : warp_wait(q_full, 0, ab, 29);
         if (ok) {
             fence_after();
             const float by = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
-            // the rings are idle now: their memory stages the rows
+            // this warpgroup's queries have been multiplied for the last time: their memory stages the rows
             const int t0 = q0 + w * kTile + (warp & 3) * 32;
             bf16* out = (bf16*)p.a.out + (int64_t)b * p.a.os.b + (int64_t)t0 * p.a.os.t + (int64_t)h * p.a.os.h;
-            store_rows<DP>(o_at(w) + lanes, n > 0, ring + (warp - 4) * (64 * DP), by, p.a.q_len - t0, p.a.dim, [&](int r) { return out + r * p.a.os.t; });
+            store_rows<DP>(o_at(w) + lanes, n > 0, q_at + (warp - 4) * (64 * DP), by, p.a.q_len - t0, p.a.dim, [&](int r) { return out + r * p.a.os.t; });
             if (live && p.a.lse) p.a.lse[((int64_t)b * p.a.heads + h) * p.a.q_len + t] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
         }
     }

@@ -76,12 +76,12 @@ __device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t b) {
     for (int k = 0; k < DP / 16; ++k)
         mma_ss(d, da + (((k / 4) * (128 * 128) + (k % 4) * 32) >> 4), db + (((k / 4) * (N * 128) + (k % 4) * 32) >> 4), idesc(N, false), k > 0);
 }
-// D[128 x DP] (+)= A[128 x K] . B[K x DP], A in tensor memory, B in boxes of K rows, which run along the product.
-template <int DP, int K>
+// D[128 x DP] (+)= A[128 x 128] . B[128 x DP], A in tensor memory, B in boxes of 128 rows, which run along the product.
+template <int DP>
 __device__ __forceinline__ void product_tn(uint32_t d, uint32_t a, uint32_t b, uint32_t accumulate) {
-    const uint64_t db = desc_mn<K>(b);
+    const uint64_t db = desc_mn<128>(b);
 #pragma unroll
-    for (int k = 0; k < K / 16; ++k) mma_ts(d, a + k * 8, db + ((k * 2048) >> 4), idesc(DP, true), accumulate || k > 0);
+    for (int k = 0; k < 8; ++k) mma_ts(d, a + k * 8, db + ((k * 2048) >> 4), idesc(DP, true), accumulate || k > 0);
 }
 // True in one lane of a converged warp.  The products are issued by a whole warp that runs its loop together and elects a
 // lane around the instructions only: their descriptors then live in uniform registers.  (Issued from a branch that a single

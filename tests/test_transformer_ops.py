@@ -2,6 +2,7 @@
 GPU against plain 64-bit evaluations with elementwise bounds (tests/block_reference.py)."""
 import ctypes
 import math
+import os
 import types
 
 import numpy as np
@@ -721,7 +722,11 @@ def test_adamw_8_bit_rounding_has_no_drift(device):
         assert abs(float(value[:, k::2].mean()) - want) < 0.03 * want
 
 
+no_guard_zones = pytest.mark.skipif(os.environ.get("ORMI_B200_POOL_CANARY", "0") not in ("", "0"), reason="a capture is refused while guard zones are on")
+
+
 @gpu
+@no_guard_zones
 def test_adamw_with_a_device_counter_captured_and_replayed(device):
     from ormi_b200.runtime import Device
     dev = Device(0)
@@ -905,6 +910,7 @@ def test_mlp_trainer_refuses_unknown_optimizers():
 
 
 @gpu
+@no_guard_zones
 def test_captured_block_replays_with_new_inputs_and_weights():
     """A captured forward and backward pass with an AdamW step: replays read the buffers' new contents, update in place, and a bf16
     copy made of a captured output outside is not used after a replay."""
