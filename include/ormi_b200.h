@@ -301,9 +301,9 @@ int ormi_b200_rmsnorm_backward(ormi_b200_ctx* ctx, const ormi_b200_rmsnorm_backw
  *     j < key_len[batch]                            (key_len left out: every key; what lies behind it is never used)
  *     not causal, or j <= pos, or j < prefix[batch] (prefix left out: 0)
  *     q_docs[batch, query] == k_docs[batch, j]      (left out: one document)
- * pos = q_start[batch] + query; q_start left out: k_len - q_len, the last q_len positions.  A query that sees no key
- * gets out = 0 and lse = -infinity (and zero gradients).  Keys and values inside key_len have to be finite where a
- * query of the same call sees them or not; behind key_len they may hold anything.
+ * pos = q_start[batch] + query (below 2^31); q_start left out: k_len - q_len, the last q_len positions.  A query that sees
+ * no key gets out = 0 and lse = -infinity (and zero gradients).  Keys and values inside key_len have to be finite, whether
+ * a query sees them or not (they take part in products with zeros); behind key_len they may hold anything.
  * heads is a multiple of kv_heads: query head h reads key/value head h / (heads / kv_heads).
  * q, k, v, out: one type, F32 or BF16.  lse: [batch, heads, q_len] F32, contiguous, optional.  slopes: [heads] F32.
  * q_docs [batch, q_len], k_docs [batch, k_len], prefix, key_len, q_start [batch]: I32, contiguous, on the device. */
@@ -318,7 +318,10 @@ int ormi_b200_attention(ormi_b200_ctx* ctx, const ormi_b200_attention_args* args
 
 /* Its backward pass: dq, dk, dv from dout and the forward call's arguments, `out` and `lse` (required here) as the
  * forward call wrote them.  dk and dv of a shared head are the sums over its query heads; keys nobody sees get zero.
- * dq, dk, dv: q's type, the shapes of q, k, v.  Slopes, cap and scale are constants. */
+ * dq, dk, dv: q's type, the shapes of q, k, v; they may be slices of one buffer.  Slopes, cap and scale are constants.
+ * On the tensor cores (BF16, head_dim a multiple of 8 up to 128, 16-byte aligned addresses and strides, scale > 0, up to
+ * 2^20 keys forward and 2^19 positions backward) both passes round probabilities and score gradients to bf16; other cases
+ * run in fp32 arithmetic. */
 typedef struct ormi_b200_attention_backward_args {
     ormi_b200_attention_args forward;
     ormi_b200_view dout, dq, dk, dv;
@@ -334,7 +337,9 @@ int ormi_b200_attention_backward(ormi_b200_ctx* ctx, const ormi_b200_attention_b
  * with one fp32 scale for every 128 elements in m_scales / v_scales (ceil(n / 128) each; value = code * scale, scale =
  * largest magnitude of the block / 448).  Codes are rounded up or down at random in proportion to the distance (a state
  * that moves by less than half a step would otherwise stand still), with bits hashed from (seed, step, tensor, element);
- * a positive sqrt(v) never becomes zero.  All-zero codes and scales are the initial state.
+ * a positive sqrt(v) never becomes zero.  All-zero codes and scales are the initial state.  A gradient that is not finite
+ * leaves its element, and with 8-bit states the 128 elements of its block, not finite.
+ * Buffers are contiguous; none that is written may overlap another one of the call.
  * device_step (optional, for captured steps): a device counter of the steps done so far; the call takes *device_step + 1
  * as its step and adds one.  device_lr, grad_scale (optional): device floats, read when the kernel runs. */
 typedef struct ormi_b200_adamw_tensor {

@@ -163,13 +163,15 @@ __global__ void __launch_bounds__(kThreads) adamw_f32(const __grid_constant__ Ba
 __device__ __forceinline__ void step_block(const Common& c, const Rates& r, float decay, const uint32_t (&h)[4], const float (&g)[4], const float (&cm)[4], const float (&cv)[4], float sm, float sv,
                                            float (&p)[4], float (&qm)[4], float (&qv)[4], float& hi_m, float& hi_v) {
     using namespace tc;
+    // a packed product and a packed sum were seen to be fused into one operation; a packed product and two plain sums are not
+    auto sum_of = [](const float2& a, const float2& b) { return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)); };
     float2 m[2], root[2];
     uint32_t top_m = 0, top_v = 0;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const float2 grad = mul2(make_float2(g[2 * k], g[2 * k + 1]), both(r.gs)), old = mul2(make_float2(cv[2 * k], cv[2 * k + 1]), both(sv));
-        m[k] = add2(mul2(both(c.b1), mul2(make_float2(cm[2 * k], cm[2 * k + 1]), both(sm))), mul2(both(c.c1), grad));
-        const float2 v = add2(mul2(both(c.b2), mul2(old, old)), mul2(mul2(both(c.c2), grad), grad));
+        m[k] = sum_of(mul2(both(c.b1), mul2(make_float2(cm[2 * k], cm[2 * k + 1]), both(sm))), mul2(both(c.c1), grad));
+        const float2 v = sum_of(mul2(both(c.b2), mul2(old, old)), mul2(mul2(both(c.c2), grad), grad));
         root[k] = make_float2(sqrtf(v.x), sqrtf(v.y));
         const float2 den = fma2(root[k], both(r.inv_sqrt_bc2), both(c.eps));
         const float2 up = mul2(mul2(m[k], both(r.lr * r.inv_bc1)), make_float2(quick_inverse(den.x), quick_inverse(den.y)));
@@ -332,7 +334,8 @@ void launch(ormi_b200_ctx* ctx, Batch<N>& b, int chunks, int state_bits) {
 void* kept_copy(ormi_b200_ctx* ctx, const ormi_b200_adamw_tensor& t) {
     if (ctx->shadows.empty()) return nullptr;
     auto it = ctx->shadows.find(t.param);
-    const bool whole = it != ctx->shadows.end() && it->second.ld == it->second.cols && (int64_t)it->second.rows * it->second.cols == t.n;
+    // (a copy that already belongs to another captured step is not shared with this one)
+    const bool whole = it != ctx->shadows.end() && !(ctx->capturing && ctx->graph_owned.count(it->second.ptr)) && it->second.ld == it->second.cols && (int64_t)it->second.rows * it->second.cols == t.n;
     if (!whole || t.copy16) { shadow_drop(ctx, t.param, (size_t)t.n * 4); return nullptr; }
     const Shadow16 keep = it->second;
     ctx->shadows.erase(it);

@@ -112,6 +112,8 @@ def test_attention_accepts_what_is_documented():
 
 @pytest.mark.parametrize("words, change", [
     ("head_dim is 1 to 256", dict(d=257)),
+    ("above 2^30", dict(nk=(1 << 30) + 1)),
+    ("above 2^30", dict(b=1, nq=1 << 29)),
     ("multiple of kv_heads", dict(h=3)),
     ("another type", dict(k=V(0x200000, (2, 16, 2, 32), "f32"))),
     ("another batch", dict(k=V(0x200000, (3, 16, 2, 32), "bf16"), v=V(0x300000, (3, 16, 2, 32), "bf16"))),
@@ -152,7 +154,12 @@ def test_attention_backward_arguments():
     accepted(attn_back(dq=joint(0, 4), dk=joint(4, 2), dv=joint(6, 2)))                   # slices of one gradient
     refused(attn_back(lse=None), "lse")
     refused(attn_back(dk=V(0x30000, (2, 16, 2, 32), "bf16")), "dk overlaps k")
-    refused(attn_back(dv=V(0x80000, (2, 16, 2, 32), "bf16")), "same buffer")
+    refused(attn_back(dv=V(0x80000, (2, 16, 2, 32), "bf16")), "dv overlaps dk")
+    refused(attn_back(dq=joint(0, 4), dk=joint(3, 2), dv=joint(6, 2)), "dk overlaps dq")
+    refused(attn_back(dq=joint(0, 4), dk=joint(4, 2), dv=joint(7, 2)), "dv overlaps dq")          # runs into the next position
+    heads_first = lambda first, n: V(0x70000 + first * 16 * 64, (2, 16, n, 32), "bf16", (8 * 16 * 32, 32, 16 * 32, 1))      # noqa: E731
+    accepted(attn_back(dq=heads_first(0, 4), dk=heads_first(4, 2), dv=heads_first(6, 2)))
+    refused(attn_back(dq=heads_first(0, 4), dk=heads_first(4, 2), dv=heads_first(5, 2)), "dv overlaps dk")
     refused(attn_back(dq=V(0x70000, (2, 16, 2, 32), "bf16")), "another shape")
     refused(attn_back(dk=V(0x80000, (2, 16, 2, 32), "bf16", (1024, 64, 0, 1))), "rows overlap")
 
@@ -562,6 +569,42 @@ def test_attention_is_deterministic(device, dtype, d):
 
 
 @gpu
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-4, 3.0])
+@pytest.mark.parametrize("nq", [3, 200])
+def test_attention_scales(device, scale, nq):
+    run_attention(device, *qkv(1, nq, 260, 2, 1, 64, BF), scale=scale, causal=True)
+    run_attention(device, *qkv(1, nq, 260, 2, 1, 64, BF), scale=scale, cap=4.0)
+
+
+@gpu
+@pytest.mark.parametrize("group", [2, 3, 4, 8])
+@pytest.mark.parametrize("nk", [100, 1500])
+def test_attention_gradients_of_shared_heads(device, group, nk):
+    """Few blocks (clusters share the heads), many, groups that do not divide into clusters."""
+    docs = (torch.arange(nk, device="cuda") // 300).int()[None].repeat(2, 1)
+    run_attention(device, *qkv(2, nk, nk, 2 * group, 2, 72, BF), causal=True, q_docs=docs, k_docs=docs)
+    run_attention(device, *qkv(2, nk, nk, 2 * group, 2, 128, BF))
+
+
+@gpu
+def test_attention_rows_that_are_not_finite_stay_alone(device):
+    """A query that is not finite spoils its own row; the others, keys behind key_len and NaN included, come out as without it."""
+    for nq in (4, 300):
+        q, k, v = qkv(1, nq, 300, 4, 2, 64, BF)
+        want = torch.empty_like(q)
+        got, bad = torch.empty_like(q), q.clone()
+        bad[0, nq // 2, 1] = float("nan")
+        bad[0, nq // 2, 2] = float("inf")
+        torch.cuda.synchronize()
+        ops.attention(device, q, k, v, want, causal=True, key_len=ints(260), q_start=ints(0))
+        ops.attention(device, bad, k, v, got, causal=True, key_len=ints(260), q_start=ints(0))
+        done(device)
+        rows = torch.ones(nq, 4, dtype=torch.bool, device="cuda")
+        rows[nq // 2, 1:3] = False
+        assert torch.equal(got[0][rows], want[0][rows]) and bool(got[0, nq // 2, 1].isnan().all())
+
+
+@gpu
 def test_attention_of_nothing(device):
     q, k, v = qkv(2, 5, 0, 2, 2, 64, BF)
     out, lse = run_attention(device, q, k, v, back=True)
@@ -698,6 +741,38 @@ def test_adamw_states_in_8_bits(device, grads):
             assert bool(((got.abs() == want.clamp(max=448.0)) | unsure).all()), name
             close(name + " codes", got.abs(), a, step + 2 * a_err)
             assert bool(((got == 0) | (torch.sign(got) == torch.sign(value)) | (value.abs() <= err)).all())
+
+
+@gpu
+def test_adamw_8_bit_codes_are_those_of_the_formulas_in_fp32(device):
+    """m, sqrt(v), scales and codes evaluated operation by operation in fp32, in their written order, twice in a row: bit for bit."""
+    n = 1 << 20
+    s = adam_state([n, 1000], bits=8)
+    m, r, ms, rs = ([x.clone() for x in y] for y in (s.m, s.v, s.ms, s.vs))
+    gs = torch.tensor([0.5], device="cuda")
+    opt = ops.AdamW(device, s.p, s.g, s.m, s.v, m_scales=s.ms, v_scales=s.vs, betas=(0.9, 0.95), seed=99)
+    torch.cuda.synchronize()
+    for step in (5, 6):
+        opt.step(lr=0.01, step=step, grad_scale=gs)
+        done(device)
+        for i in range(2):
+            size = s.p[i].numel()
+            wide = lambda x: x.repeat_interleave(128)[:size]      # noqa: E731
+            g = s.g[i] * gs
+            nm = 0.9 * (m[i].float() * wide(ms[i])) + (1 - 0.9) * g
+            nr = torch.sqrt(0.95 * (r[i].float() * wide(rs[i])).square() + (1 - 0.95) * g * g)
+            h = mix32(torch.arange(size, device="cuda") ^ int(mix32(torch.tensor((int(mix32(torch.tensor(99 ^ step))) + i) & 0xffffffff))))
+            for name, x, bits, codes, scales, old, old_scale in (("m", nm, h & 0xffff, s.m[i], s.ms[i], m, ms), ("r", nr, h >> 16, s.v[i], s.vs[i], r, rs)):
+                top = torch.nn.functional.pad(x, (0, -size % 128)).view(-1, 128).abs().amax(1)
+                assert torch.equal(scales, top * (1 / torch.tensor(448.0, device="cuda"))), name
+                a = (x * wide((1 / top) * 448)).abs().clamp(max=448)
+                if name == "r":
+                    a = torch.where(x > 0, a.clamp(min=2.0 ** -9), a)
+                e = torch.frexp(a)[1].clamp(min=-5) - 1
+                unit = torch.ldexp(torch.ones_like(a), e - 3)
+                want = torch.copysign(torch.floor(a / unit + bits.float() / 65536) * unit, x).to(torch.float8_e4m3fn)
+                assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8)), name
+                old[i], old_scale[i] = codes.clone(), scales.clone()
 
 
 @gpu
@@ -893,14 +968,17 @@ def test_mlp_trainer_with_adamw(matmul, sharded, monkeypatch):
 def test_mlp_trainer_with_adamw_in_8_bits_stays_near_32(device):
     from ormi_b200.train_step import MLPTrainer
     x, t, *params = mlp()
-    losses = {}
+    lr, steps, got = 0.003, 10, {}
     for bits in (32, 8):
-        tr = MLPTrainer(device, x, t, *params, lr=0.003, optimizer="adamw", adamw=dict(state_bits=bits, betas=(0.9, 0.99)))
-        for _ in range(10):
+        tr = MLPTrainer(device, x, t, *params, lr=lr, optimizer="adamw", adamw=dict(state_bits=bits, betas=(0.9, 0.99)))
+        for _ in range(steps):
             tr.step()
-        losses[bits] = tr.loss()
-        assert all(np.isfinite(tr.parameter(k)).all() for k in ("w1", "b1", "w2", "b2"))
-    assert abs(losses[8] - losses[32]) < 0.1 * losses[32]
+        got[bits] = [tr.parameter(k) for k in ("w1", "b1", "w2", "b2")]
+    for p8, p32, old in zip(got[8], got[32], params):
+        # a code is off by a step (1/8 of the value) at most and by less on average, so an update m / sqrt(v) of size lr is off by
+        # 1/4 at most to first order; the mean over a tensor and ten steps stays below that
+        assert np.abs(p8 - p32).mean() < 0.25 * steps * lr
+        assert np.isfinite(p8).all() and np.abs(p8 - old.ravel()).mean() > lr
 
 
 def test_mlp_trainer_refuses_unknown_optimizers():
