@@ -246,6 +246,12 @@ __global__ void __launch_bounds__(256) attn_delta(AttnParams p) {
     if (lane == 0) p.delta[((int64_t)b * p.heads + h) * p.q_len + t] = s;
 }
 
+// Rows of the partial gradients of a split loop, and a row's place among them.
+template <bool QUERY> __host__ __device__ inline int64_t part_rows(const AttnParams& p) { return (int64_t)p.batch * (QUERY ? (int64_t)p.q_len * p.heads : (int64_t)p.k_len * p.kv_heads); }
+template <bool QUERY> __device__ __forceinline__ int64_t part_row(const AttnParams& p, int b, int t, int h) {
+    return QUERY ? ((int64_t)b * p.q_len + t) * p.heads + h : ((int64_t)b * p.k_len + t) * p.kv_heads + h;
+}
+
 // dk and dv of one tile of keys: a loop over the packed query rows.  QUERY: dq of one tile of rows, a loop over the keys.
 template <typename T, int B, int DP, bool QUERY>
 __global__ void __launch_bounds__(kThreads) attn_backward(AttnParams p) {
@@ -280,6 +286,11 @@ __global__ void __launch_bounds__(kThreads) attn_backward(AttnParams p) {
         const int last = min(mine + B, rows) - 1;
         hi = (key_end(m, m.start + last / p.group) + B - 1) / B;
     } else if (mine >= m.keys) hi = 0;
+    if (p.splits > 1) {                              // a part of the loop for each block in z
+        const int per = (max(hi, 0) + p.splits - 1) / p.splits;
+        lo = blockIdx.z * per;
+        hi = min(lo + per, hi);
+    }
     for (int n = lo; n < hi; ++n) {
         const int row0 = QUERY ? mine : n * B, key0 = QUERY ? n * B : mine;
         if (!QUERY) {
@@ -322,6 +333,15 @@ __global__ void __launch_bounds__(kThreads) attn_backward(AttnParams p) {
     for (int i = 0; i < RI; ++i) {
         const int r = mine + ty + 16 * i;
         if (r >= (QUERY ? rows : p.k_len)) continue;
+        if (p.splits > 1) {
+            const int64_t at_row = part_row<QUERY>(p, b, r / (QUERY ? p.group : 1), QUERY ? kvh * p.group + r % p.group : kvh);
+            for (int c = 0; c < DP / 64; ++c) {
+                const int d = c * 64 + tx * 4;
+                store4(p.part_out + ((int64_t)blockIdx.z * part_rows<QUERY>(p) + at_row) * p.dim, d, p.dim, one[i][c], 1.f);
+                if (!QUERY) store4(p.part_out + ((int64_t)(p.splits + blockIdx.z) * part_rows<QUERY>(p) + at_row) * p.dim, d, p.dim, two[i][c], 1.f);
+            }
+            continue;
+        }
         for (int c = 0; c < DP / 64; ++c) {
             const int d = c * 64 + tx * 4;
             if (QUERY) store4((T*)p.dq + at(p.dqs, b, r / p.group, kvh * p.group + r % p.group), d, p.dim, one[i][c], 1.f);
@@ -330,6 +350,21 @@ __global__ void __launch_bounds__(kThreads) attn_backward(AttnParams p) {
                 store4((T*)p.dv + at(p.dvs, b, r, kvh), d, p.dim, two[i][c], 1.f);
             }
         }
+    }
+}
+
+// The parts of a split backward loop, added in order: a warp per row.
+template <typename T, bool QUERY>
+__global__ void __launch_bounds__(256) attn_backward_join(AttnParams p) {
+    const int64_t rows = part_rows<QUERY>(p), row = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) % rows, which = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) / rows;
+    if (which >= (QUERY ? 1 : 2)) return;
+    const int heads = QUERY ? p.heads : p.kv_heads, len = QUERY ? p.q_len : p.k_len;
+    const int h = row % heads, t = row / heads % len, b = row / heads / len;
+    T* out = QUERY ? (T*)p.dq + at(p.dqs, b, t, h) : which ? (T*)p.dv + at(p.dvs, b, t, h) : (T*)p.dk + at(p.dks, b, t, h);
+    for (int d = threadIdx.x & 31; d < p.dim; d += 32) {
+        float v = 0.f;
+        for (int s = 0; s < p.splits; ++s) v += p.part_out[((which * p.splits + s) * rows + row) * p.dim + d];
+        out[d] = from_f32<T>(v);
     }
 }
 
@@ -384,9 +419,22 @@ void run_backward(ormi_b200_ctx* ctx, AttnParams& p) {
     const int64_t rows = QUERY ? (int64_t)p.q_len * p.group : p.k_len;
     if (!rows) return;
     allow_smem(kernel, smem);
-    kernel<<<dim3(tiles(rows, B), p.batch * p.kv_heads), kThreads, smem, ctx->stream>>>(p);
+    const int blocks_x = tiles(rows, B), pairs = p.batch * p.kv_heads;
+    // Too few blocks for two per SM: the loop is cut, with two turns left for each part, and the parts are added afterwards
+    // (333 tokens, 4 heads over 2, head_dim 40, fp32: 179 -> 81 us for the whole backward pass).
+    const int64_t turns = ((QUERY ? (int64_t)p.k_len : (int64_t)p.q_len * p.group) + B - 1) / B;
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({2ll * ctx->num_sms / ((int64_t)blocks_x * pairs), turns / 2, 16}));
+    Scratch part(ctx, p.splits > 1 ? (size_t)p.splits * (QUERY ? 1 : 2) * part_rows<QUERY>(p) * p.dim * 4 : 0);
+    p.part_out = (float*)part.ptr;
+    kernel<<<dim3(blocks_x, pairs, p.splits), kThreads, smem, ctx->stream>>>(p);
     ORMI_CUDA(cudaGetLastError());
     count_launch(ctx);
+    if (p.splits > 1) {
+        attn_backward_join<T, QUERY><<<tiles(part_rows<QUERY>(p) * (QUERY ? 1 : 2), 8), 256, 0, ctx->stream>>>(p);
+        ORMI_CUDA(cudaGetLastError());
+        count_launch(ctx);
+    }
+    part.release();
 }
 
 template <typename T, bool QUERY>
