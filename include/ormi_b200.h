@@ -255,6 +255,7 @@ int ormi_b200_colsum_static(const float* in, int64_t rows, int64_t cols, float* 
  *   - arguments are checked before the context is looked at and before anything is queued: a refused call has written
  *     nothing;
  *   - scratch comes from the context's pool, so the calls may be captured (ormi_b200_capture_begin) after one plain run;
+ *   - calls on one context come from one host thread at a time (contexts of their own may be used side by side);
  *   - buffers live on the context's device; an output may overlap an input only where its description says so;
  *   - results are bit-identical run to run (no atomics on values). */
 enum ormi_b200_dtype { ORMI_F32 = 0, ORMI_BF16 = 1, ORMI_E4M3 = 2, ORMI_I32 = 3 };

@@ -828,6 +828,116 @@ def test_adamw_with_a_device_counter_captured_and_replayed(device):
         dev.close()
 
 
+# ---- offsets past 32 bits
+
+@gpu
+def test_attention_over_a_cache_whose_offsets_pass_32_bits(device):
+    """Two sequences of 524 293 positions, 32 heads of 128: 4.3e9 elements each for keys and values; one new token and 130 of them."""
+    b, nk, h, d = 2, (1 << 19) + 5, 32, 128
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.empty(b, nk, h, d, device="cuda", dtype=BF).normal_(generator=g) for _ in range(2))
+    assert k.numel() > 1 << 32
+    for nq in (1, 130):
+        q = randn(b, nq, h, d, dtype=BF, seed=nq)
+        out, lse = torch.empty_like(q), torch.empty(b, h, nq, device="cuda")
+        torch.cuda.synchronize()
+        ops.attention(device, q, k, v, out, lse, causal=True, scale=0.3)
+        done(device)
+        for i, n in ((0, 0), (1, 31)):
+            ref = Attention(q[i:i + 1, :, n:n + 1], k[i:i + 1, :, n:n + 1], v[i:i + 1, :, n:n + 1], causal=True, scale=0.3)
+            want, bound, want_lse, lse_bound = ref.forward()
+            close("out", out[i:i + 1, :, n:n + 1], want, bound)
+            close("lse", lse[i:i + 1, n:n + 1], want_lse, lse_bound)
+            del ref, want, bound
+    del k, v
+    torch.cuda.empty_cache()
+
+
+@gpu
+def test_norm_over_rows_whose_offsets_pass_32_bits(device):
+    rows, cols = (1 << 20) + 7, 4096
+    x = torch.empty(rows, cols, device="cuda", dtype=BF).normal_(generator=torch.Generator(device="cuda").manual_seed(2))
+    out, rstd, w = torch.empty_like(x), torch.empty(rows, device="cuda"), randn(cols, dtype=BF, seed=3)
+    torch.cuda.synchronize()
+    ops.rmsnorm(device, x, w, out, rstd=rstd)
+    done(device)
+    pick = torch.tensor([0, 1 << 19, (1 << 20) + 1, rows - 1], device="cuda")
+    y = x[pick].to(F8) / torch.sqrt(x[pick].to(F8).square().mean(1, keepdim=True) + 1e-6)
+    close("out", out[pick], y * w.to(F8), 1.02 * 2.0 ** -8 * (y * w.to(F8)).abs())
+    dx = x                                                          # in place of the gradient
+    ops.rmsnorm_backward(device, out, out.clone(), w, rstd, dx)
+    done(device)
+    s, inv = out[pick].to(F8), rstd[pick].to(F8)[:, None]
+    gw = s * w.to(F8)
+    want = inv * (gw - s * (gw * s).mean(1, keepdim=True) * inv * inv)
+    size = inv * (gw.abs() + s.abs() * (gw * s).abs().mean(1, keepdim=True) * inv * inv)
+    close("dx", dx[pick], want, 1.01 * (2.0 ** -8 * want.abs() + (cols + 16) * 2.0 ** -24 * size))
+    del x, out, dx, y, s
+    torch.cuda.empty_cache()
+
+
+@gpu
+def test_attention_of_many_documents_in_a_long_row(device):
+    """2^18 + 3 positions in documents of 100: nearly every pair of tiles is skipped."""
+    n, h, d = (1 << 18) + 3, 2, 64
+    q, k, v = (randn(1, n, h, d, dtype=BF, seed=i) for i in range(3))
+    dout = randn(1, n, h, d, dtype=BF, seed=7)
+    docs = (torch.arange(n, device="cuda") // 100).int()[None]
+    out, lse = torch.empty_like(q), torch.empty(1, h, n, device="cuda")
+    g = [torch.empty_like(q) for _ in range(3)]
+    torch.cuda.synchronize()
+    ops.attention(device, q, k, v, out, lse, causal=True, q_docs=docs, k_docs=docs)
+    ops.attention_backward(device, dout, q, k, v, out, lse, *g, causal=True, q_docs=docs, k_docs=docs)
+    done(device)
+    for first in (0, 100, 1300, 131000, n // 100 * 100):
+        cut = slice(first, min(first + 100, n))
+        ref = Attention(q[:, cut], k[:, cut], v[:, cut], causal=True)
+        want, bound, want_lse, lse_bound = ref.forward()
+        close("out", out[:, cut], want, bound)
+        close("lse", lse[:, :, cut], want_lse, lse_bound)
+        for (name, (want, bound)), got in zip(ref.backward(dout[:, cut], out[:, cut], lse[:, :, cut]).items(), g):
+            close(name, got[:, cut], want, bound)
+
+
+@gpu
+def test_two_contexts_and_their_threads_at_once(device):
+    """Two contexts' streams side by side, queued by one host thread and by a thread each: the results of calls made alone."""
+    import threading
+    from ormi_b200.runtime import Device
+    devs = [device, Device(0), Device(0), Device(0)]
+    try:
+        jobs = []
+        for i, (n, dt, dd) in enumerate(((700, BF, 64), (900, BF, 128), (300, FP, 64), (5, BF, 128))):
+            q, k, v = qkv(2, n, 1100, 4, 2, dd, dt)
+            jobs.append((q, k, v, randn(2, n, 4, dd, dtype=dt, seed=30 + i)))
+        blank = lambda q, k, v, dout: [torch.empty_like(q), torch.empty(2, 4, q.shape[1], device="cuda"), torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)]      # noqa: E731
+
+        def run(dev, job, got, times):
+            q, k, v, dout = job
+            for _ in range(times):
+                ops.attention(dev, q, k, v, got[0], got[1], causal=True)
+                ops.attention_backward(dev, dout, q, k, v, got[0], got[1], got[2], got[3], got[4], causal=True)
+        want, side, apart = ([blank(*job) for job in jobs] for _ in range(3))
+        torch.cuda.synchronize()
+        for job, got in zip(jobs, want):
+            run(device, job, got, 1)
+            done(device)
+        for i, (job, got) in enumerate(zip(jobs, side)):
+            run(devs[i % 2], job, got, 20)
+        threads = [threading.Thread(target=run, args=(devs[i], jobs[i], apart[i], 20)) for i in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        for d in devs:
+            d.sync()
+        for other in (side, apart):
+            assert all(torch.equal(x, y) for one, two in zip(want, other) for x, y in zip(one, two))
+    finally:
+        for d in devs[1:]:
+            d.close()
+
+
 # ---- together, and inside the training loop
 
 @gpu
