@@ -300,7 +300,7 @@ int ormi_b200_rmsnorm_backward(ormi_b200_ctx* ctx, const ormi_b200_rmsnorm_backw
  *     out = softmax over the visible keys j of z, times v;   lse = log(sum of exp(z))
  * Key j is visible to the query at position pos when all of these hold:
  *     j < key_len[batch]                            (key_len left out: every key; what lies behind it is never used)
- *     not causal, or j <= pos, or j < prefix[batch] (prefix left out: 0)
+ *     not causal, or j <= pos, or j < prefix[batch] (prefix left out: 0; without causal it changes nothing)
  *     q_docs[batch, query] == k_docs[batch, j]      (left out: one document)
  * pos = q_start[batch] + query (below 2^31); q_start left out: k_len - q_len, the last q_len positions.  A query that sees
  * no key gets out = 0 and lse = -infinity (and zero gradients).  Keys and values inside key_len have to be finite, whether

@@ -144,6 +144,11 @@ __global__ void __launch_bounds__(kThreads) attn_forward(AttnParams p) {
     const int tiles = (end + BN - 1) / BN, per = (tiles + p.splits - 1) / p.splits;
     const int lo = blockIdx.z * per, hi = min(lo + per, tiles);
     for (int n = lo; n < hi; ++n) {
+        if (m.k_docs) {                              // a tile of other documents is not loaded at all
+            bool any = false;
+            for (int i = 0; i < RI; ++i) for (int j = 0; j < RJ; ++j) any |= sees(m, o[i], n * BN + tx + 16 * j);
+            if (!__syncthreads_or(any)) continue;
+        }
         __syncthreads();
         load_rows<T, BN, DP>(K, n * BN, m.keys, p.dim, [&](int j) { return (const T*)p.k + at(p.ks, b, j, kvh); });
         load_rows<T, BN, DP>(V, n * BN, m.keys, p.dim, [&](int j) { return (const T*)p.v + at(p.vs, b, j, kvh); });
@@ -298,6 +303,14 @@ __global__ void __launch_bounds__(kThreads) attn_backward(AttnParams p) {
             const int last = min(row0 + B, rows) - 1;                 // the furthest that any row of this tile sees
             if (key_end(m, m.start + last / p.group) <= key0) continue;
         }
+        if (m.k_docs) {                              // a tile of other documents is not loaded at all
+            bool any = false;
+            for (int i = 0; i < RI; ++i) {
+                const RowOf o = row_of(p, m, kvh, row0 + ty + 16 * i);
+                for (int j = 0; j < RI; ++j) any |= sees(m, o, key0 + tx + 16 * j);
+            }
+            if (!__syncthreads_or(any)) continue;
+        }
         __syncthreads();
         if (QUERY) load_keys(key0); else load_queries(row0);
         __syncthreads();
@@ -383,9 +396,10 @@ void run_forward(ormi_b200_ctx* ctx, AttnParams& p) {
     const int smem = ((BM + 2 * BN) * (DP + 4) + BM * (BN + 4)) * 4;
     allow_smem(attn_forward<T, BM, BN, DP>, smem);
     const int rows = tiles((int64_t)p.q_len * p.group, BM), pairs = p.batch * p.kv_heads;
-    // Few rows over many keys: the keys are split until there are two blocks per SM, each with four tiles of keys at least.
+    // Few rows over many keys: the keys are split until there are two blocks per SM (four of the small ones, which wait for
+    // their loads most of the time), each with two tiles of keys at least.
     const int key_tiles = std::max(1, (p.k_len + BN - 1) / BN);
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(2ll * ctx->num_sms + (int64_t)rows * pairs - 1) / ((int64_t)rows * pairs), key_tiles / 4, 128}));
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({((BM < 64 ? 4ll : 2ll) * ctx->num_sms + (int64_t)rows * pairs - 1) / ((int64_t)rows * pairs), key_tiles / 2, 128}));
     const size_t lines = (size_t)p.batch * p.heads * p.q_len;
     Scratch part(ctx, p.splits > 1 ? p.splits * lines * (p.dim + 2) * 4 : 0);
     if (p.splits > 1) {
@@ -409,7 +423,7 @@ void forward_by_size(ormi_b200_ctx* ctx, AttnParams& p) {
     const int64_t rows = (int64_t)p.q_len * p.group;
     const int tile = rows <= 16 ? 16 : spread(ctx, p, rows) ? 32 : 64;
     if (p.dim <= 64) { if (tile == 16) run_forward<T, 16, 64, 64>(ctx, p); else if (tile == 32) run_forward<T, 32, 64, 64>(ctx, p); else run_forward<T, 64, 64, 64>(ctx, p); }
-    else if (p.dim <= 128) { if (tile == 16) run_forward<T, 16, 64, 128>(ctx, p); else if (tile == 32) run_forward<T, 32, 64, 128>(ctx, p); else run_forward<T, 64, 64, 128>(ctx, p); }
+    else if (p.dim <= 128) { if (tile == 16) run_forward<T, 16, 64, 128>(ctx, p); else if (tile == 32) run_forward<T, 32, 64, 128>(ctx, p); else run_forward<T, 64, 32, 128>(ctx, p); }
     else { if (tile == 16) run_forward<T, 16, 32, 256>(ctx, p); else run_forward<T, 64, 32, 256>(ctx, p); }
 }
 
@@ -531,7 +545,6 @@ void forward_check(const char* op, const ormi_b200_attention_args& a, bool backw
     ints_check(op, "q_start", a.q_start, b, -1);
     OP_NEED(std::isfinite(a.scale), op, "scale is not finite");
     OP_NEED(a.cap >= 0.f && std::isfinite(a.cap), op, "cap is negative or not finite");
-    OP_NEED(a.causal || !a.prefix.data, op, "prefix goes with causal");
 }
 
 // Whether two views whose spans overlap are slices of one buffer that never meet, such as the gradients of q, k and v side by

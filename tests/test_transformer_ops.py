@@ -104,6 +104,7 @@ def test_attention_accepts_what_is_documented():
     accepted(attn_args())
     accepted(attn_args(t="f32", d=256))
     accepted(attn_args(nq=0))
+    accepted(attn_args(prefix=V(0x500000, (2,), "i32")))
     accepted(attn_args(nk=0, k=V(0, (2, 0, 2, 32), "bf16"), v=V(0, (2, 0, 2, 32), "bf16")))
     accepted(attn_args(k=V(0x200000, (2, 16, 2, 32), "bf16", (0, 32, 512, 1))))
     accepted(attn_args(causal=True, prefix=V(0x500000, (2,), "i32"), key_len=V(0x500100, (2,), "i32"), q_start=V(0x500200, (2,), "i32"),
@@ -130,7 +131,6 @@ def test_attention_accepts_what_is_documented():
     ("key_len", dict(key_len=V(0x500000, (4,), "i32", (2,)))),
     ("scale is not finite", dict(scale=float("inf"))),
     ("cap", dict(cap=-1.0)),
-    ("prefix goes with causal", dict(prefix=V(0x500000, (2,), "i32"))),
     ("out overlaps q", dict(out=V(0x100000, (2, 16, 4, 32), "bf16"))),
     ("lse overlaps key_len", dict(lse=V(0x800000, (2, 4, 16)), key_len=V(0x800000, (2,), "i32"))),
     ("missing", dict(v=None)),
@@ -420,6 +420,7 @@ MASKS = {
     "bias": lambda: dict(slopes=torch.tensor([0.5, 0.1, 0.0, 2.0], device="cuda")),
     "bias_causal": lambda: dict(slopes=torch.tensor([0.5, 0.1, 0.0, 2.0], device="cuda"), causal=True),
     "prefix": lambda: dict(causal=True, prefix=ints(0, 200, 77)),
+    "prefix_alone": lambda: dict(prefix=ints(0, 200, 77)),
     "prefix_everything": lambda: dict(causal=True, prefix=ints(1000, -5, 1)),
     "key_len": lambda: dict(key_len=ints(0, 131, 300)),
     "key_len_causal": lambda: dict(key_len=ints(1, 64, 290), causal=True, q_start=ints(0, 0, 0)),
