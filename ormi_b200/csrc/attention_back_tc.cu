@@ -318,7 +318,8 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             __syncwarp();
             if (lane == 0) { mbar_arrive(ds_ready); mbar_arrive(stat_empty(s)); }
         }
-        if (ok && total) ok = warp_wait(done, 0, ab, 40);
+        // (keys that nobody sees still wait for their K and V: that memory is written below)
+        if (ok) ok = total ? warp_wait(done, 0, ab, 40) : warp_wait(kv_full, 0, ab, 40);
         if (ok) {
             // warpgroup 0 takes dV out of tensor memory, warpgroup 1 dK; keys that nobody sees get zero
             fence_after();
