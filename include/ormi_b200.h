@@ -411,7 +411,9 @@ int ormi_b200_set_option(ormi_b200_ctx* ctx, const char* key, const char* value)
  * for the device, copy to or from the host, or use the second stream (collectives) fail while a capture is open; the
  * replays read the inputs and write the results at the addresses the capture saw, so every pool block handed out during
  * the capture — results included — belongs to the graph until ormi_b200_graph_destroy: ormi_b200_free of one of them is
- * a no-op while the graph lives, and the results die with the graph.  Not with "pool_canary" on. */
+ * a no-op while the graph lives, and the results die with the graph.  A matmul that reads a bf16 copy the context keeps of an
+ * operand ("matmul" = "bf16") records no conversion: graph_launch converts the operand again where something has written it
+ * since, so replays multiply with what stands at the address.  Not with "pool_canary" on. */
 int ormi_b200_capture_begin(ormi_b200_ctx* ctx);
 int ormi_b200_capture_end(ormi_b200_ctx* ctx, void** out_graph);
 int ormi_b200_graph_launch(ormi_b200_ctx* ctx, void* graph);

@@ -527,9 +527,22 @@ int ormi_b200_set_option(ormi_b200_ctx* ctx, const char* key, const char* value)
 struct CapturedStep {
     cudaGraph_t graph = nullptr;
     cudaGraphExec_t exec = nullptr;
-    std::vector<std::pair<void*, size_t>> blocks;      // every pool block the step touched: owned until the graph is destroyed
+    std::vector<std::pair<void*, size_t>> blocks;      // every pool block the step touched: held until the graph is destroyed
     std::vector<std::pair<const void*, size_t>> writes;   // caller-owned memory that a replay writes
+    // bf16 copies of matmul operands in this graph's blocks: `reads` were made before the capture, so they have to be up to
+    // date when a replay begins; `leaves` are what the context may use after a replay (made or kept up to date by it)
+    std::vector<CopyOf> reads, leaves;
+    bool holds(const void* p) const {
+        for (auto& b : blocks) if ((const char*)p >= (const char*)b.first && (const char*)p < (const char*)b.first + b.second) return true;
+        return false;
+    }
 };
+
+// Whether the matrix at `src` went back to the pool: nothing is copied from there.
+static bool gone(ormi_b200_ctx* ctx, const void* src) {
+    std::lock_guard<std::mutex> lock(ctx->pool_mutex);
+    return ctx->pooled.count(const_cast<void*>(src)) != 0;
+}
 
 int ormi_b200_capture_begin(ormi_b200_ctx* ctx) {
     return guarded([&] {
@@ -541,6 +554,7 @@ int ormi_b200_capture_begin(ormi_b200_ctx* ctx) {
         ORMI_CUDA(cudaStreamBeginCapture(ctx->stream, cudaStreamCaptureModeThreadLocal));
         ctx->capture_blocks.clear();
         ctx->capture_writes.clear();
+        ctx->capture_reads.clear();
         ctx->capturing = true;
     });
 }
@@ -551,30 +565,46 @@ int ormi_b200_capture_end(ormi_b200_ctx* ctx, void** out_graph) {
         ORMI_CUDA(cudaSetDevice(ctx->device));
         if (!ctx->capturing) throw Error("ormi_b200_capture_end: no capture is open");
         ctx->capturing = false;
+        // copies whose conversion was recorded: it has not run
+        auto borrowed = [&](const void* src, const Shadow16& s) {
+            for (auto& r : ctx->capture_reads) if (r.src == src && r.copy.ptr == s.ptr) return true;
+            return false;
+        };
+        std::vector<CopyOf> unmade;
+        for (auto& kv : ctx->shadows) if (ctx->capture_blocks.count(kv.second.ptr) && !borrowed(kv.first, kv.second)) unmade.push_back({kv.first, kv.second});
         auto step = std::make_unique<CapturedStep>();
         cudaError_t e = cudaStreamEndCapture(ctx->stream, &step->graph);
         if (e == cudaSuccess) e = cudaGraphInstantiate(&step->exec, step->graph, 0);
         if (e != cudaSuccess) {
             cudaGetLastError();
             if (step->graph) cudaGraphDestroy(step->graph);
+            for (auto& c : unmade) shadow_drop(ctx, c.src, 1);
             ctx->capture_blocks.clear();
             throw Error(std::string("CUDA Error: ") + cudaGetErrorString(e) + " (ending the capture)");
         }
         // Every block the pool handed out during the capture is read or written by the replays: the graph owns them all
         // from here on.  Those that went back to the pool in the meantime are taken out of it again; freeing one of
         // the others (a result the caller holds) is a no-op while the graph lives.
-        std::lock_guard<std::mutex> lock(ctx->pool_mutex);
-        for (auto& kv : ctx->capture_blocks) {
-            step->blocks.push_back(kv);
-            ctx->graph_owned.insert(kv.first);
-            if (ctx->pooled.erase(kv.first)) {
-                auto& v = ctx->free_blocks[kv.second];
-                v.erase(std::remove(v.begin(), v.end(), kv.first), v.end());
+        {
+            std::lock_guard<std::mutex> lock(ctx->pool_mutex);
+            for (auto& kv : ctx->capture_blocks) {
+                step->blocks.push_back(kv);
+                ++ctx->graph_owned[kv.first];
+                if (ctx->pooled.erase(kv.first)) {
+                    auto& v = ctx->free_blocks[kv.second];
+                    v.erase(std::remove(v.begin(), v.end(), kv.first), v.end());
+                }
             }
         }
-        ctx->capture_blocks.clear();
+        for (auto& kv : ctx->shadows) if (ctx->capture_blocks.count(kv.second.ptr)) step->leaves.push_back({kv.first, kv.second});
         step->writes.swap(ctx->capture_writes);
+        step->reads.swap(ctx->capture_reads);
+        ctx->capture_blocks.clear();
         ctx->capture_writes.clear();
+        ctx->capture_reads.clear();
+        // a copy of a matrix from outside is good from here on (one of the graph's own results becomes so with the first replay)
+        for (auto& c : unmade)
+            if (!step->holds(c.src)) cvt_bf16(ctx, (const float*)c.src, c.copy.ld, c.copy.rows, c.copy.cols, c.copy.ptr);
         ctx->counters["captured_steps"]++;
         *out_graph = step.release();
     });
@@ -584,8 +614,23 @@ int ormi_b200_graph_launch(ormi_b200_ctx* ctx, void* graph) {
     return guarded([&] {
         bind(ctx, "ormi_b200_graph_launch");
         if (!graph) throw Error("ormi_b200_graph_launch: NULL graph");
-        ORMI_CUDA(cudaGraphLaunch(((CapturedStep*)graph)->exec, ctx->stream));
-        for (auto& w : ((CapturedStep*)graph)->writes) shadow_drop(ctx, w.first, w.second);
+        const CapturedStep& step = *(const CapturedStep*)graph;
+        // copies that the replay reads and that something has overtaken since: a write of the matrix, another graph's replay
+        for (auto& r : step.reads) {
+            auto it = ctx->shadows.find(r.src);
+            if ((it == ctx->shadows.end() || it->second.ptr != r.copy.ptr) && !gone(ctx, r.src))
+                cvt_bf16(ctx, (const float*)r.src, r.copy.ld, r.copy.rows, r.copy.cols, r.copy.ptr);
+        }
+        ORMI_CUDA(cudaGraphLaunch(step.exec, ctx->stream));
+        // what the replay overwrites: matrices that copies were made of, and copies in its blocks
+        for (auto& w : step.writes) shadow_drop(ctx, w.first, w.second);
+        for (auto& b : step.blocks) shadow_drop(ctx, b.first, b.second);
+        for (auto it = ctx->shadows.begin(); it != ctx->shadows.end();) it = step.holds(it->second.ptr) ? ctx->shadows.erase(it) : std::next(it);
+        for (auto& c : step.leaves) {
+            if (gone(ctx, c.src)) continue;
+            if (ctx->shadows.count(c.src)) shadow_drop(ctx, c.src, 1);
+            ctx->shadows[c.src] = c.copy;
+        }
         ctx->gemm_err_pending = true;
         ctx->counters["graph_launches"]++;
     });
@@ -600,15 +645,12 @@ int ormi_b200_graph_destroy(ormi_b200_ctx* ctx, void* graph) {
         cudaGraphDestroy(step->graph);
         {
             std::lock_guard<std::mutex> lock(ctx->pool_mutex);
-            for (auto& b : step->blocks) ctx->graph_owned.erase(b.first);
+            for (auto& b : step->blocks) if (--ctx->graph_owned[b.first] <= 0) ctx->graph_owned.erase(b.first);
         }
         // bf16 twins that live in the graph's blocks go with them; the blocks return to the pool behind the replays
-        // already queued on the compute stream
-        for (auto it = ctx->shadows.begin(); it != ctx->shadows.end();) {
-            bool mine = false;
-            for (auto& b : step->blocks) if (b.first == it->second.ptr) mine = true;
-            it = mine ? ctx->shadows.erase(it) : std::next(it);
-        }
+        // already queued on the compute stream.  What another graph holds too stays with that one.
+        for (auto it = ctx->shadows.begin(); it != ctx->shadows.end();)
+            it = step->holds(it->second.ptr) && !ctx->graph_owned.count(it->second.ptr) ? ctx->shadows.erase(it) : std::next(it);
         for (auto& b : step->blocks) pool_free(ctx, b.first, b.second);
     });
 }

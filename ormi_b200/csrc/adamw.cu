@@ -331,19 +331,18 @@ void launch(ormi_b200_ctx* ctx, Batch<N>& b, int chunks, int state_bits) {
 }
 
 // The context's bf16 copy of `param` when it is a plain copy of exactly these n values (it is rewritten along with them);
-// any other copy that overlaps is stale and goes.  A captured step keeps rewriting the copy on every replay, so the
-// copy's block stays with the graph.
+// any other copy that overlaps is stale and goes.  A captured step keeps rewriting the copy on every replay, so its graph
+// holds the copy's block.
 void* kept_copy(ormi_b200_ctx* ctx, const ormi_b200_adamw_tensor& t) {
     if (ctx->shadows.empty()) return nullptr;
     auto it = ctx->shadows.find(t.param);
-    // (a copy that already belongs to another captured step is not shared with this one)
-    const bool whole = it != ctx->shadows.end() && !(ctx->capturing && ctx->graph_owned.count(it->second.ptr)) && it->second.ld == it->second.cols && (int64_t)it->second.rows * it->second.cols == t.n;
+    const bool whole = it != ctx->shadows.end() && it->second.ld == it->second.cols && (int64_t)it->second.rows * it->second.cols == t.n;
     if (!whole || t.copy16) { shadow_drop(ctx, t.param, (size_t)t.n * 4); return nullptr; }
     const Shadow16 keep = it->second;
     ctx->shadows.erase(it);
     shadow_drop(ctx, t.param, (size_t)t.n * 4);
     ctx->shadows[t.param] = keep;
-    if (ctx->capturing) ctx->capture_blocks[keep.ptr] = keep.bytes;
+    shadow_borrow(ctx, t.param, keep);
     return keep.ptr;
 }
 

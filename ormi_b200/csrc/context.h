@@ -78,6 +78,8 @@ struct Shadow16 {
     long long ld = 0;
 };
 
+struct CopyOf { const void* src; Shadow16 copy; };   // a bf16 copy and the fp32 matrix it belongs to
+
 struct TcKernel { CompiledKernel* kernel = nullptr; int block = 0, smem = 0; };
 
 // Generated epilogue of the run-time compiled tensor-core GEMM: text spliced into the kernel template plus the
@@ -110,8 +112,9 @@ struct ormi_b200_ctx {
     bool auto_graph = true;                // option "auto_graph": realize replays a plan's launches as a CUDA graph when the addresses repeat
     bool capturing = false;
     std::unordered_map<void*, size_t> capture_blocks;
-    std::unordered_set<void*> graph_owned;
+    std::unordered_map<void*, int> graph_owned;                   // block -> live graphs that hold it
     std::vector<std::pair<const void*, size_t>> capture_writes;   // caller-owned memory the captured operators write: bf16 copies of it are stale after a replay
+    std::vector<ormi_b200::CopyOf> capture_reads;                 // bf16 copies from before the capture that the captured calls use
     bool pool_canary = false;              // option "pool_canary": a guard zone behind every block, checked when the block comes back
     std::unordered_map<void*, size_t> canaries;   // block -> bytes asked for, of the blocks that carry a guard zone
     std::unordered_set<void*> pooled;      // every block that sits in free_blocks: a block returned twice is caught, not handed to two owners
@@ -182,6 +185,7 @@ const void* shadow_of(ormi_b200_ctx* ctx, const float* src, int rows, int cols, 
 const void* shadow_find(ormi_b200_ctx* ctx, const void* src, int rows, int cols, long long ld);
 void shadow_register(ormi_b200_ctx* ctx, const void* src, void* p16, int rows, int cols, long long ld);
 void shadow_drop(ormi_b200_ctx* ctx, const void* ptr, size_t bytes);
+void shadow_borrow(ormi_b200_ctx* ctx, const void* src, const Shadow16& copy);
 
 // collectives (comm.cu)
 void comm_unique_id(char* out128);

@@ -154,8 +154,20 @@ const void* shadow_find(ormi_b200_ctx* ctx, const void* src, int rows, int cols,
     return (same || flat) ? s.ptr : nullptr;
 }
 
+// A captured call that uses a copy from before the capture: no conversion is recorded, so the graph holds the copy's block and
+// ormi_b200_graph_launch sees to it that it is the matrix's copy when the replay begins.
+void shadow_borrow(ormi_b200_ctx* ctx, const void* src, const Shadow16& copy) {
+    if (!ctx->capturing) return;
+    std::lock_guard<std::mutex> lock(ctx->pool_mutex);
+    if (ctx->capture_blocks.emplace(copy.ptr, copy.bytes).second) ctx->capture_reads.push_back({src, copy});
+}
+
 const void* shadow_of(ormi_b200_ctx* ctx, const float* src, int rows, int cols, long long ld) {
-    if (const void* p = shadow_find(ctx, src, rows, cols, ld)) { ctx->counters["shadow_hits"]++; return p; }
+    if (const void* p = shadow_find(ctx, src, rows, cols, ld)) {
+        shadow_borrow(ctx, src, ctx->shadows.find(src)->second);
+        ctx->counters["shadow_hits"]++;
+        return p;
+    }
     void* p16 = pool_alloc(ctx, (size_t)rows * cols * 2);
     try { cvt_bf16(ctx, src, ld, rows, cols, p16); }
     catch (...) { pool_free(ctx, p16, (size_t)rows * cols * 2); throw; }

@@ -1,8 +1,13 @@
 """Transformer-block operators at the edges of what their documentation allows."""
+import ctypes
+
 import pytest
 
+from ormi_b200 import graph as G
 from ormi_b200 import ops
-from test_transformer_ops import BF, done, gpu, ints, randn, torch
+from ormi_b200 import workloads as W
+from ormi_b200._lib import check, lib
+from test_transformer_ops import ACC, BF, F8, done, gpu, ints, no_guard_zones, randn, torch
 
 
 # ---- attention
@@ -53,3 +58,162 @@ def test_attention_gradients_of_keys_that_nobody_sees(device, mask, d, b, nk, h,
         if seen is None:
             seen = [x.clone() for x in grads]
         assert all(torch.equal(x, y) for x, y in zip(grads, seen)), f"call {turn} differs from the first"
+
+
+# ---- captured steps over weights that have a bf16 copy
+
+class Steps:
+    """A context in "bf16" arithmetic with y = x w (the products read bf16 copies that the context keeps of x and w) and an
+    optimizer of w.  `check` compares y with the product of the weights as they stood before the call."""
+    N = 128                                                     # the smallest cube that takes the path with copies
+
+    def __init__(self):
+        from ormi_b200.runtime import Device
+        self.dev = Device(0)
+        self.dev.set_option("matmul", "bf16")
+        n = self.N
+        self.x, self.w, self.g = (ops.upload(self.dev, W.normal(seed, (n, n))) for seed in (1, 2, 3))
+        self.y, self.z = ops.empty(self.dev, (n, n)), ops.empty(self.dev, (n, n))
+        self.opt = ops.AdamW(self.dev, [self.w], [self.g], [ops.zeros(self.dev, (n, n))], [ops.zeros(self.dev, (n, n))], betas=(0.0, 0.0))
+        self.count = ops.zeros(self.dev, (2,), "i32")           # a 64-bit counter
+
+    def product(self, y=None, w=None):
+        n = self.N
+        dims, strides = (ctypes.c_int32 * 2)(n, n), (ctypes.c_int32 * 2)(n, 1)
+        check(lib.ormi_b200_matmul(self.dev.handle, self.x.ptr, 2, dims, strides, (w or self.w).ptr, 2, dims, strides, (y or self.y).ptr, 2, dims))
+
+    def update(self):
+        """Every weight moves by about 1 (betas of 0: the update is lr times the gradient's sign)."""
+        self.opt.step(lr=1.0, device_step=self.count.ptr)
+
+    def put(self, seed):
+        self.dev.h2d(self.w.ptr, W.normal(seed, (self.N, self.N)))
+
+    def check(self, what, call, y=None):
+        y = y or self.y
+        rounded = lambda a: torch.from_numpy(a.numpy()).to(BF).to(F8)      # noqa: E731
+        x, w = rounded(self.x), rounded(self.w)
+        check(lib.ormi_b200_memset(self.dev.handle, y.ptr, 0, y.nbytes))
+        call()
+        got = torch.from_numpy(y.numpy()).to(F8)
+        bound = ACC * (self.N + 4) * (x.abs() @ w.abs())        # fp32 sums of exact products
+        assert bool(((got - x @ w).abs() <= bound).all()), f"{what}: y is not the product of the weights, off by {float((got - x @ w).abs().max()):.3g}"
+
+
+@pytest.fixture
+def steps():
+    s = Steps()
+    yield s
+    s.dev.close()
+
+
+def outside(s):
+    """Ways in which a weight changes between two replays."""
+    other = ops.upload(s.dev, W.normal(77, (s.N, s.N)))
+    return [("nothing", lambda: None), ("an update", s.update), ("an upload", lambda: s.put(50)), ("a copy", lambda: check(lib.ormi_b200_memcpy_d2d(s.dev.handle, s.w.ptr, other.ptr, other.nbytes))),
+            ("an upload and an update", lambda: (s.put(51), s.update())), ("an upload and a product", lambda: (s.put(52), s.product(s.z))), ("nothing again", lambda: None)]
+
+
+@gpu
+@no_guard_zones
+@pytest.mark.parametrize("trains", [False, True])
+def test_captured_product_follows_its_weights(steps, trains):
+    """A replay multiplies with the weights as they are, whatever changed them; and so does a plain product after a replay."""
+    s = steps
+
+    def step():
+        s.product()
+        if trains:
+            s.update()
+    s.check("plain", step)
+    with s.dev.capture() as one:
+        step()
+    for what, change in outside(s):
+        change()
+        s.check(f"replay after {what}", one.launch)
+        s.check(f"replay after a replay after {what}", one.launch)
+        s.check(f"product after {what} and a replay", s.product)
+        s.check(f"product again after {what}", s.product)
+    one.destroy()
+    s.check("product after the graph", s.product)
+    s.check("step after the graph", step)
+
+
+@gpu
+@no_guard_zones
+@pytest.mark.parametrize("first, second", [("both", "both"), ("both", "product"), ("product", "both"), ("product", "update"), ("update", "product")])
+def test_two_captured_steps_share_their_weights(steps, first, second):
+    s = steps
+    parts = {"both": lambda: (s.product(), s.update()), "product": s.product, "update": s.update}
+    s.check("plain", parts["both"])
+    with s.dev.capture() as one:
+        parts[first]()
+    with s.dev.capture() as two:
+        parts[second]()
+    graphs = [(g, name != "update") for g, name in ((one, first), (two, second))]
+
+    def run(order):
+        for i in order:
+            g, multiplies = graphs[i]
+            if multiplies:
+                s.check(f"graph {i} of {order}", g.launch)
+            else:
+                g.launch()
+    run([0, 0, 1, 1, 0, 1])
+    for what, change in outside(s):
+        change()
+        run([1, 0, 1])
+        s.check(f"product after {what}", s.product)
+    one.destroy()                                               # the second one's copies stay its own
+    junk = [ops.zeros(s.dev, (s.N, s.N), "bf16") for _ in range(6)]
+    for j in junk:
+        check(lib.ormi_b200_memset(s.dev.handle, j.ptr, 0x55, j.nbytes))
+    graphs[0] = (two, second != "update")
+    run([1, 0])
+    s.put(60)
+    run([1, 1])
+    two.destroy()
+    s.check("product after both", s.product)
+
+
+@gpu
+@no_guard_zones
+def test_a_copy_that_a_capture_recorded_is_not_taken_for_made(steps):
+    """The weight's copy is dropped before the capture, so its conversion is recorded: a plain product between the capture and the
+    first replay does not read a copy that nothing has written yet."""
+    s = steps
+    s.check("plain", s.product)
+    s.put(40)
+    with s.dev.capture() as one:
+        s.product(s.z)
+    s.check("product before the first replay", s.product)
+    s.put(41)
+    s.check("replay", one.launch, s.z)
+    s.check("product", s.product)
+    one.destroy()
+
+
+@gpu
+@no_guard_zones
+def test_results_of_a_captured_realize_are_multiplied_as_they_are(steps):
+    """A plain product with a captured result as its weight makes a copy of it, which the next replay overtakes."""
+    s = steps
+    a = s.dev.leaf(W.normal(20, (s.N, s.N)))
+    for _ in range(2):
+        kept = G.add(a, a)
+        s.dev.realize([kept])
+        del kept
+    with s.dev.capture() as one:
+        kept = G.add(a, a)
+        s.dev.realize([kept])
+    for seed in (21, 22, 23):
+        s.dev.h2d(a.data.dev_ptr, W.normal(seed, (s.N, s.N)))
+        one.launch()
+        s.w, w = ops.view(kept.data.dev_ptr, (s.N, s.N)), s.w
+        want = torch.from_numpy(2 * W.normal(seed, (s.N, s.N))).to(BF).to(F8)
+        x = torch.from_numpy(s.x.numpy()).to(BF).to(F8)
+        s.product()
+        s.w = w
+        got = torch.from_numpy(s.y.numpy()).to(F8)
+        assert bool(((got - x @ want).abs() <= ACC * (s.N + 4) * (x.abs() @ want.abs())).all()), seed
+    one.destroy()
