@@ -119,11 +119,11 @@ int ormi_b200_trim(ormi_b200_ctx* ctx) {
 }
 
 int ormi_b200_memset(ormi_b200_ctx* ctx, void* ptr, int value, size_t bytes) {
-    return guarded([&] { bind(ctx, "ormi_b200_memset", true); shadow_drop(ctx, ptr, bytes); ORMI_CUDA(cudaMemsetAsync(ptr, value, bytes, ctx->stream)); });
+    return guarded([&] { bind(ctx, "ormi_b200_memset", true); written(ctx, ptr, bytes); ORMI_CUDA(cudaMemsetAsync(ptr, value, bytes, ctx->stream)); });
 }
 
 int ormi_b200_memcpy_d2d(ormi_b200_ctx* ctx, void* dst, const void* src, size_t bytes) {
-    return guarded([&] { bind(ctx, "ormi_b200_memcpy_d2d", true); shadow_drop(ctx, dst, bytes); ORMI_CUDA(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyDeviceToDevice, ctx->stream)); });
+    return guarded([&] { bind(ctx, "ormi_b200_memcpy_d2d", true); written(ctx, dst, bytes); ORMI_CUDA(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyDeviceToDevice, ctx->stream)); });
 }
 
 int ormi_b200_memcpy_h2d(ormi_b200_ctx* ctx, void* dst, const void* src, size_t bytes) {
@@ -218,7 +218,7 @@ int ormi_b200_fill_u32(ormi_b200_ctx* ctx, void* dst, uint32_t pattern, size_t c
     return guarded([&] {
         bind(ctx, "ormi_b200_fill_u32", true);
         if (count == 0) return;
-        shadow_drop(ctx, dst, count * 4);
+        written(ctx, dst, count * 4);
         int grid = (int)std::min<size_t>((count + 255) / 256, (size_t)ctx->num_sms * 8);
         fill_u32_kernel<<<grid, 256, 0, ctx->stream>>>((uint32_t*)dst, pattern, count);
         ORMI_CUDA(cudaGetLastError());
@@ -226,7 +226,7 @@ int ormi_b200_fill_u32(ormi_b200_ctx* ctx, void* dst, uint32_t pattern, size_t c
 }
 
 int ormi_b200_fill_u8(ormi_b200_ctx* ctx, void* dst, uint8_t pattern, size_t count) {
-    return guarded([&] { bind(ctx, "ormi_b200_fill_u8", true); shadow_drop(ctx, dst, count); ORMI_CUDA(cudaMemsetAsync(dst, pattern, count, ctx->stream)); });
+    return guarded([&] { bind(ctx, "ormi_b200_fill_u8", true); written(ctx, dst, count); ORMI_CUDA(cudaMemsetAsync(dst, pattern, count, ctx->stream)); });
 }
 
 int ormi_b200_sync(ormi_b200_ctx* ctx) {
@@ -366,6 +366,7 @@ int ormi_b200_gemm_bf16_kmajor(ormi_b200_ctx* ctx, const void* a16, const void* 
     return guarded([&] {
         need(a16 && b16 && C, "ormi_b200_gemm_bf16_kmajor: NULL argument");
         bind(ctx, "ormi_b200_gemm_bf16_kmajor", true);
+        if (M > 0 && N > 0) written(ctx, C, (size_t)M * N * 4);
         gemm_bf16_kmajor(ctx, a16, b16, C, M, N, Kp);
     });
 }
@@ -383,7 +384,7 @@ int ormi_b200_gemm_bf16(ormi_b200_ctx* ctx, const void* a16, int a_transposed, c
     return guarded([&] {
         need(a16 && b16 && C, "ormi_b200_gemm_bf16: NULL argument");
         bind(ctx, "ormi_b200_gemm_bf16", true);
-        shadow_drop(ctx, C, (size_t)M * N * 4);
+        written(ctx, C, (size_t)M * N * 4);
         gemm_tc(ctx, a16, a_transposed ? 1 : 0, b16, b_transposed ? 0 : 1, C, M, N, K);
     });
 }
@@ -451,6 +452,7 @@ int ormi_b200_allreduce_sum_f32(ormi_b200_ctx* ctx, void* const* buffers, const 
     return guarded([&] {
         need(buffers && counts && n > 0, "ormi_b200_allreduce_sum_f32: bad arguments");
         bind(ctx, "ormi_b200_allreduce_sum_f32");
+        for (int i = 0; i < n; ++i) written(ctx, buffers[i], counts[i] * 4);
         comm_allreduce(ctx, buffers, counts, n, overlap);
     });
 }

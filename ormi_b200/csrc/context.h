@@ -113,7 +113,7 @@ struct ormi_b200_ctx {
     bool capturing = false;
     std::unordered_map<void*, size_t> capture_blocks;
     std::unordered_map<void*, int> graph_owned;                   // block -> live graphs that hold it
-    std::vector<std::pair<const void*, size_t>> capture_writes;   // caller-owned memory the captured operators write: bf16 copies of it are stale after a replay
+    std::vector<std::pair<const void*, size_t>> capture_writes;   // caller-owned memory the captured calls write: bf16 copies of it are stale after a replay
     std::vector<ormi_b200::CopyOf> capture_reads;                 // bf16 copies from before the capture that the captured calls use
     bool pool_canary = false;              // option "pool_canary": a guard zone behind every block, checked when the block comes back
     std::unordered_map<void*, size_t> canaries;   // block -> bytes asked for, of the blocks that carry a guard zone
@@ -186,6 +186,7 @@ const void* shadow_find(ormi_b200_ctx* ctx, const void* src, int rows, int cols,
 void shadow_register(ormi_b200_ctx* ctx, const void* src, void* p16, int rows, int cols, long long ld);
 void shadow_drop(ormi_b200_ctx* ctx, const void* ptr, size_t bytes);
 void shadow_borrow(ormi_b200_ctx* ctx, const void* src, const Shadow16& copy);
+void written(ormi_b200_ctx* ctx, const void* ptr, size_t bytes);
 
 // collectives (comm.cu)
 void comm_unique_id(char* out128);

@@ -162,6 +162,14 @@ void shadow_borrow(ormi_b200_ctx* ctx, const void* src, const Shadow16& copy) {
     if (ctx->capture_blocks.emplace(copy.ptr, copy.bytes).second) ctx->capture_reads.push_back({src, copy});
 }
 
+// A result written through a raw pointer: a bf16 copy kept of that buffer is stale from here on, and again after every
+// replay of a captured call.
+void written(ormi_b200_ctx* ctx, const void* ptr, size_t bytes) {
+    if (!ptr || !bytes) return;
+    shadow_drop(ctx, ptr, bytes);
+    if (ctx->capturing) ctx->capture_writes.push_back({ptr, bytes});
+}
+
 const void* shadow_of(ormi_b200_ctx* ctx, const float* src, int rows, int cols, long long ld) {
     if (const void* p = shadow_find(ctx, src, rows, cols, ld)) {
         shadow_borrow(ctx, src, ctx->shadows.find(src)->second);

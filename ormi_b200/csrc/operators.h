@@ -99,13 +99,6 @@ struct Scratch {
     ~Scratch() { try { release(); } catch (...) {} }
 };
 
-// A result written through a raw pointer: a bf16 copy kept of that buffer is stale from here on, and again after every
-// replay of a captured call.
-inline void written(ormi_b200_ctx* ctx, const void* p, size_t bytes) {
-    if (!p || !bytes) return;
-    shadow_drop(ctx, p, bytes);
-    if (ctx->capturing) ctx->capture_writes.push_back({p, bytes});
-}
 inline void written(ormi_b200_ctx* ctx, const ormi_b200_view& v) {
     if (!v.data) return;
     const Span s = span_of(v);

@@ -351,7 +351,7 @@ void realize(ormi_b200_ctx* ctx, ormi_b200_node* nodes, int n_nodes, const int* 
                 handed[b] = true;      // not a pool block
             } else {
                 if (preassigned && pb.kind == BufKind::NodeOut)
-                    for (auto& pr : *preassigned) if (pr.first == pb.node) { bufs[b] = pr.second; handed[b] = true; }
+                    for (auto& pr : *preassigned) if (pr.first == pb.node) { bufs[b] = pr.second; handed[b] = true; written(ctx, pr.second, (size_t)pb.bytes); }
                 if (!bufs[b] && cp->first_use[b] < 0) bufs[b] = pool_alloc(ctx, (size_t)pb.bytes);   // scratch comes later
             }
         }

@@ -1,6 +1,7 @@
 """Transformer-block operators at the edges of what their documentation allows."""
 import ctypes
 
+import numpy as np
 import pytest
 
 from ormi_b200 import graph as G
@@ -195,6 +196,22 @@ def test_a_copy_that_a_capture_recorded_is_not_taken_for_made(steps):
 
 @gpu
 @no_guard_zones
+def test_writes_inside_a_capture_make_copies_stale_at_every_replay(steps):
+    """A captured fill of the weight: copies that plain products made between two replays are not used after the second."""
+    s = steps
+    s.check("plain", s.product)
+    with s.dev.capture() as one:
+        check(lib.ormi_b200_fill_u32(s.dev.handle, s.w.ptr, int(np.float32(0.5).view(np.uint32)), s.N * s.N))
+    for seed in (30, 31):
+        s.put(seed)
+        s.check("product between", s.product)
+        one.launch()
+        s.check("product after the fill", s.product)
+    one.destroy()
+
+
+@gpu
+@no_guard_zones
 def test_results_of_a_captured_realize_are_multiplied_as_they_are(steps):
     """A plain product with a captured result as its weight makes a copy of it, which the next replay overtakes."""
     s = steps
@@ -217,3 +234,27 @@ def test_results_of_a_captured_realize_are_multiplied_as_they_are(steps):
         got = torch.from_numpy(s.y.numpy()).to(F8)
         assert bool(((got - x @ want).abs() <= ACC * (s.N + 4) * (x.abs() @ want.abs())).all()), seed
     one.destroy()
+
+
+@gpu
+@pytest.mark.parametrize("writer", ["matmul", "sum", "gemm_bf16", "gemm_bf16_kmajor", "memset", "copy"])
+def test_raw_results_make_the_copies_of_their_buffer_stale(steps, writer):
+    """A buffer that was multiplied with (so that the context has a bf16 copy of it) is written by a raw call and multiplied with again."""
+    s, n = steps, steps.N
+    two, one = (ctypes.c_int32 * 2)(n, n), (ctypes.c_int32 * 1)(0)
+    many = ops.upload(s.dev, W.normal(9, (2, n, n)))
+    half = [ops.upload(s.dev, W.normal(seed, (n, n)), "bf16") for seed in (4, 5)]
+    shape3, strides3 = (ctypes.c_int32 * 3)(2, n, n), (ctypes.c_int32 * 3)(n * n, n, 1)
+    calls = {
+        "matmul": lambda: lib.ormi_b200_matmul(s.dev.handle, s.x.ptr, 2, two, (ctypes.c_int32 * 2)(n, 1), s.g.ptr, 2, two, (ctypes.c_int32 * 2)(n, 1), s.w.ptr, 2, two),
+        "sum": lambda: lib.ormi_b200_sum(s.dev.handle, many.ptr, 3, shape3, strides3, one, 1, s.w.ptr),
+        "gemm_bf16": lambda: lib.ormi_b200_gemm_bf16(s.dev.handle, half[0].ptr, 0, half[1].ptr, 0, s.w.ptr, n, n, n),
+        "gemm_bf16_kmajor": lambda: lib.ormi_b200_gemm_bf16_kmajor(s.dev.handle, half[0].ptr, half[1].ptr, s.w.ptr, n, n, n),
+        "memset": lambda: lib.ormi_b200_memset(s.dev.handle, s.w.ptr, 0x3f, s.w.nbytes),
+        "copy": lambda: lib.ormi_b200_memcpy_d2d(s.dev.handle, s.w.ptr, s.g.ptr, s.w.nbytes),
+    }
+    before = s.w.numpy()
+    s.check("before", s.product)
+    check(calls[writer]())
+    assert np.abs(s.w.numpy() - before).max() > 0.5
+    s.check(f"after {writer}", s.product)
