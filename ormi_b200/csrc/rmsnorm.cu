@@ -27,6 +27,10 @@ __device__ __forceinline__ float weight_at(const void* w, int f32, int c) {
     return !w ? 1.f : f32 ? ((const float*)w)[c] : __bfloat162float(((const bf16*)w)[c]);
 }
 
+// The factor 448 / top of a group of e4m3 codes leaves fp32 below 1.3e-36: a smaller group is lifted by 2^64 first (exact).
+__device__ __forceinline__ float lift_of(float top) { return top < 0x1p-100f ? 0x1p64f : 1.f; }
+__device__ __forceinline__ float codes_per_unit(float top, float lift) { return top > 0.f ? 448.f * (1.f / (top * lift)) : 0.f; }
+
 // One block per row, any width, any alignment (rows too wide for norm_row): three passes over the row (four with one scale for the row), the second
 // and later ones out of the caches.  Each element is handled by the same thread in every pass, so `out` and
 // `residual_out` may be the inputs.
@@ -55,9 +59,9 @@ __global__ void __launch_bounds__(256) norm_any(NormParams p) {
             uint32_t m = 0;
             for (int c = threadIdx.x; c < p.cols; c += blockDim.x) m = max(m, mag(y(c)));
             const float top = block_max_mag(m, (uint32_t*)box);
-            const float up = top > 0.f ? 448.f * (1.f / top) : 0.f;
+            const float lift = lift_of(top), up = codes_per_unit(top, lift);
             if (threadIdx.x == 0) p.scales[row] = top * (1.f / 448.f);
-            for (int c = threadIdx.x; c < p.cols; c += blockDim.x) out[c] = from_f32<O>(y(c) * up);
+            for (int c = threadIdx.x; c < p.cols; c += blockDim.x) out[c] = from_f32<O>(y(c) * lift * up);
         } else {
             // a warp per group of 128 columns
             const int lane = threadIdx.x & 31;
@@ -70,11 +74,11 @@ __global__ void __launch_bounds__(256) norm_any(NormParams p) {
                     m = max(m, mag(v[k]));
                 }
                 const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, m));
-                const float up = top > 0.f ? 448.f * (1.f / top) : 0.f;
+                const float lift = lift_of(top), up = codes_per_unit(top, lift);
                 if (lane == 0) p.scales[row * p.groups + g] = top * (1.f / 448.f);
                 for (int k = 0; k < 4; ++k) {
                     const int c = g * 128 + k * 32 + lane;
-                    if (c < p.cols) out[c] = from_f32<O>(v[k] * up);
+                    if (c < p.cols) out[c] = from_f32<O>(v[k] * lift * up);
                 }
             }
         }
@@ -216,8 +220,14 @@ __global__ void __launch_bounds__(WARP_ROW ? 256 : 1024) norm_row(NormParams p) 
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) m = max(m, mag(s[v][e]));
             const float top = WARP_ROW ? __uint_as_float(__reduce_max_sync(0xffffffffu, m)) : block_max_mag(m, (uint32_t*)box);
-            const float up = top > 0.f ? 448.f * (1.f / top) : 0.f;
+            const float lift = lift_of(top), up = codes_per_unit(top, lift);
             if ((WARP_ROW ? (threadIdx.x & 31) : threadIdx.x) == 0) p.scales[row] = top * (1.f / 448.f);
+            if (lift != 1.f) {
+#pragma unroll
+                for (int v = 0; v < NV; ++v)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) s[v][e] *= lift;
+            }
 #pragma unroll
             for (int v = 0; v < NV; ++v)
 #pragma unroll
@@ -231,8 +241,12 @@ __global__ void __launch_bounds__(WARP_ROW ? 256 : 1024) norm_row(NormParams p) 
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) m = max(m, mag(s[v][e]));
                 const float top = __uint_as_float(__reduce_max_sync(half, m));
-                const float up = top > 0.f ? 448.f * (1.f / top) : 0.f;
+                const float lift = lift_of(top), up = codes_per_unit(top, lift);
                 if ((threadIdx.x & (VEC == 8 ? 15 : 31)) == 0 && c0[v] < p.cols) p.scales[row * p.groups + c0[v] / 128] = top * (1.f / 448.f);
+                if (lift != 1.f) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) s[v][e] *= lift;
+                }
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) s[v][e] *= up;
             }

@@ -8,7 +8,7 @@ from ormi_b200 import graph as G
 from ormi_b200 import ops
 from ormi_b200 import workloads as W
 from ormi_b200._lib import check, lib
-from test_transformer_ops import ACC, BF, F8, done, gpu, ints, no_guard_zones, randn, torch
+from test_transformer_ops import ACC, BF, F8, FP, done, gpu, ints, no_guard_zones, randn, torch
 
 
 # ---- attention
@@ -59,6 +59,38 @@ def test_attention_gradients_of_keys_that_nobody_sees(device, mask, d, b, nk, h,
         if seen is None:
             seen = [x.clone() for x in grads]
         assert all(torch.equal(x, y) for x, y in zip(grads, seen)), f"call {turn} differs from the first"
+
+
+# ---- RMS norm
+
+@gpu
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("cols", [100, 256, 1111, 4096, 40000])
+@pytest.mark.parametrize("group", [0, 128])
+def test_norm_to_eight_bits_of_tiny_groups(device, dtype, cols, group):
+    """Maxima down to 1e-39, where 448 / maximum is not an fp32 number: codes follow the values, zeros stay zeros."""
+    sizes = [1e-30, 3e-36, 1e-37, 2e-39]
+    x = randn(len(sizes) + 1, cols, seed=5).to(F8) * torch.tensor([*sizes, 0.0], dtype=F8, device="cuda")[:, None]     # (and a row of zeros)
+    x[:, ::3] = 0.0
+    x = x.to(dtype)
+    # rstd = 1 / sqrt(eps) = 2^10 exactly, since s^2 vanishes against eps, and the weight takes that back
+    weight, groups = torch.full((cols,), 2.0 ** -10, device="cuda"), 1 if not group else -(-cols // group)
+    out, scales = torch.empty(x.shape, device="cuda", dtype=torch.float8_e4m3fn), torch.empty(len(x), groups, device="cuda")
+    torch.cuda.synchronize()
+    ops.rmsnorm(device, x, weight, out, scales=scales, group=group, eps=2.0 ** -20)
+    done(device)
+    y = torch.nn.functional.pad(x.to(F8), (0, groups * (group or cols) - cols)).view(len(x), groups, -1)
+    got = torch.nn.functional.pad(out.to(F8), (0, groups * (group or cols) - cols)).view(len(x), groups, -1)
+    top = y.abs().amax(-1, keepdim=True)
+    # y may be off by half of the smallest fp32 number, and relatively by a few roundings
+    off = (2.0 ** -149 + 2.0 ** -20 * y.abs()) * torch.where(top > 0, 448 / top, 0.0)
+    want = y * torch.where(top > 0, 448 / top, 0.0)
+    # half a step of e4m3: 2^-4 of the value, 2^-10 below 2^-6
+    bound = (want.abs() * 2.0 ** -4).clamp_min(2.0 ** -10) + 2 * off
+    assert bool(torch.isfinite(got).all())
+    assert bool(((got - want).abs() <= bound).all())
+    assert bool((got[y == 0] == 0).all())
+    assert bool(((scales.to(F8) - top[..., 0] / 448).abs() <= 2.0 ** -149 + 2.0 ** -22 * top[..., 0] / 448).all())
 
 
 # ---- captured steps over weights that have a bf16 copy
