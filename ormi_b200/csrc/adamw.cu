@@ -185,8 +185,14 @@ __device__ __forceinline__ void step_block(const Common& c, const Rates& r, floa
     }
     hi_m = __uint_as_float(__reduce_max_sync(0xffffffffu, top_m));
     hi_v = __uint_as_float(__reduce_max_sync(0xffffffffu, top_v));
-    // codes per unit, 448 / top: one half of the warp divides for m, the other for sqrt(v)
-    const float mine = threadIdx.x & 16 ? hi_v : hi_m, up = mine > 0.f ? __fmul_rn(1.f / mine, 448.f) : 0.f;
+    // codes per unit, 448 / top: one half of the warp divides for m, the other for sqrt(v).  Below 1.3e-36 that leaves fp32 (only
+    // m gets there: the root of the smallest v is 3.7e-23), so a small m is lifted by 2^64 first, which is exact.
+    float top = hi_m;
+    if (hi_m < 0x1p-100f) {
+        top *= 0x1p64f;
+        m[0] = mul2(m[0], both(0x1p64f)); m[1] = mul2(m[1], both(0x1p64f));
+    }
+    const float mine = threadIdx.x & 16 ? hi_v : top, up = mine > 0.f ? __fmul_rn(1.f / mine, 448.f) : 0.f;
     const float2 up_m = both(__shfl_sync(0xffffffffu, up, 0)), up_v = both(__shfl_sync(0xffffffffu, up, 16));
     uint32_t a[4], b[4], least = 0xffffffffu;
 #pragma unroll

@@ -93,6 +93,33 @@ def test_norm_to_eight_bits_of_tiny_groups(device, dtype, cols, group):
     assert bool(((scales.to(F8) - top[..., 0] / 448).abs() <= 2.0 ** -149 + 2.0 ** -22 * top[..., 0] / 448).all())
 
 
+# ---- AdamW
+
+@gpu
+@pytest.mark.parametrize("size", [1e-30, 1e-35, 1e-37])
+def test_adamw_8_bit_states_of_tiny_gradients(device, size):
+    """m far below 1e-36, where 448 / maximum is not an fp32 number: what was zero stays zero, the rest keeps its size.  9000 elements:
+    two whole chunks and a part of one."""
+    n, b1 = 9000, 0.75
+    g = randn(n, seed=6) * size
+    g[::3] = 0.0
+    p, m, v = torch.zeros(n, device="cuda"), *(torch.zeros(n, device="cuda").to(torch.float8_e4m3fn) for _ in range(2))
+    scales = [torch.zeros(-(-n // 128), device="cuda") for _ in range(2)]
+    opt = ops.AdamW(device, [p], [g], [m], [v], m_scales=[scales[0]], v_scales=[scales[1]], betas=(b1, 0.9))
+    torch.cuda.synchronize()
+    opt.step(lr=0.1)
+    done(device)
+    want = (1 - b1) * g.to(F8)
+    tops = torch.nn.functional.pad(want, (0, -n % 128)).view(-1, 128).abs().amax(1)
+    top = tops.repeat_interleave(128)[:n]
+    got = m.to(F8) * scales[0].to(F8).repeat_interleave(128)[:n]
+    # rounded up or down by less than a step: 2^-3 of the value, 2^-9 of a code below 2^-6; codes are at most 448, and a
+    # scale (or an m) may be off by the smallest fp32 number
+    bound = torch.maximum(want.abs() * 2.0 ** -3, 2.0 ** -9 * top / 448) * 1.01 + 450 * 2.0 ** -149 + 2.0 ** -20 * top
+    assert bool(torch.isfinite(m.to(F8)).all()) and bool((m.to(F8)[::3] == 0).all())
+    assert bool(((got - want).abs() <= bound).all())
+
+
 # ---- captured steps over weights that have a bf16 copy
 
 class Steps:
