@@ -292,11 +292,13 @@ class AdamW:
                     raise ValueError(f"tensor {i}: the gradient has another type or size, or is not contiguous")
                 struct.pack_into("=Q", blob, i * _ADAM_TENSOR.size + 8, ptr)
             blob = bytes(blob)
+        count = self.steps_done
         if device_step is None:
-            self.steps_done = self.steps_done + 1 if step is None else int(step)
-        config = _ADAM_CONFIG.pack(lr, self.betas[0], self.betas[1], self.eps, self.steps_done, _scalar(device_step, 8, self.dev), _scalar(device_lr, 4, self.dev),
+            count = count + 1 if step is None else int(step)
+        config = _ADAM_CONFIG.pack(lr, self.betas[0], self.betas[1], self.eps, count, _scalar(device_step, 8, self.dev), _scalar(device_lr, 4, self.dev),
                                    _scalar(grad_scale, 4, self.dev), self.seed & 0xffffffff, self.state_bits)
         check(lib.ormi_b200_adamw(self.dev.handle, blob, self.n, config))
+        self.steps_done = count                    # a refused call has not counted
 
 
 def _scalar(x, size: int, dev) -> int:

@@ -7,8 +7,8 @@ import pytest
 from ormi_b200 import graph as G
 from ormi_b200 import ops
 from ormi_b200 import workloads as W
-from ormi_b200._lib import check, lib
-from test_transformer_ops import ACC, BF, F8, FP, done, gpu, ints, no_guard_zones, randn, torch
+from ormi_b200._lib import BackendError, check, lib
+from test_transformer_ops import ACC, BF, F8, FP, NODEV, V, done, gpu, ints, no_guard_zones, randn, torch
 
 
 # ---- attention
@@ -94,6 +94,35 @@ def test_norm_to_eight_bits_of_tiny_groups(device, dtype, cols, group):
 
 
 # ---- AdamW
+
+def test_a_refused_adamw_step_does_not_count():
+    """Refused for its rate, its gradient, its step number or its scalars: the next step is still the one that comes after the last good one."""
+    opt = ops.AdamW(NODEV, [V(0x10000, (300,))], [V(0x20000, (300,))], [V(0x30000, (300,))], [V(0x40000, (300,))])
+    for bad in (dict(lr=float("nan")), dict(lr=0.1, grads=[V(0x10000, (300,))]), dict(lr=0.1, grads=[]), dict(lr=0.1, step=0), dict(lr=0.1, step=-3), dict(lr=0.1, grad_scale=0x8002)):
+        with pytest.raises((BackendError, ValueError)):
+            opt.step(**bad)
+        assert opt.steps_done == 0, bad
+
+
+@gpu
+def test_adamw_goes_on_after_a_refused_step(device):
+    n = 500
+    g = randn(n, seed=8)
+    got = []
+    for refuse in (False, True):
+        p, m, v = torch.ones(n, device="cuda"), torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+        opt = ops.AdamW(device, [p], [g], [m], [v])
+        torch.cuda.synchronize()
+        for _ in range(3):
+            if refuse:
+                with pytest.raises(BackendError):
+                    opt.step(lr=float("inf"))
+            opt.step(lr=0.1)
+        done(device)
+        assert opt.steps_done == 3
+        got.append((p, m, v))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
 
 @gpu
 @pytest.mark.parametrize("size", [1e-30, 1e-35, 1e-37])
