@@ -246,7 +246,7 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             // the capped score, its slope and the exponential of two columns: the polynomial runs on the FMA pipe while the
             // special function unit is busy with the exponentials before it
             auto expo = [&](int c, const float2& neg_lse2) {
-                if (CAP) g[c] = cap_slope(p, z[c]);
+                if (CAP) g[c] = cap_slope(p.cap, z[c]);
                 if (BIAS) {
                     if (!CAP) z[c] = mul2(z[c], both(p.scale_log2));
                     z[c] = make_float2(fmaf(-slope, fabsf(ahead + (float)(2 * c)), z[c].x), fmaf(-slope, fabsf(ahead + (float)(2 * c + 1)), z[c].y));
@@ -254,11 +254,11 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 z[c] = CAP || BIAS ? add2(z[c], neg_lse2) : fma2(z[c], both(p.scale_log2), neg_lse2);
                 z[c] = make_float2(ex2(z[c].x), ex2(z[c].y));
             };
-            if (!CAP || cap_is_polynomial<32>(p, z)) {
+            if (!CAP || cap_is_polynomial<32>(p.cap, z)) {
 #pragma unroll
                 for (int c = 0; c < 32; c += 2) {
                     const float4 l = *reinterpret_cast<const float4*>(&st.lse2[64 * w + 2 * c]);
-                    if (CAP) { z[c] = cap_polynomial(p, z[c]); z[c + 1] = cap_polynomial(p, z[c + 1]); }
+                    if (CAP) { z[c] = cap_polynomial(p.cap, z[c]); z[c + 1] = cap_polynomial(p.cap, z[c + 1]); }
                     expo(c, make_float2(l.x, l.y));
                     expo(c + 1, make_float2(l.z, l.w));
                 }
@@ -266,7 +266,7 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
 #pragma unroll
                 for (int c = 0; c < 32; c += 2) {
                     const float4 l = *reinterpret_cast<const float4*>(&st.lse2[64 * w + 2 * c]);
-                    z[c] = cap_any(p, z[c]); z[c + 1] = cap_any(p, z[c + 1]);
+                    z[c] = cap_any(p.cap, z[c]); z[c + 1] = cap_any(p.cap, z[c + 1]);
                     expo(c, make_float2(l.x, l.y));
                     expo(c + 1, make_float2(l.z, l.w));
                 }
@@ -604,7 +604,7 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
             const float ahead = (float)(pos - key0);
             const int left = end - key0;
             auto expo = [&](int c) {                                  // as in attn_back_kv
-                if (CAP) g[c] = cap_slope(p, z[c]);
+                if (CAP) g[c] = cap_slope(p.cap, z[c]);
                 if (BIAS) {
                     if (!CAP) z[c] = mul2(z[c], both(p.scale_log2));
                     z[c] = make_float2(fmaf(-slope, fabsf(ahead - (float)(2 * c)), z[c].x), fmaf(-slope, fabsf(ahead - (float)(2 * c + 1)), z[c].y));
@@ -613,12 +613,12 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                 z[c] = make_float2(ex2(z[c].x), ex2(z[c].y));
                 g[c] = CAP ? mul2(g[c], z[c]) : z[c];
             };
-            if (!CAP || cap_is_polynomial<32>(p, z)) {
+            if (!CAP || cap_is_polynomial<32>(p.cap, z)) {
 #pragma unroll
-                for (int c = 0; c < 32; ++c) { if (CAP) z[c] = cap_polynomial(p, z[c]); expo(c); }
+                for (int c = 0; c < 32; ++c) { if (CAP) z[c] = cap_polynomial(p.cap, z[c]); expo(c); }
             } else {
 #pragma unroll
-                for (int c = 0; c < 32; ++c) { z[c] = cap_any(p, z[c]); expo(c); }
+                for (int c = 0; c < 32; ++c) { z[c] = cap_any(p.cap, z[c]); expo(c); }
             }
             if (DOCS && cls == kDocs) {
 #pragma unroll

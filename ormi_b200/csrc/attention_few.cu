@@ -38,7 +38,8 @@ struct FewRow { int t, h, pos, end, doc; float slope; bool live; };
 
 template <int DP, bool CAP>
 __global__ void __launch_bounds__(kWarps * 32, 3)
-attn_few(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnParams p, int part_keys, int* err) {
+attn_few(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnParams p,
+         const __grid_constant__ CapTerms cap, int part_keys, int* err) {
     constexpr int kStages = FewShape<DP>::kStages, kStage = FewShape<DP>::kStage, kBox16 = kKeys * 128;
     extern __shared__ unsigned char raw[];
     const uint32_t base = (tc::smem_u32(raw) + 1023u) & ~1023u;
@@ -100,7 +101,7 @@ attn_few(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUte
     float o[DP / 8][4], top[2] = {-INFINITY, -INFINITY}, total[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    const float scale2 = p.scale * kLog2e, cap2 = p.cap * kLog2e, ecap = CAP ? 2.f * kLog2e * p.scale * p.inv_cap : 0.f;
+    const float scale2 = p.scale * kLog2e;
     int key0 = first + warp * kKeys;
     for (int k = 0; k < kStages; ++k) ask(key0 + k * kWarps * kKeys, k);
     bool ok = true;
@@ -123,10 +124,26 @@ attn_few(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUte
             mma16(s[0], q[k], kb[0], kb[1]);
             mma16(s[1], q[k], kb[2], kb[3]);
         }
+        if (CAP) {
+            // the polynomial wherever it holds: beyond it the cap is off by a few 1e-7 of the cap, whatever the score
+            float2 z[4] = {{s[0][0], s[0][1]}, {s[0][2], s[0][3]}, {s[1][0], s[1][1]}, {s[1][2], s[1][3]}};
+            const bool small = cap_is_polynomial<4>(cap, z);
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+            for (int i = 0; i < 4; ++i) {
+                float2 c = cap_polynomial(cap, z[i]);
+                if (!small) {
+                    const float2 far = cap_any(cap, z[i]);
+                    if (!(fabsf(z[i].x) <= cap.poly_limit)) c.x = far.x;
+                    if (!(fabsf(z[i].y) <= cap.poly_limit)) c.y = far.y;
+                }
+                s[i >> 1][2 * (i & 1)] = c.x; s[i >> 1][2 * (i & 1) + 1] = c.y;
+            }
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][i] = CAP ? cap2 - __fdividef(2.f * cap2, tc::ex2(s[n][i] * ecap) + 1.f) : s[n][i] * scale2;
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[n][i] *= scale2;
+        }
         if (p.slopes) {
 #pragma unroll
             for (int n = 0; n < 2; ++n)
@@ -251,7 +268,7 @@ void launch_few(ormi_b200_ctx* ctx, AttnParams& p) {
         p.part_max = p.part_out + p.splits * lines * p.dim;
         p.part_sum = p.part_max + p.splits * lines;
     }
-    kernel<<<dim3(p.splits, (unsigned)pairs, (unsigned)row_tiles), kWarps * 32, smem, ctx->stream>>>(maps[0], maps[1], p, part_keys, err);
+    kernel<<<dim3(p.splits, (unsigned)pairs, (unsigned)row_tiles), kWarps * 32, smem, ctx->stream>>>(maps[0], maps[1], p, cap_terms(p), part_keys, err);
     ORMI_CUDA(cudaGetLastError());
     count_launch(ctx);
     if (p.splits > 1) attention_join(ctx, p, ORMI_BF16);

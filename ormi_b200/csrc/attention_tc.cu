@@ -230,12 +230,12 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             // riding on the subtraction of the maximum.
             constexpr bool PLAIN = !CAP && !BIAS;
             if (CAP) {
-                if (cap_is_polynomial<64>(p, z)) {
+                if (cap_is_polynomial<64>(p.cap, z)) {
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) z[i] = cap_polynomial(p, z[i]);
+                    for (int i = 0; i < 64; ++i) z[i] = cap_polynomial(p.cap, z[i]);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) z[i] = cap_any(p, z[i]);
+                    for (int i = 0; i < 64; ++i) z[i] = cap_any(p.cap, z[i]);
                 }
             }
             if (BIAS) {
@@ -405,21 +405,26 @@ size_t bounds_bytes(const AttnParams& p) {
     return p.k_docs ? (size_t)p.batch * (units_of(p.q_len + kTile) + units_of(p.k_len)) * sizeof(int2) : 0;
 }
 
+CapTerms cap_terms(const AttnParams& a) {
+    CapTerms t{};
+    if (!(a.cap > 0.f)) return t;
+    const double k = (double)a.scale / a.cap, c = (double)a.scale * 1.4426950408889634;
+    static const double terms[4] = {0.9999999028730692, -0.333313732975708, 0.1327115660233386, -0.04756107721454571};
+    t.cap_log2 = a.cap * kLog2e;
+    for (int i = 0; i < 4; ++i) t.poly[i] = (float)(c * terms[i] * std::pow(k, 2 * i));
+    t.poly_limit = (float)std::min(0.4 / std::abs(k), 1e9);       // (a power that overflows has no business here)
+    t.exp_per_raw = (float)(2 * 1.4426950408889634 * k);
+    t.minus_inv_cap2 = -1.f / (t.cap_log2 * t.cap_log2);
+    return t;
+}
+
 TcParams tc_params(ormi_b200_ctx* ctx, const AttnParams& a, int2* bounds) {
     TcParams p{};
     p.a = a;
     p.q_units = units_of(a.q_len + kTile);
     p.k_units = units_of(a.k_len);
     p.scale_log2 = a.scale * kLog2e;
-    p.cap_log2 = a.cap * kLog2e;
-    if (a.cap > 0.f) {
-        const double k = (double)a.scale / a.cap, c = (double)a.scale * 1.4426950408889634;
-        static const double terms[4] = {0.9999999028730692, -0.333313732975708, 0.1327115660233386, -0.04756107721454571};
-        for (int i = 0; i < 4; ++i) p.poly[i] = (float)(c * terms[i] * std::pow(k, 2 * i));
-        p.poly_limit = (float)std::min(0.4 / k, 1e9);             // (a power that overflows has no business here)
-        p.exp_per_raw = (float)(2 * 1.4426950408889634 * k);
-        p.minus_inv_cap2 = -1.f / (p.cap_log2 * p.cap_log2);
-    }
+    p.cap = cap_terms(a);
     p.err = device_error_word(ctx);
     ctx->gemm_err_pending = true;
     if (a.k_docs) {

@@ -10,13 +10,16 @@ constexpr int kTile = 128, kUnit = 64;           // positions of a tile, and of 
 constexpr int kMaxTiles = 8192;                  // tiles (forward) or units (backward) that a block keeps a class for
 enum TileClass { kSkip = 0, kFull = 1, kPartial = 2, kDocs = 3 };   // no pair visible; every pair; look at positions; and at documents too
 
+// Raw products to capped base-2 scores (below).  With a cap: cap * log2(e), 2 log2(e) scale / cap, -1 / cap_log2^2, the
+// polynomial and the largest |raw| for it.
+struct CapTerms { float cap_log2, exp_per_raw, minus_inv_cap2, poly[4], poly_limit; };
+
 struct TcParams {
     AttnParams a;
     const int2 *q_bounds, *k_bounds;             // smallest and largest document of every unit, [batch][units]; NULL without documents
     int q_units, k_units;                        // even
-    float scale_log2, cap_log2;                  // scale * log2(e), cap * log2(e)
-    // with a cap: 2 log2(e) scale / cap, -1 / cap_log2^2, the polynomial and the largest |raw| for it
-    float exp_per_raw, minus_inv_cap2, poly[4], poly_limit;
+    float scale_log2;                            // scale * log2(e)
+    CapTerms cap;
     int cluster;                                 // backward pass: blocks that share the query heads of a key/value head
     int* err;
 };
@@ -44,23 +47,23 @@ __device__ __forceinline__ int tile_class(const TcParams& p, int b, int q_unit, 
 // z / raw.  A warp whose products leave that range takes tanh(x) = 1 - 2 / (e^2x + 1): two operations of the special
 // function unit, off by a few 1e-7 of the cap.
 template <int N>
-__device__ __forceinline__ bool cap_is_polynomial(const TcParams& p, const float2 (&z)[N]) {
+__device__ __forceinline__ bool cap_is_polynomial(const CapTerms& p, const float2 (&z)[N]) {
     float big = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) big = tc::max3(big, fabsf(z[i].x), fabsf(z[i].y));
     return __all_sync(0xffffffffu, big <= p.poly_limit);
 }
-__device__ __forceinline__ float2 cap_polynomial(const TcParams& p, const float2& raw) {
+__device__ __forceinline__ float2 cap_polynomial(const CapTerms& p, const float2& raw) {
     const float2 u = tc::mul2(raw, raw);
     float2 t = tc::fma2(u, tc::both(p.poly[3]), tc::both(p.poly[2]));
     t = tc::fma2(u, t, tc::both(p.poly[1]));
     return tc::mul2(raw, tc::fma2(u, t, tc::both(p.poly[0])));
 }
-__device__ __forceinline__ float2 cap_any(const TcParams& p, const float2& raw) {
+__device__ __forceinline__ float2 cap_any(const CapTerms& p, const float2& raw) {
     return make_float2(fmaf(-2.f * p.cap_log2, __fdividef(1.f, tc::ex2(raw.x * p.exp_per_raw) + 1.f), p.cap_log2),
                        fmaf(-2.f * p.cap_log2, __fdividef(1.f, tc::ex2(raw.y * p.exp_per_raw) + 1.f), p.cap_log2));
 }
-__device__ __forceinline__ float2 cap_slope(const TcParams& p, const float2& z) { return tc::fma2(tc::mul2(z, z), tc::both(p.minus_inv_cap2), tc::both(1.f)); }
+__device__ __forceinline__ float2 cap_slope(const CapTerms& p, const float2& z) { return tc::fma2(tc::mul2(z, z), tc::both(p.minus_inv_cap2), tc::both(1.f)); }
 
 // A warp's 32 rows x COLS columns of fp32 accumulators in tensor memory (a row per lane) as bf16 to global memory, times `by`:
 // through a staging buffer of the warp (32 x COLS x 2 bytes), so that neighbouring lanes write a whole row and not each lane
@@ -106,6 +109,7 @@ void head_map(ormi_b200_ctx* ctx, CUtensorMap* map, const void* ptr, const Strid
 bool map_allowed(const void* ptr, const Strides4& s, int batch, int len, int heads);
 TcParams tc_params(ormi_b200_ctx* ctx, const AttnParams& p, int2* bounds);
 size_t bounds_bytes(const AttnParams& p);
+CapTerms cap_terms(const AttnParams& p);
 template <typename T> inline int units_of(T len) { return (int)((len + kTile - 1) / kTile) * 2; }
 
 }  // namespace ormi_b200

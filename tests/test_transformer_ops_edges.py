@@ -8,7 +8,7 @@ from ormi_b200 import graph as G
 from ormi_b200 import ops
 from ormi_b200 import workloads as W
 from ormi_b200._lib import BackendError, check, lib
-from test_transformer_ops import ACC, BF, F8, FP, NODEV, V, done, gpu, ints, no_guard_zones, randn, torch
+from test_transformer_ops import ACC, BF, F8, FP, NODEV, V, Attention, close, done, gpu, ints, no_guard_zones, randn, run_attention, torch
 
 
 # ---- attention
@@ -59,6 +59,36 @@ def test_attention_gradients_of_keys_that_nobody_sees(device, mask, d, b, nk, h,
         if seen is None:
             seen = [x.clone() for x in grads]
         assert all(torch.equal(x, y) for x, y in zip(grads, seen)), f"call {turn} differs from the first"
+
+
+@gpu
+@pytest.mark.parametrize("nq, nk, d", [(1, 700, 64), (3, 1500, 128), (16, 90, 64), (200, 300, 64)])
+@pytest.mark.parametrize("cap", [1e4, 1e6, 1e9, 1e30])
+@pytest.mark.parametrize("scale", [None, -0.2])
+def test_attention_under_a_cap_far_above_the_scores(device, nq, nk, d, cap, scale):
+    """Such a cap changes nothing: |z - cap tanh(z / cap)| < |z|^3 / (3 cap^2) < 1e-5 for |z| < 30 and caps from 1e4 on, so the bounds
+    are those of the call without a cap, which do not grow with it.  Few queries and many, either sign of the scale."""
+    b, h, hk = 2, 4, 2
+    q, k, v = randn(b, nq, h, d, dtype=BF, seed=1), randn(b, nk, hk, d, dtype=BF, seed=2), randn(b, nk, hk, d, dtype=BF, seed=3)
+    out, lse = torch.empty_like(q), torch.empty(b, h, nq, device="cuda")
+    torch.cuda.synchronize()
+    ops.attention(device, q, k, v, out, lse, causal=True, cap=cap, scale=scale)
+    done(device)
+    ref = Attention(q, k, v, causal=True, scale=scale)
+    want, bound, want_lse, lse_bound = ref.forward()
+    size = float(ref.z[ref.seen].abs().max())
+    assert size < 30
+    off = size ** 3 / (3 * cap ** 2)
+    close("lse", lse, want_lse, lse_bound + off)
+    close("out", out, want, bound + 3 * off * float(v.abs().max()))
+
+
+@gpu
+@pytest.mark.parametrize("nq, nk", [(1, 700), (5, 300), (200, 300)])
+@pytest.mark.parametrize("cap, scale", [(0.5, 0.3), (3.0, -0.4), (20.0, 2.0), (5.0, 0.0)])
+def test_attention_caps_of_either_sign_that_scores_reach(device, nq, nk, cap, scale):
+    """Scores on both sides of the border between the polynomial and the exponential form of the cap."""
+    run_attention(device, randn(2, nq, 4, 64, dtype=BF, seed=1), randn(2, nk, 2, 64, dtype=BF, seed=2), randn(2, nk, 2, 64, dtype=BF, seed=3), causal=True, cap=cap, scale=scale)
 
 
 # ---- RMS norm
