@@ -547,6 +547,7 @@ void forward_check(const char* op, const ormi_b200_attention_args& a, bool backw
     ints_check(op, "q_start", a.q_start, b, -1);
     OP_NEED(std::isfinite(a.scale), op, "scale is not finite");
     OP_NEED(a.cap >= 0.f && std::isfinite(a.cap), op, "cap is negative or not finite");
+    OP_NEED(a.cap == 0.f || std::isfinite(1.f / a.cap), op, "cap is too small: 1 / cap is not finite");
 }
 
 // Whether two views whose spans overlap are slices of one buffer that never meet, such as the gradients of q, k and v side by

@@ -278,7 +278,7 @@ void launch_few(ormi_b200_ctx* ctx, AttnParams& p) {
 }  // namespace
 
 bool attention_few_supported(const AttnParams& p, int dtype) {
-    return dtype == ORMI_BF16 && p.dim <= 128 && p.dim % 8 == 0 && p.k_len >= 1 && (int64_t)p.q_len * p.group <= 64 && map_allowed(p.q, p.qs, p.batch, p.q_len, p.heads) &&
+    return dtype == ORMI_BF16 && cap_terms_exist(p) && p.dim <= 128 && p.dim % 8 == 0 && p.k_len >= 1 && (int64_t)p.q_len * p.group <= 64 && map_allowed(p.q, p.qs, p.batch, p.q_len, p.heads) &&
            map_allowed(p.k, p.ks, p.batch, p.k_len, p.kv_heads) && map_allowed(p.v, p.vs, p.batch, p.k_len, p.kv_heads);
 }
 

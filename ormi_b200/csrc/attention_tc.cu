@@ -15,6 +15,7 @@
 // nothing in fp32 sums nor, relatively, in bf16.
 #include <algorithm>
 #include <cmath>
+#include <limits>
 
 #include "attention_tc.cuh"
 
@@ -411,8 +412,15 @@ CapTerms cap_terms(const AttnParams& a) {
     const double k = (double)a.scale / a.cap, c = (double)a.scale * 1.4426950408889634;
     static const double terms[4] = {0.9999999028730692, -0.333313732975708, 0.1327115660233386, -0.04756107721454571};
     t.cap_log2 = a.cap * kLog2e;
-    for (int i = 0; i < 4; ++i) t.poly[i] = (float)(c * terms[i] * std::pow(k, 2 * i));
-    t.poly_limit = (float)std::min(0.4 / std::abs(k), 1e9);       // (a power that overflows has no business here)
+    // A coefficient below fp32's normal numbers (a cap far above any score) is worth nothing, so the polynomial ends where its
+    // term would matter (2^-24 of the score); one above them (a cap far below) leaves no place for the polynomial at all.
+    double limit = 0.4;
+    for (int i = 0; i < 4; ++i) {
+        t.poly[i] = (float)(c * terms[i] * std::pow(k, 2 * i));
+        if (!std::isfinite(t.poly[i])) limit = -1;
+        else if (i && std::abs(t.poly[i]) < std::numeric_limits<float>::min()) limit = std::min(limit, std::pow(0x1p-24 / std::abs(terms[i]), 0.5 / i));
+    }
+    t.poly_limit = (float)(limit < 0 ? -1 : std::min(limit / std::abs(k), 1e18));     // (its square is an fp32 number)
     t.exp_per_raw = (float)(2 * 1.4426950408889634 * k);
     t.minus_inv_cap2 = -1.f / (t.cap_log2 * t.cap_log2);
     return t;
@@ -437,8 +445,14 @@ TcParams tc_params(ormi_b200_ctx* ctx, const AttnParams& a, int2* bounds) {
     return p;
 }
 
+// Scales and caps whose products with log2(e), ratio and square are fp32 numbers; others go to the kernels that use tanhf.
+bool cap_terms_exist(const AttnParams& p) {
+    const double scale = std::abs((double)p.scale), cap = p.cap;
+    return scale <= 1e30 && (cap == 0 || (cap >= 1e-15 && cap <= 1e35 && scale <= 1e30 * cap));
+}
+
 bool attention_tc_supported(const AttnParams& p, int dtype) {
-    return dtype == ORMI_BF16 && p.scale > 0.f && p.dim <= 128 && p.dim % 8 == 0 && p.k_len >= 1 && p.k_len <= kMaxTiles * kTile && p.q_len <= 65535 * 2 * kTile &&
+    return dtype == ORMI_BF16 && cap_terms_exist(p) && p.scale > 0.f && p.dim <= 128 && p.dim % 8 == 0 && p.k_len >= 1 && p.k_len <= kMaxTiles * kTile && p.q_len <= 65535 * 2 * kTile &&
            (int64_t)p.batch * p.heads < 0x7fffffff && map_allowed(p.q, p.qs, p.batch, p.q_len, p.heads) && map_allowed(p.k, p.ks, p.batch, p.k_len, p.kv_heads) &&
            map_allowed(p.v, p.vs, p.batch, p.k_len, p.kv_heads) && map_allowed(p.out, p.os, p.batch, p.q_len, p.heads);
 }

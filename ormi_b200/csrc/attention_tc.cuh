@@ -110,6 +110,7 @@ bool map_allowed(const void* ptr, const Strides4& s, int batch, int len, int hea
 TcParams tc_params(ormi_b200_ctx* ctx, const AttnParams& p, int2* bounds);
 size_t bounds_bytes(const AttnParams& p);
 CapTerms cap_terms(const AttnParams& p);
+bool cap_terms_exist(const AttnParams& p);
 template <typename T> inline int units_of(T len) { return (int)((len + kTile - 1) / kTile) * 2; }
 
 }  // namespace ormi_b200

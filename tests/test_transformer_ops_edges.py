@@ -1,5 +1,6 @@
 """Transformer-block operators at the edges of what their documentation allows."""
 import ctypes
+import math
 
 import numpy as np
 import pytest
@@ -8,7 +9,7 @@ from ormi_b200 import graph as G
 from ormi_b200 import ops
 from ormi_b200 import workloads as W
 from ormi_b200._lib import BackendError, check, lib
-from test_transformer_ops import ACC, BF, F8, FP, NODEV, V, Attention, close, done, gpu, ints, no_guard_zones, randn, run_attention, torch
+from test_transformer_ops import ACC, BF, F8, FP, NODEV, V, Attention, accepted, attn_args, close, done, gpu, ints, no_guard_zones, randn, refused, run_attention, torch
 
 
 # ---- attention
@@ -89,6 +90,44 @@ def test_attention_under_a_cap_far_above_the_scores(device, nq, nk, d, cap, scal
 def test_attention_caps_of_either_sign_that_scores_reach(device, nq, nk, cap, scale):
     """Scores on both sides of the border between the polynomial and the exponential form of the cap."""
     run_attention(device, randn(2, nq, 4, 64, dtype=BF, seed=1), randn(2, nk, 2, 64, dtype=BF, seed=2), randn(2, nk, 2, 64, dtype=BF, seed=3), causal=True, cap=cap, scale=scale)
+
+
+@gpu
+@pytest.mark.parametrize("nq, nk", [(2, 400), (200, 300)])
+@pytest.mark.parametrize("cap", [3e6, 1e7, 1e8, 1e12])
+def test_attention_large_caps_that_scores_reach(device, nq, nk, cap):
+    """Scores up to 0.4 of a cap whose sixth power leaves fp32 against the scale: capped scores to 2^-16 (the exponential form is off by
+    5e-7 of the cap, on scores from a tenth of it on; below, the polynomial's terms are worth less than 2^-24)."""
+    b, h, d = 2, 2, 64
+    q, k, v = (randn(b, n, h, d, dtype=BF, seed=i) for i, n in ((1, nq), (2, nk), (3, nk)))
+    scale = 0.125
+    size = (q.float().transpose(1, 2) @ k.float().permute(0, 2, 3, 1)).abs().max().item() * scale
+    q = (q * (0.4 * cap / size) ** 0.5).to(BF)
+    k = (k * (0.4 * cap / size) ** 0.5).to(BF)
+    out, lse = torch.empty_like(q), torch.empty(b, h, nq, device="cuda")
+    torch.cuda.synchronize()
+    ops.attention(device, q, k, v, out, lse, cap=cap, scale=scale)
+    done(device)
+    want = Attention(q, k, v, cap=cap, scale=scale).lse
+    close("lse", lse, want, 2.0 ** -16 * want.abs() + 2.0 ** -20 * math.log(nk))
+
+
+@gpu
+@pytest.mark.parametrize("nq, nk", [(1, 400), (8, 90), (200, 300)])
+@pytest.mark.parametrize("cap", [1e-6, 1e-8, 1e-14, 1e-20, 1e-37])
+@pytest.mark.parametrize("scale", [0.125, -3.0])
+def test_attention_caps_far_below_the_scores(device, nq, nk, cap, scale):
+    """Capped scores are all but equal; queries of zeros have scores of zero, whatever power of scale / cap leaves fp32."""
+    q, k, v = randn(2, nq, 4, 64, dtype=BF, seed=1), randn(2, nk, 2, 64, dtype=BF, seed=2), randn(2, nk, 2, 64, dtype=BF, seed=3)
+    q[0] = 0.0
+    k[1, 5] = 0.0
+    run_attention(device, q, k, v, causal=True, cap=cap, scale=scale)
+
+
+def test_attention_refuses_caps_without_an_inverse():
+    for cap in (1e-39, 1e-45):
+        refused(attn_args(cap=cap), "cap")
+    accepted(attn_args(cap=1e-37))
 
 
 # ---- RMS norm
