@@ -321,7 +321,7 @@ int ormi_b200_attention(ormi_b200_ctx* ctx, const ormi_b200_attention_args* args
  * forward call wrote them.  dk and dv of a shared head are the sums over its query heads; keys nobody sees get zero.
  * dq, dk, dv: q's type, the shapes of q, k, v; they may be slices of one buffer.  Slopes, cap and scale are constants.
  * On the tensor cores (BF16, head_dim a multiple of 8 up to 128, 16-byte aligned addresses and strides, scale > 0, cap 0
- * or 1e-15 to 1e35, up to 2^20 keys forward and 2^19 positions backward) both passes round probabilities and score gradients to bf16; other cases
+ * or 1e-15 to 1e35, up to 2^20 keys, and backward 2^20 queries) both passes round probabilities and score gradients to bf16; other cases
  * run in fp32 arithmetic. */
 typedef struct ormi_b200_attention_backward_args {
     ormi_b200_attention_args forward;

@@ -104,7 +104,7 @@ attn_back_kv(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     if (warp == 2) {
         const int n = key0 >= m.keys ? 0 : list_tiles(list, (p.a.q_len + kTile - 1) / kTile, [&](int t) {
             const int first = t * kTile, last = min(first + kTile, p.a.q_len) - 1;
-            return tile_class<2, 2>(p, b, 2 * t, key_end(m, m.start + first), key_end(m, m.start + last), key0 / kUnit);
+            return tile_class(p, b, 2 * t, key_end(m, m.start + first), key_end(m, m.start + last), key0 / kUnit);
         });
         if (lane == 0) list_size = n;
     }
@@ -418,7 +418,7 @@ attn_back_q(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     const int blank_tile = m.keys < p.a.k_len && m.keys % kTile ? m.keys / kTile : -1;
     if (warp == 2) {
         const int lo = key_end(m, m.start + q0), hi = key_end(m, m.start + min(q0 + kTile, p.a.q_len) - 1);
-        const int n = list_tiles(list, (max(hi, 0) + kTile - 1) / kTile, [&](int j) { return tile_class<2, 2>(p, b, q0 / kUnit, lo, hi, 2 * j); });
+        const int n = list_tiles(list, (max(hi, 0) + kTile - 1) / kTile, [&](int j) { return tile_class(p, b, q0 / kUnit, lo, hi, 2 * j); });
         if (lane == 0) list_size = n;
     }
     if (threadIdx.x == 0) {

@@ -86,7 +86,7 @@ attn_forward_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     // classes of the tiles, and which union tile holds the last valid key in its middle
     for (int j = threadIdx.x; j < tiles; j += kThreads) {
         int c = 0;
-        for (int w = 0; w < 2; ++w) c |= tile_class<2, 2>(p, b, q0 / kUnit + 2 * w, lo[w], hi[w], 2 * j) << (2 * w);
+        for (int w = 0; w < 2; ++w) c |= tile_class(p, b, q0 / kUnit + 2 * w, lo[w], hi[w], 2 * j) << (2 * w);
         cls[j] = (unsigned char)c;
     }
     fence_before();

@@ -7,7 +7,7 @@
 namespace ormi_b200 {
 
 constexpr int kTile = 128, kUnit = 64;           // positions of a tile, and of half of one
-constexpr int kMaxTiles = 8192;                  // tiles (forward) or units (backward) that a block keeps a class for
+constexpr int kMaxTiles = 8192;                  // tiles of keys (of queries in attn_back_kv) that a block keeps a class for: 2^20 positions
 enum TileClass { kSkip = 0, kFull = 1, kPartial = 2, kDocs = 3 };   // no pair visible; every pair; look at positions; and at documents too
 
 // Raw products to capped base-2 scores (below).  With a cap: cap * log2(e), 2 log2(e) scale / cap, -1 / cap_log2^2, the
@@ -24,19 +24,16 @@ struct TcParams {
     int* err;
 };
 
-// Class of QU units of queries from q_unit on against KU units of keys from k_unit on.  `lo` and `hi`: key_end of the first
+// Class of a tile of queries (the two units from q_unit on) against a tile of keys (two from k_unit on).  `lo` and `hi`: key_end of the first
 // query and of the last one that exists.
-template <int QU, int KU>
 __device__ __forceinline__ int tile_class(const TcParams& p, int b, int q_unit, int lo, int hi, int k_unit) {
     const int key0 = k_unit * kUnit;
     if (key0 >= hi) return kSkip;
-    const int c = key0 + KU * kUnit <= lo ? kFull : kPartial;
+    const int c = key0 + kTile <= lo ? kFull : kPartial;
     if (!p.k_bounds) return c;
     const int2* qb = p.q_bounds + (int64_t)b * p.q_units + q_unit;
     const int2* kb = p.k_bounds + (int64_t)b * p.k_units + k_unit;
-    int2 q = qb[0], k = kb[0];
-    if (QU == 2) q = make_int2(min(q.x, qb[1].x), max(q.y, qb[1].y));
-    if (KU == 2) k = make_int2(min(k.x, kb[1].x), max(k.y, kb[1].y));
+    const int2 q = make_int2(min(qb[0].x, qb[1].x), max(qb[0].y, qb[1].y)), k = make_int2(min(kb[0].x, kb[1].x), max(kb[0].y, kb[1].y));
     if (k.y < q.x || k.x > q.y) return kSkip;
     return k.x == k.y && q.x == q.y ? c : kDocs;
 }

@@ -130,6 +130,30 @@ def test_attention_refuses_caps_without_an_inverse():
     accepted(attn_args(cap=1e-37))
 
 
+@gpu
+@pytest.mark.parametrize("n", [(1 << 19) + 77, (1 << 20) - 5])
+def test_attention_of_documents_up_to_the_longest_row(device, n):
+    """Up to the 2^20 positions that the tensor-core kernels take, in documents of 200."""
+    h, d, size = 1, 64, 200
+    q, k, v, dout = (randn(1, n, h, d, dtype=BF, seed=i) for i in range(4))
+    docs = (torch.arange(n, device="cuda") // size).int()[None]
+    out, lse = torch.empty_like(q), torch.empty(1, h, n, device="cuda")
+    g = [torch.full_like(q, 3.0) for _ in range(3)]
+    torch.cuda.synchronize()
+    ops.attention(device, q, k, v, out, lse, causal=True, q_docs=docs, k_docs=docs)
+    ops.attention_backward(device, dout, q, k, v, out, lse, *g, causal=True, q_docs=docs, k_docs=docs)
+    done(device)
+    for first in (0, 400, (1 << 18) // size * size, (1 << 19) // size * size - size, (1 << 19) // size * size, n // size * size - size, n // size * size):
+        cut = slice(first, min(first + size, n))
+        ref = Attention(q[:, cut], k[:, cut], v[:, cut], causal=True)
+        want, bound, want_lse, lse_bound = ref.forward()
+        close("out", out[:, cut], want, bound)
+        close("lse", lse[:, :, cut], want_lse, lse_bound)
+        for (name, (want, bound)), got in zip(ref.backward(dout[:, cut], out[:, cut], lse[:, :, cut]).items(), g):
+            close(name, got[:, cut], want, bound)
+    assert all(bool(torch.isfinite(x).all()) and not bool((x == 3.0).all(-1).any()) for x in g)
+
+
 # ---- RMS norm
 
 @gpu
