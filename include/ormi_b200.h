@@ -260,7 +260,8 @@ int ormi_b200_colsum_static(const float* in, int64_t rows, int64_t cols, float* 
  *   - results are bit-identical run to run (no atomics on values). */
 enum ormi_b200_dtype { ORMI_F32 = 0, ORMI_BF16 = 1, ORMI_E4M3 = 2, ORMI_I32 = 3 };
 
-/* A strided view of device memory; strides in elements, never negative.  data == NULL: the argument is left out. */
+/* A strided view of device memory; strides in elements, never negative; at most 2^48 elements, repeated ones included.
+ * data == NULL: the argument is left out. */
 typedef struct ormi_b200_view {
     void*   data;
     int32_t dtype;                         /* enum ormi_b200_dtype */

@@ -49,7 +49,8 @@ inline bool same_place(const ormi_b200_view& a, const ormi_b200_view& b) {
     return true;
 }
 
-// The checks every view goes through: rank, extents, strides whose span fits in 63 bits, alignment to the element.
+// The checks every view goes through: rank, extents, alignment to the element, and that neither the number of elements (2^48,
+// repeated ones included) nor the way to the last one (2^56 elements) comes near 63 bits.
 inline void view_check(const char* op, const char* name, const ormi_b200_view& v, int lo_rank, int hi_rank) {
     auto n = [&] { return std::string(name); };
     OP_NEED(v.ndim >= 1 && v.ndim <= 4, op, v.data ? n() + " has " + std::to_string(v.ndim) + " dimensions" : n() + " is missing");
@@ -63,6 +64,9 @@ inline void view_check(const char* op, const char* name, const ormi_b200_view& v
         OP_NEED(v.shape[d] >= 0 && v.shape[d] < (int64_t)1 << 31, op, n() + " has an extent below zero or above 2^31 - 1");
         OP_NEED(v.strides[d] >= 0 && v.strides[d] < (int64_t)1 << 40, op, n() + " has a stride below zero or above 2^40");
     }
+    double elements = 1, last = 0;
+    for (int d = 0; d < v.ndim; ++d) { elements *= (double)v.shape[d]; last += (double)v.shape[d] * (double)v.strides[d]; }
+    OP_NEED(elements <= 0x1p48 && (elements == 0 || last <= 0x1p56), op, n() + " is too large");
     OP_NEED((uintptr_t)v.data % dtype_bytes(v.dtype) == 0, op, n() + " does not start on a whole element");
 }
 inline int64_t count_of(const ormi_b200_view& v) {

@@ -9,7 +9,7 @@ from ormi_b200 import graph as G
 from ormi_b200 import ops
 from ormi_b200 import workloads as W
 from ormi_b200._lib import BackendError, check, lib
-from test_transformer_ops import ACC, BF, F8, FP, NODEV, V, Attention, accepted, attn_args, close, done, gpu, ints, no_guard_zones, randn, refused, run_attention, torch
+from test_transformer_ops import ACC, Attention, BF, F8, FP, NODEV, V, accepted, attn_args, close, done, gpu, ints, no_guard_zones, norm_args, norm_back, randn, refused, run_attention, torch
 
 
 # ---- attention
@@ -122,6 +122,18 @@ def test_attention_caps_far_below_the_scores(device, nq, nk, cap, scale):
     q[0] = 0.0
     k[1, 5] = 0.0
     run_attention(device, q, k, v, causal=True, cap=cap, scale=scale)
+
+
+@pytest.mark.parametrize("call", [
+    # as many rows as 2^64 is zero of: an output whose rows all lie on one another is not an empty one
+    lambda: norm_args(x=V(0x1000, (1 << 30, 1 << 30, 16, 64), "bf16", (0, 0, 0, 1)), out=V(0x8000, (1 << 30, 1 << 30, 16, 64), "bf16", (0, 0, 0, 1))),
+    lambda: attn_args(b=16, nq=1 << 30, h=1 << 30, hk=1, q=V(0x100000, (16, 1 << 30, 1 << 30, 32), "bf16", (0, 0, 0, 1)), out=V(0x400000, (16, 1 << 30, 1 << 30, 32), "bf16", (0, 0, 0, 1))),
+    # spans beyond 63 bits
+    lambda: norm_args(x=V(0x1000, ((1 << 31) - 1, 64), "bf16", ((1 << 40) - 1, 1)), out=V(0x8000, ((1 << 31) - 1, 64), "bf16", ((1 << 40) - 1, 1))),
+    lambda: attn_args(b=1, nk=1 << 30, k=V(0x200000, (1, 1 << 30, 2, 32), "bf16", (0, (1 << 40) - 8, 32, 1)), v=V(0x300000, (1, 1 << 30, 2, 32), "bf16", (0, (1 << 40) - 8, 32, 1))),
+])
+def test_views_beyond_the_address_space_are_refused(call):
+    refused(call(), "too large")
 
 
 def test_attention_refuses_caps_without_an_inverse():
