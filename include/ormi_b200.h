@@ -273,8 +273,8 @@ typedef struct ormi_b200_view {
 /* Root-mean-square norm of the last dimension, with the residual's addition in front of it:
  *     s = x + residual            (rounded to x's type, stored to residual_out when given)
  *     rstd = 1 / sqrt(mean(s^2) + eps),    out = s * rstd * weight
- * x, residual, residual_out: F32 or BF16, one type, same shape; leading dimensions that do not collapse into one row
- * stride are refused.  weight: [cols], F32 or BF16, or left out (ones).  out: F32, BF16 or E4M3.  rstd: [rows] F32,
+ * x, residual, residual_out: F32 or BF16, one type, same shape, at most 2^30 columns; leading dimensions that do not
+ * collapse into one row stride are refused.  weight: [cols], F32 or BF16, or left out (ones).  out: F32, BF16 or E4M3.  rstd: [rows] F32,
  * optional (the backward pass reads it).  With an E4M3 `out`, scales is [rows, groups] F32, contiguous: group = 0 is one
  * scale for the row, group = 128 one for every 128 columns; scale = max|y| / 448 and out = round(y * (448 / max|y|)), zero
  * for a group of zeros.  out may be x or residual in place; residual_out may be x or residual. */

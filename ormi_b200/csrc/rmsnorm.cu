@@ -461,6 +461,7 @@ __global__ void __launch_bounds__(1024) norm_dweight_join(const float* __restric
 
 // ------------------------------------------------------------------------------------------------ host side
 // The leading dimensions of a view as one row index: rows and the stride between them.  Throws when they do not collapse.
+constexpr int64_t kMaxCols = (int64_t)1 << 30;                   // a step past the last column is still an int
 struct Rows { int64_t rows, stride; };
 Rows rows_of(const char* op, const char* name, const ormi_b200_view& v) {
     Rows r{1, 0};
@@ -604,6 +605,7 @@ void rmsnorm_check(const ormi_b200_rmsnorm_args& a) {
     matrix_check(op, "x", a.x, a.x, true);
     const int64_t cols = a.x.shape[a.x.ndim - 1], rows = rows_of(op, "x", a.x).rows;
     OP_NEED(cols >= 1, op, "x has no columns");
+    OP_NEED(cols <= kMaxCols, op, "x has more than 2^30 columns");
     OP_NEED(a.eps >= 0.f, op, "eps is negative or not a number");
     if (a.residual.data) matrix_check(op, "residual", a.residual, a.x, true);
     if (a.residual_out.data) {
@@ -658,6 +660,7 @@ void rmsnorm_backward_check(const ormi_b200_rmsnorm_backward_args& a) {
     matrix_check(op, "dout", a.dout, a.dout, true);
     const int64_t cols = a.dout.shape[a.dout.ndim - 1], rows = rows_of(op, "dout", a.dout).rows;
     OP_NEED(cols >= 1, op, "dout has no columns");
+    OP_NEED(cols <= kMaxCols, op, "dout has more than 2^30 columns");
     matrix_check(op, "s", a.s, a.dout, true);
     if (a.dresidual.data) matrix_check(op, "dresidual", a.dresidual, a.dout, true);
     matrix_check(op, "dx", a.dx, a.dout, true);

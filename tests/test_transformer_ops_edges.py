@@ -168,6 +168,14 @@ def test_attention_of_documents_up_to_the_longest_row(device, n):
 
 # ---- RMS norm
 
+def test_norm_refuses_rows_whose_columns_pass_an_int():
+    """(The kernels step past the last column in 32 bits.)"""
+    at = lambda address, cols: V(address << 36, (2, cols), "bf16", (1 << 33, 1))      # noqa: E731
+    for cols in ((1 << 30) + 1, (1 << 31) - 1):
+        refused(norm_args(x=at(1, cols), weight=None, out=at(2, cols)), "2^30 columns")
+        refused(norm_back(dout=at(1, cols), s=at(2, cols), weight=None, dx=at(3, cols), rstd=V(0x4000, (2,)), dweight=None), "2^30 columns")
+    accepted(norm_args(x=at(1, 1 << 30), weight=None, out=at(2, 1 << 30)))
+
 @gpu
 @pytest.mark.parametrize("dtype", [FP, BF])
 @pytest.mark.parametrize("cols", [100, 256, 1111, 4096, 40000])
