@@ -341,7 +341,7 @@ int ormi_b200_attention_backward(ormi_b200_ctx* ctx, const ormi_b200_attention_b
  * that moves by less than half a step would otherwise stand still), with bits hashed from (seed, step, tensor, element);
  * a positive sqrt(v) never becomes zero.  All-zero codes and scales are the initial state.  A gradient that is not finite
  * leaves its element, and with 8-bit states the 128 elements of its block, not finite.
- * Buffers are contiguous; none that is written may overlap another one of the call.
+ * Buffers are contiguous; none that is written (device_step among them) may overlap another one of the call.
  * device_step (optional, for captured steps): a device counter of the steps done so far; the call takes *device_step + 1
  * as its step and adds one.  device_lr, grad_scale (optional): device floats, read when the kernel runs. */
 typedef struct ormi_b200_adamw_tensor {

@@ -382,11 +382,13 @@ void adamw_check(const ormi_b200_adamw_tensor* t, int n, const ormi_b200_adamw_c
         add(x.m_scales, (x.n + 127) / 128 * 4, true); add(x.v_scales, (x.n + 127) / 128 * 4, true);
         add(x.copy16, x.n * 2, true);
     }
+    auto scalar = [&](const void* p, int64_t bytes, bool out) { if (p) ranges.push_back({(const char*)p, (const char*)p + bytes, out, -1}); };
+    scalar(c.device_step, 8, true); scalar(c.device_lr, 4, false); scalar(c.grad_scale, 4, false);
     // what is written lies apart from everything else (the same tensor twice would be updated by two blocks at once)
     std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.lo < b.lo; });
     const char* end_any = nullptr; const char* end_out = nullptr;
     for (const Range& r : ranges) {
-        OP_NEED(!(r.lo < end_out || (r.out && r.lo < end_any)), op, "tensor " + std::to_string(r.tensor) + ": a buffer that is written overlaps another one");
+        OP_NEED(!(r.lo < end_out || (r.out && r.lo < end_any)), op, (r.tensor < 0 ? std::string("a device scalar") : "tensor " + std::to_string(r.tensor)) + ": a buffer that is written overlaps another one");
         end_any = std::max(end_any, r.hi);
         if (r.out) end_out = std::max(end_out, r.hi);
     }

@@ -217,6 +217,18 @@ def test_a_refused_adamw_step_does_not_count():
         assert opt.steps_done == 0, bad
 
 
+def test_adamw_refuses_device_scalars_inside_what_it_writes():
+    """The blocks of a launch would read them while others write there."""
+    def opt(**more):
+        return ops.AdamW(NODEV, [V(0x10000, (300,))], [V(0x20000, (300,))], [V(0x30000, (300,))], [V(0x40000, (300,))], **more)
+    refused(lambda: opt().step(lr=0.1, grad_scale=0x10004), "overlaps")
+    refused(lambda: opt().step(device_lr=0x30000 + 1196), "overlaps")
+    refused(lambda: opt().step(lr=0.1, device_step=0x40008), "overlaps")
+    refused(lambda: opt().step(lr=0.1, device_step=0x20008), "overlaps")
+    refused(lambda: opt().step(lr=0.1, device_step=0x80000, grad_scale=0x80004), "overlaps")
+    accepted(lambda: opt().step(grad_scale=0x20004, device_lr=0x20004, device_step=0x80000))
+
+
 @gpu
 def test_adamw_goes_on_after_a_refused_step(device):
     n = 500
