@@ -333,7 +333,7 @@ int ormi_b200_attention_backward(ormi_b200_ctx* ctx, const ormi_b200_attention_b
 /* One AdamW step over many tensors, in place (`step` counts from 1):
  *     g = grad * grad_scale;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *     param -= lr * weight_decay * param + lr * (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps)
- * param: n fp32 values.  grad: F32 or BF16.  copy16 (optional): n bf16 values, the new parameters rounded.  A bf16 copy
+ * eps: 0, or at least 2^-126.  param: n fp32 values.  grad: F32 or BF16.  copy16 (optional): n bf16 values, the new parameters rounded.  A bf16 copy
  * that the context keeps of `param` for its matmuls ("matmul" = "bf16") is rewritten along with it.
  * state_bits = 32: m and v are fp32.  state_bits = 8: m holds e4m3 codes of m, v holds e4m3 codes of sqrt(v), both n bytes,
  * with one fp32 scale for every 128 elements in m_scales / v_scales (ceil(n / 128) each; value = code * scale, scale =

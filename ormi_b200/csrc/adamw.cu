@@ -15,6 +15,7 @@
 // written order give the same codes on any machine.
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <type_traits>
 #include <vector>
 
@@ -360,6 +361,7 @@ void adamw_check(const ormi_b200_adamw_tensor* t, int n, const ormi_b200_adamw_c
     OP_NEED(c.device_step || c.step >= 1, op, "step counts from 1");
     OP_NEED(c.beta1 >= 0 && c.beta1 < 1 && c.beta2 >= 0 && c.beta2 < 1, op, "beta1 and beta2 lie in [0, 1)");
     OP_NEED(c.eps >= 0 && std::isfinite(c.eps), op, "eps is negative or not finite");
+    OP_NEED(c.eps == 0 || (float)c.eps >= std::numeric_limits<float>::min(), op, "eps is above zero and below 2^-126");
     OP_NEED(std::isfinite(c.lr), op, "lr is not finite");
     OP_NEED((uintptr_t)c.device_step % 8 == 0 && (uintptr_t)c.device_lr % 4 == 0 && (uintptr_t)c.grad_scale % 4 == 0, op, "a device scalar does not start on a whole element");
     struct Range { const char* lo; const char* hi; bool out; int tensor; };

@@ -229,6 +229,16 @@ def test_adamw_refuses_device_scalars_inside_what_it_writes():
     accepted(lambda: opt().step(grad_scale=0x20004, device_lr=0x20004, device_step=0x80000))
 
 
+def test_adamw_refuses_an_eps_that_its_reciprocal_takes_for_zero():
+    """The quotient is m times an approximate reciprocal that flushes numbers below 2^-126: an element without a gradient would be 0 * inf."""
+    def opt(eps):
+        return ops.AdamW(NODEV, [V(0x10000, (300,))], [V(0x20000, (300,))], [V(0x30000, (300,))], [V(0x40000, (300,))], eps=eps)
+    for eps in (1e-38, 1e-45, 1e-60):
+        refused(lambda: opt(eps).step(lr=0.1), "eps")
+    for eps in (0.0, 1.2e-38, 1e-8):
+        accepted(lambda: opt(eps).step(lr=0.1))
+
+
 @gpu
 def test_adamw_goes_on_after_a_refused_step(device):
     n = 500
