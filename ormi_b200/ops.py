@@ -121,6 +121,12 @@ def upload(dev, array, dtype: str = "f32") -> Array:
     return out
 
 
+def _same_gpu(owner, dev_index: int):
+    index = getattr(owner, "index", None)
+    if isinstance(index, int) and index != dev_index:
+        raise ValueError(f"a buffer on cuda:{index} where the device is cuda:{dev_index}")
+
+
 def _pack(x, dev_index: int) -> bytes:
     """``x`` as an ormi_b200_view."""
     if x is None:
@@ -139,6 +145,7 @@ def _pack(x, dev_index: int) -> bytes:
                 return _VIEW_PACK(x.data_ptr(), code, 1, shape[0], 0, 0, 0, strides[0], 0, 0, 0)
     if isinstance(x, View):
         ptr, code, shape, strides = x.ptr, x.dtype, x.shape, x.strides
+        _same_gpu(x.dev if isinstance(x, Array) else None, dev_index)
     elif hasattr(x, "data_ptr"):
         dt = x.dtype
         code = _by_dtype.get(dt)
@@ -155,6 +162,7 @@ def _pack(x, dev_index: int) -> bytes:
         data = x.data if isinstance(x, G.Node) else x
         if data is None or data.dev_ptr is None:
             raise ValueError("a graph node that is not realized on the device")
+        _same_gpu(getattr(data._release, "__self__", None), dev_index)      # the device whose pool the block goes back to
         ptr, shape = data.dev_ptr, tuple(x.shape)
         strides = tuple(x.strides) if isinstance(x, G.Node) else G.calc_contiguous_strides(shape)
         code = BF16 if isinstance(x, G.Node) and x.bf16 else F32

@@ -166,6 +166,31 @@ def test_attention_of_documents_up_to_the_longest_row(device, n):
     assert all(bool(torch.isfinite(x).all()) and not bool((x == 3.0).all(-1).any()) for x in g)
 
 
+# ---- buffers
+
+class _Elsewhere:
+    """A device of another GPU, as far as buffers know one."""
+    index, handle = 1, None
+
+    def alloc(self, nbytes):
+        return 0x700000
+
+    def free(self, ptr, nbytes):
+        pass
+
+
+def test_buffers_of_another_gpu_are_refused():
+    far = _Elsewhere()
+    buf = G.Buffer((4, 64))
+    buf.dev_ptr, buf._release = far.alloc(buf.nbytes), far.free
+    node = G.Node(G.OpEnum.LEAF, data=buf)
+    for x in (ops.empty(far, (4, 64)), buf, node):
+        refused(norm_args(x=x, out=V(0x8000, (4, 64))), "cuda:1")
+    near = G.Buffer((4, 64))
+    near.dev_ptr = 0x1000
+    accepted(norm_args(x=near, out=V(0x8000, (4, 64))))
+
+
 # ---- RMS norm
 
 def test_norm_refuses_rows_whose_columns_pass_an_int():
