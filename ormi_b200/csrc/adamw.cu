@@ -254,7 +254,8 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_e4m3(const __grid_constant_
     if (t.vec && end - base == kChunk) {
         // A warp takes four blocks.  All their values are asked for at once, into shared memory (cp.async, every lane its own
         // pieces: nobody waits for anybody), so that 160 KB per SM are on their way without holding registers (134 million parameters:
-        // 379 us, 5710 GB/s; loads into registers, two blocks per SM: 457 us).
+        // 388 us, 5560 GB/s alone at 1965 MHz, 421 us in a loop, where the power limit leaves 1730 MHz; loads into registers, two
+        // blocks per SM: 457 us alone).
         constexpr int TURNS = kChunk / (kThreads / 32 * 128);
         __shared__ __align__(16) struct { float4 p[kThreads], g[kThreads]; uint32_t m[kThreads], v[kThreads]; } box[TURNS];
         auto first_of = [&](int k) { return base + (k * (kThreads / 32) + warp) * 128; };

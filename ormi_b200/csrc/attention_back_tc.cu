@@ -9,8 +9,8 @@
 //                  Blocks of a cluster share the heads and add their dK and dV up through each other's shared memory, in a
 //                  fixed order: with four heads in one block the longest block took most of the launch.
 // The price is that both compute the scores (7 products instead of 5).  2 x 4096 tokens, 16 heads over 4, causal, head_dim
-// 128: 428 us, 800 TFLOP/s counting the five.  Warp 0 loads, warp 1 issues the products, warp 2
-// fetches the queries' statistics (or blanks the keys behind key_len), and two warpgroups do the arithmetic, each half of the
+// 128: 430 us, 799 TFLOP/s counting the five, alone at 1965 MHz, 476 us in a loop at 1750 MHz.  Warp 0 loads, warp 1 issues the
+// products, warp 2 fetches the queries' statistics (or blanks the keys behind key_len), and two warpgroups do the arithmetic, each half of the
 // columns of a tile: while they work on the gradients of a tile the tensor cores multiply its probabilities and compute
 // the next scores, and the other way round.  (Tiles of 64, one warpgroup each, were slower: a product of 64 columns takes
 // the tensor cores as long as one of 128.)

@@ -6,7 +6,8 @@
 // turn, each through a ring of its own that one lane fills by TMA, so no warp waits for another until the end, where
 // their maxima, sums and outputs are joined through shared memory.  The parts of a head are joined by a second launch.
 // Three blocks of 64 KB are resident per SM: a warp's chain of products and exponentials is long, so warps count for more
-// than the depth of a ring (32 sequences over 8192 keys, 32 heads over 8: 6300 GB/s; two blocks of 96 KB 4950).
+// than the depth of a ring (32 sequences over 8192 keys, 32 heads over 8: 6370 GB/s in a loop, 5820 alone behind a fill of the
+// caches; two blocks of 96 KB 4950; lengths that differ from sequence to sequence 5900).
 #include <algorithm>
 
 #include "attention_tc.cuh"

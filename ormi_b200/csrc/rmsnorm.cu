@@ -166,8 +166,8 @@ __device__ __forceinline__ void weights(const void* w, int f32, int c0, int cols
 }
 
 // One row per block (of as many warps as the row needs), or per warp for narrow rows: the row is read once and stays in
-// registers, four pieces per thread, so that all its loads are in flight together (16384 x 4096 bf16 with residual: 85 us,
-// 6290 GB/s; three passes through the caches 406 us).
+// registers, four pieces per thread, so that all its loads are in flight together (16384 x 4096 bf16 with residual: 84 us,
+// 6360 GB/s; three passes through the caches 406 us).
 template <typename T, typename O, bool AL, bool WARP_ROW>
 __global__ void __launch_bounds__(WARP_ROW ? 256 : 1024) norm_row(NormParams p) {
     using P = Piece<T, AL>;
