@@ -534,10 +534,23 @@ struct CapturedStep {
     // bf16 copies of matmul operands in this graph's blocks: `reads` were made before the capture, so they have to be up to
     // date when a replay begins; `leaves` are what the context may use after a replay (made or kept up to date by it)
     std::vector<CopyOf> reads, leaves;
-    bool holds(const void* p) const {
-        for (auto& b : blocks) if ((const char*)p >= (const char*)b.first && (const char*)p < (const char*)b.first + b.second) return true;
-        return false;
+    using Ranges = std::vector<std::pair<const char*, const char*>>;      // sorted, apart
+    Ranges held, overwritten;                                             // `blocks`; and what a replay may write
+    void lay_out() {
+        for (auto& b : blocks) held.push_back({(const char*)b.first, (const char*)b.first + b.second});
+        Ranges all = held;
+        for (auto& w : writes) all.push_back({(const char*)w.first, (const char*)w.first + w.second});
+        std::sort(held.begin(), held.end());
+        std::sort(all.begin(), all.end());
+        for (auto& r : all)
+            if (overwritten.empty() || r.first > overwritten.back().second) overwritten.push_back(r);
+            else overwritten.back().second = std::max(overwritten.back().second, r.second);
     }
+    static bool meets(const Ranges& in, const void* p, size_t bytes) {
+        auto it = std::upper_bound(in.begin(), in.end(), (const char*)p, [](const char* a, const std::pair<const char*, const char*>& r) { return a < r.second; });
+        return it != in.end() && it->first < (const char*)p + bytes;
+    }
+    bool holds(const void* p) const { return meets(held, p, 1); }
 };
 
 // Whether the matrix at `src` went back to the pool: nothing is copied from there.
@@ -601,6 +614,7 @@ int ormi_b200_capture_end(ormi_b200_ctx* ctx, void** out_graph) {
         for (auto& kv : ctx->shadows) if (ctx->capture_blocks.count(kv.second.ptr)) step->leaves.push_back({kv.first, kv.second});
         step->writes.swap(ctx->capture_writes);
         step->reads.swap(ctx->capture_reads);
+        step->lay_out();
         ctx->capture_blocks.clear();
         ctx->capture_writes.clear();
         ctx->capture_reads.clear();
@@ -624,10 +638,14 @@ int ormi_b200_graph_launch(ormi_b200_ctx* ctx, void* graph) {
                 cvt_bf16(ctx, (const float*)r.src, r.copy.ld, r.copy.rows, r.copy.cols, r.copy.ptr);
         }
         ORMI_CUDA(cudaGraphLaunch(step.exec, ctx->stream));
-        // what the replay overwrites: matrices that copies were made of, and copies in its blocks
-        for (auto& w : step.writes) shadow_drop(ctx, w.first, w.second);
-        for (auto& b : step.blocks) shadow_drop(ctx, b.first, b.second);
-        for (auto it = ctx->shadows.begin(); it != ctx->shadows.end();) it = step.holds(it->second.ptr) ? ctx->shadows.erase(it) : std::next(it);
+        // what the replay overwrites: copies in its blocks (these stay the graph's), and matrices that copies were made of
+        std::vector<const void*> stale;
+        for (auto it = ctx->shadows.begin(); it != ctx->shadows.end();) {
+            if (step.holds(it->second.ptr)) { it = ctx->shadows.erase(it); continue; }
+            if (CapturedStep::meets(step.overwritten, it->first, it->second.src_bytes)) stale.push_back(it->first);
+            ++it;
+        }
+        for (auto* src : stale) shadow_drop(ctx, src, 1);
         for (auto& c : step.leaves) {
             if (gone(ctx, c.src)) continue;
             if (ctx->shadows.count(c.src)) shadow_drop(ctx, c.src, 1);
